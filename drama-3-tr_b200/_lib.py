@@ -19,6 +19,7 @@ HEADER = PKG_DIR.parent / "include" / "dm3.h"
 DM3_OK, DM3_EINVAL, DM3_ECUDA, DM3_ETIMEOUT, DM3_ENOSPACE = 0, 1, 2, 3, 4
 
 _p, _i, _i64, _sz, _u32p = ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_size_t, ctypes.POINTER(ctypes.c_uint32)
+_f32, _f64 = ctypes.c_float, ctypes.c_double
 
 # name -> (restype, argtypes), in the order of include/dm3.h
 SIGNATURES = {
@@ -63,6 +64,13 @@ SIGNATURES = {
                             _i, _p, _p, _p, _i, _i, _i, _p, _p, _sz, _p]),
     "dm3_moe_layer_ep": (_i, [_p, _i, _i, _i, _p, _i, _i, _i, _i, _p, _p, _i64, _p, _i64, _p, _i64, _p, _i64, _i, _p,
                               _p, _p, _p, _i, _p, _p, _p, _p, _p, _i, _i, _i, _p, _p, _sz, _p]),
+    "dm3_rope": (_i, [_p, _i, _i, _i, _i64, _i64, _p, _p, _i, _i, _f64, _p, _p]),
+    "dm3_kv_write": (_i, [_p, _i, _i64, _i64, _p, _i64, _i64, _p, _i64, _i64, _i, _i, _i, _p, _p, _p, _i64, _i, _i, _p,
+                          _p, _i64, _p, _p, _i64, _i, _i, _p, _i, _i, _f64, _p, _p, _p]),
+    "dm3_kv_read": (_i, [_p, _p, _i64, _p, _p, _i64, _i, _i, _i, _i, _p, _i64, _i, _i, _p, _i64, _p, _p, _p, _p]),
+    "dm3_paged_attention_workspace_bytes": (_sz, [_i, _i, _i, _i, _i, _i]),
+    "dm3_paged_attention": (_i, [_p, _i64, _i64, _i, _p, _p, _i64, _p, _p, _i64, _i, _i, _i, _i, _p, _i64, _i, _i, _p,
+                                 _f32, _i64, _p, _p, _p, _p, _sz, _p]),
     "dm3_last_launch_count": (_i, []),
 }
 

@@ -363,6 +363,74 @@ int dm3_moe_layer_ep(const void* x, int T, int H, int I, const void* router_w, i
                      int64_t* ids_out, void* w_out, int world, int rank, int tokens_per_rank, void* const* arenas,
                      void* workspace, size_t workspace_bytes, void* stream);
 
+/* ------------------------------------------------------------------ rotary positions and the paged cache */
+
+/*
+ * Rotary positions: y[t, h, :] = x[t, h, :] with its first rot values turned in pairs (a, b) by
+ * angle = positions[t] * inv_freq[i] (formed in 64 bits): a cos - b sin, b cos + a sin, times
+ * factor. Pair i is (2i, 2i + 1) when interleaved, else (i, i + rot / 2).
+ *   x          bf16 [T, heads, dim], token stride ts and head stride hs in elements
+ *   positions  device int64 [T]; inv_freq device double [rot / 2]
+ *   y          bf16 [T, heads, dim] contiguous
+ * rot even, 2 <= rot <= min(dim, 1024); any dim, strides and alignment (16-byte rows with
+ * rot % 16 == 0 take the wide path).
+ */
+int dm3_rope(const void* x, int T, int heads, int dim, int64_t ts, int64_t hs, const int64_t* positions,
+             const double* inv_freq, int rot, int interleaved, double factor, void* y, void* stream);
+
+/*
+ * A paged cache, as dm3_kv_write, dm3_kv_read and dm3_paged_attention take it:
+ *   k_cache, v_cache  [pages][kv_heads][page_size][dim], pages page_stride elements apart (16-byte aligned);
+ *                     bf16 when k_exp and v_exp are null, else e4m3 codes
+ *   k_exp, v_exp      int8 [pages][kv_heads][page_size], pages exp_stride apart: a row stands for
+ *                     code * 2^exp, exp = the smallest with amax <= 448 * 2^exp, in [-110, 119]
+ *   table             int32 [table_rows][per_row] page ids, rows table_stride apart: token t of row r lies
+ *                     in page table[r][t / page_size]
+ *   status            one device word; STATUS_BAD_PAGE (4) is or-ed in when a page id, row, position or
+ *                     length outside the cache or table was met (such tokens are skipped, never accessed)
+ * dim 64, 128, 192 or 256; page_size a multiple of 16.
+ */
+
+/*
+ * Writes T tokens' keys and values at (rows[t], positions[t]) (rows null: token t is row t), the keys
+ * rotated first when rot > 0, and the rotated queries to q_out (q_heads 0: none). A token with a
+ * negative row or position is padding: nothing is cached and its q_out rows are zeros. A quantised
+ * key is rotated, rounded to bf16, then coded; what is not finite becomes NaN. Two tokens of one
+ * call must not share a place. rot % 16 == 0; q, k, v bf16 [T, heads, dim] with 16-byte aligned rows.
+ */
+int dm3_kv_write(const void* q, int q_heads, int64_t q_ts, int64_t q_hs, const void* k, int64_t k_ts, int64_t k_hs,
+                 const void* v, int64_t v_ts, int64_t v_hs, int T, int kv_heads, int dim, const int64_t* rows,
+                 const int64_t* positions, const int32_t* table, int64_t table_stride, int table_rows, int per_row,
+                 void* k_cache, void* v_cache, int64_t page_stride, int8_t* k_exp, int8_t* v_exp, int64_t exp_stride,
+                 int pages, int page_size, const double* inv_freq, int rot, int interleaved, double factor, void* q_out,
+                 uint32_t* status, void* stream);
+
+/*
+ * Reads the first min(lengths[r], max_length) tokens of every row back as bf16
+ * [table_rows][kv_heads][max_length][dim], exactly the values the cache stands for, and zeros behind them.
+ */
+int dm3_kv_read(const void* k_cache, const void* v_cache, int64_t page_stride, const int8_t* k_exp, const int8_t* v_exp,
+                int64_t exp_stride, int pages, int page_size, int kv_heads, int dim, const int32_t* table,
+                int64_t table_stride, int table_rows, int per_row, const int64_t* lengths, int64_t max_length,
+                void* k_out, void* v_out, uint32_t* status, void* stream);
+
+/* Workspace bytes of dm3_paged_attention (its contents need no initial value). */
+size_t dm3_paged_attention_workspace_bytes(int rows, int q_heads, int kv_heads, int dim, int page_size, int per_row);
+
+/*
+ * One new token's attention for every row: out[r, h] = sum_t p_t v_t with p = softmax(scale * q[r, h] . k_t)
+ * over max(0, n - window) <= t < n = lengths[r] (window 0: all), query head h reading cache head
+ * h / (q_heads / kv_heads); lse[r, h] = log sum exp. A row that sees nothing gives zeros and -inf.
+ *   q    bf16 [rows, q_heads, dim], row stride q_rs and head stride q_hs (16-byte aligned rows)
+ *   out  bf16 [rows, q_heads, dim]; lse fp32 [rows, q_heads]
+ *   workspace  dm3_paged_attention_workspace_bytes, 256-byte aligned, not shared by calls that may overlap
+ */
+int dm3_paged_attention(const void* q, int64_t q_rs, int64_t q_hs, int q_heads, const void* k_cache, const void* v_cache,
+                        int64_t page_stride, const int8_t* k_exp, const int8_t* v_exp, int64_t exp_stride, int pages,
+                        int page_size, int kv_heads, int dim, const int32_t* table, int64_t table_stride, int rows,
+                        int per_row, const int64_t* lengths, float scale, int64_t window, void* out, float* lse,
+                        uint32_t* status, void* workspace, size_t workspace_bytes, void* stream);
+
 /* Number of kernels the last MoE / GEMV entry point launched on this host thread. */
 int dm3_last_launch_count(void);
 

@@ -1,0 +1,270 @@
+"""dm3::paged_attention against the 64-bit oracle, alone and in a decode loop with the cache."""
+
+import math
+
+import pytest
+import torch
+
+from oracle import kv_oracle
+from tests.kv_helpers import check_attention, held, paged, to_cuda
+
+pytestmark = pytest.mark.gpu
+BF = torch.bfloat16
+
+
+def _q(rows, heads, dim, seed, size=1.0):
+    return (torch.randn(rows, heads, dim, generator=torch.Generator().manual_seed(seed)) * size).to(BF)
+
+
+def _run(dm3, d, q, scale=None, window=0):
+    dev = to_cuda(d)
+    out, lse = dm3.ops.paged_attention(q.cuda(), *held(dev), dev["table"], dev["lengths"], dev["status"], scale, window)
+    assert int(dev["status"]) == 0
+    return out, lse
+
+
+@pytest.mark.parametrize("dim", [64, 128, 192, 256])
+@pytest.mark.parametrize("kv_heads,group", [(1, 1), (2, 8), (3, 4), (1, 16), (2, 5), (1, 24), (4, 1)])
+@pytest.mark.parametrize("quant", [False, True])
+def test_heads(dm3, dim, kv_heads, group, quant):
+    d = paged([130, 0, 1, 15, 16, 17, 77], kv_heads, dim, 48, quant, dim + group)
+    q = _q(7, kv_heads * group, dim, group, 2.0)
+    check_attention(*_run(dm3, d, q), d, q)
+
+
+@pytest.mark.parametrize("size", [16, 32, 80, 256])
+@pytest.mark.parametrize("quant", [False, True])
+@pytest.mark.parametrize("window", [0, 1, 16, 100, 5000])
+def test_lengths_pages_and_windows(dm3, size, quant, window):
+    lengths = [0, 1, 2, size - 1, size, size + 1, 333, 1024, 1500, 2049]
+    d = paged(lengths, 2, 128, size, quant, size + window, capacity=2500)
+    q = _q(len(lengths), 6, 128, window)
+    check_attention(*_run(dm3, d, q, 0.07, window), d, q, 0.07, window)
+
+
+@pytest.mark.parametrize("quant", [False, True])
+def test_long_row(dm3, quant):
+    d = paged([40003, 7], 1, 64, 64, quant, 3)
+    q = _q(2, 8, 64, 3)
+    check_attention(*_run(dm3, d, q), d, q)
+
+
+def test_nothing_to_see(dm3):
+    d = paged([0, 0, 0], 2, 64, 16, False, 1)
+    q = _q(3, 4, 64, 1)
+    out, lse = _run(dm3, d, q)
+    assert (out == 0).all() and (lse == -math.inf).all()
+    e = torch.zeros(0, 4, 64, dtype=BF, device="cuda")
+    dev = to_cuda(d)
+    out, lse = dm3.ops.paged_attention(e, *held(dev), dev["table"][:0], dev["lengths"][:0], dev["status"])
+    assert out.shape == (0, 4, 64) and lse.shape == (0, 4)
+    out, lse = dm3.ops.paged_attention(q.cuda(), *held(dev), dev["table"][:, :0], dev["lengths"], dev["status"])
+    assert (out == 0).all() and (lse == -math.inf).all() and int(dev["status"]) == 0
+
+
+@pytest.mark.parametrize("quant", [False, True])
+def test_sharp_and_shifted_logits(dm3, quant):
+    """One token far above the others, early or late; all logits equal; a large common offset; logits of both signs
+    whose exp leaves fp32's range; a negative and a zero scale; value rows of very different sizes."""
+    dim, n = 128, 300
+    base = paged([n] * 6, 1, dim, 32, False, 2)
+    k = base["k"].float()
+    row = lambda r, t: (int(base["table"][r, t // 32]), 0, t % 32)  # noqa: E731
+    q = _q(6, 8, dim, 5).float()
+    for r, t in ((0, 3), (1, n - 1)):
+        k[row(r, t)] = q[r, 0] * 3
+    for t in range(n):
+        k[row(2, t)] = k[row(2, 0)]
+        k[row(3, t)] = k[row(3, t)] + q[3, 1] * 5
+        k[row(4, t)] = k[row(4, t)] * 60
+    v = base["v"].float() * torch.exp2(torch.randint(-60, 40, base["v"].shape[:3], generator=torch.Generator().manual_seed(1)).float())[..., None]
+    base["k"], base["v"] = k.to(BF), v.to(BF)
+    if quant:
+        hole = base["k"].isnan().all(-1)
+        for name in ("k", "v"):
+            x, e = kv_oracle.quantise(base[name].nan_to_num(0.0))
+            base[name] = (x * torch.exp2(-e.double())[..., None]).float().to(torch.float8_e4m3fn)
+            base[name].view(torch.uint8)[hole] = 0x7F
+            base[name + "_exp"] = e
+    q = q.to(BF)
+    for scale in (None, 1.0, -0.3, 0.0):
+        check_attention(*_run(dm3, base, q, scale), base, q, scale)
+
+
+def test_queries_of_extreme_size(dm3):
+    """Queries near the ends of bf16's range: only the products with the scale have to be in range."""
+    for quant in (False, True):
+        d = paged([50, 33], 1, 64, 16, quant, 6)
+        for size in (2.0**100, 2.0**-100):
+            q = _q(2, 4, 64, 7, size)
+            check_attention(*_run(dm3, d, q, 1.0 / size), d, q, 1.0 / size)
+
+
+def test_bad_pages_and_lengths(dm3):
+    """Tokens of a page outside the cache are left out and reported, a length behind the table is cut and reported."""
+    for quant in (False, True):
+        d = paged([100, 64], 2, 64, 16, quant, 4)
+        q = _q(2, 4, 64, 4)
+        for page in (-1, d["k"].shape[0], 2**31 - 1):
+            d["table"][0, 2] = page
+            dev = to_cuda(d)
+            out, lse = dm3.ops.paged_attention(q.cuda(), *held(dev), dev["table"], dev["lengths"], dev["status"])
+            assert int(dev["status"]) == 4
+            check_attention(out, lse, d, q)
+        d = paged([100, 112], 2, 64, 16, quant, 4)
+        d["lengths"][1] = 1 << 41
+        dev = to_cuda(d)
+        out, lse = dm3.ops.paged_attention(q.cuda(), *held(dev), dev["table"], dev["lengths"], dev["status"])
+        assert int(dev["status"]) == 4
+        d["lengths"][1] = 112
+        check_attention(out, lse, d, q)
+        d["lengths"][1] = -5
+        out, lse = _run(dm3, d, q)
+        d["lengths"][1] = 0
+        check_attention(out, lse, d, q)
+
+
+def test_strided_queries_and_narrow_tables(dm3):
+    d = paged([70, 40, 12], 2, 64, 16, False, 9, capacity=400)
+    whole = _q(3, 12, 64, 2)
+    dev = to_cuda(d)
+    wd = whole.cuda()
+    for q, qd in ((whole[:, 2:6], wd[:, 2:6]), (whole[:, ::3], wd[:, ::3]), (whole[:, :1].expand(3, 4, 64), wd[:, :1].expand(3, 4, 64)),
+                  (whole.view(3, 24, 32)[:, 1:9].reshape(3, 4, 64), wd.view(3, 24, 32)[:, 1:9].reshape(3, 4, 64))):
+        for cols in (5, 9, 25):
+            out, lse = dm3.ops.paged_attention(qd, *held(dev), dev["table"][:, :cols], dev["lengths"], dev["status"])
+            check_attention(out, lse, d, q)
+    odd = torch.empty(3 * 4 * 64 + 1, dtype=BF, device="cuda")[1:].view(3, 4, 64).copy_(wd[:, :4])
+    out, lse = dm3.ops.paged_attention(odd, *held(dev), dev["table"], dev["lengths"], dev["status"])
+    check_attention(out, lse, d, whole[:, :4])
+    assert int(dev["status"]) == 0
+
+
+def test_same_answer_every_time(dm3):
+    d = paged([5000, 37, 2048, 900], 2, 128, 32, False, 12)
+    q = _q(4, 8, 128, 1)
+    first = _run(dm3, d, q)
+    for _ in range(5):
+        again = _run(dm3, d, q)
+        assert torch.equal(first[0], again[0]) and torch.equal(first[1], again[1])
+
+
+def test_shared_pages(dm3):
+    """Two rows whose tables share a prefix's pages."""
+    d = paged([64, 64], 1, 64, 16, True, 12)
+    d["table"][1, :2] = d["table"][0, :2]
+    q = _q(2, 2, 64, 1)
+    check_attention(*_run(dm3, d, q), d, q)
+
+
+@pytest.mark.parametrize("quant", [False, True])
+def test_frames_together(dm3, quant):
+    """Prompt reading (rotate, cache, read back), then decode frames (rotate, cache, attend) from one captured graph,
+    with pages reserved between replays, against the oracle on the same tokens."""
+    g = torch.Generator().manual_seed(20)
+    rows, kv, qh, dim, rot, size, layers = 2, 2, 8, 128, 32, 16, 2
+    prompt, frames = [37, 21], 30
+    rope = dm3.Rope(rot, 1e5)
+    cache = dm3.KVCache(layers, rows, 128, kv, dim, page_size=size, quantised=quant)
+    total = sum(prompt)
+    row = torch.cat([torch.full((n,), r) for r, n in enumerate(prompt)])
+    pos = torch.cat([torch.arange(n) for n in prompt])
+    hist = {(layer, r): ([], []) for layer in range(layers) for r in range(rows)}
+
+    def remember(layer, k, v, rows_, pos_):
+        kr = kv_oracle.rope(k, pos_, rope.inv_freq.cpu(), False, 1.0).to(BF)
+        for i, r in enumerate(rows_.tolist()):
+            for x, to in zip((kr[i], v[i]), hist[layer, r]):
+                to.append(kv_oracle.quantise(x)[0] if quant else x.double())
+
+    for r, n in enumerate(prompt):
+        cache.reserve(r, n)
+    for layer in range(layers):
+        qkv = torch.randn(total, qh + 2 * kv, dim, generator=g).to(BF)
+        q, k, v = qkv.cuda().split([qh, kv, kv], 1)
+        cache.write(layer, k, v, pos.cuda(), row.cuda(), q, rope)
+        remember(layer, *qkv.split([qh, kv, kv], 1)[1:], row, pos)
+        rk, rv = cache.read(layer, torch.tensor(prompt).cuda(), max(prompt))
+        for r, n in enumerate(prompt):
+            want = torch.stack(hist[layer, r][0], 1)
+            # a bf16 key may be the neighbour of the oracle's rounding; a quantised one is exact
+            assert (rk[r, :, :n].double().cpu() - want).abs().max() <= (0 if quant else want.abs().max() * 2.0**-7)
+            assert torch.equal(rv[r, :, :n].double().cpu(), torch.stack(hist[layer, r][1], 1))
+
+    position = torch.tensor(prompt, device="cuda")
+    inputs = [torch.zeros(rows, qh + 2 * kv, dim, dtype=BF, device="cuda") for _ in range(layers)]
+
+    def frame():
+        outs = []
+        lengths = position + 1
+        for layer in range(layers):
+            q, k, v = inputs[layer].split([qh, kv, kv], 1)
+            q = cache.write(layer, k, v, position, None, q, rope)
+            outs.append((q, *cache.attend(layer, q, lengths)))
+        return outs
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    for r, n in enumerate(prompt):
+        cache.reserve(r, n + 1)
+    with torch.cuda.stream(side):
+        frame()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = frame()
+    for f in range(frames):
+        for r, n in enumerate(prompt):
+            cache.reserve(r, n + f + 1)
+        now = torch.tensor([n + f for n in prompt])
+        position.copy_(now)
+        fresh = [torch.randn(rows, qh + 2 * kv, dim, generator=g).to(BF) for _ in range(layers)]
+        for to, x in zip(inputs, fresh):
+            to.copy_(x)
+        graph.replay()
+        torch.cuda.synchronize()
+        for layer in range(layers):
+            remember(layer, *fresh[layer].split([qh, kv, kv], 1)[1:], torch.arange(rows), now)
+            if f % 7 and f != frames - 1:
+                continue
+            q, out, lse = (x.double().cpu() for x in outs[layer])
+            for r in range(rows):
+                k, v = (torch.stack(x, 1) for x in hist[layer, r])
+                for h in range(qh):
+                    s = k[h // 4] @ q[r, h] * dim ** -0.5
+                    want = s.softmax(-1) @ v[h // 4]
+                    # a bf16 key off by one step moves a logit by 2^-7 of scale * sum |q k| at most (part of rot only);
+                    # that is the tolerance's larger part for the bf16 cache, the operators' own rounding for e4m3
+                    off = 0.0 if quant else float((q[r, h, :rot].abs() @ k[h // 4][:, :rot].abs().T).max()) * dim ** -0.5 * 2.0**-7
+                    spread = s.softmax(-1) @ v[h // 4].abs()
+                    assert ((out[r, h] - want).abs() <= want.abs() * 2.0**-8 + spread * (2 * off + 2.0**-10)).all()
+                    assert abs(float(lse[r, h] - s.logsumexp(-1))) <= off + 1e-4
+    assert cache.check() == 0
+    assert torch.equal(cache.table[0, :5].cpu() >= 0, torch.ones(5, dtype=torch.bool))
+
+
+def test_two_graphs_and_two_streams(dm3):
+    """Two captured graphs and eager calls on several streams, all in flight at once, keep apart."""
+    ds = [paged([900 + 50 * i, 333], 2, 64, 32, bool(i % 2), 30 + i) for i in range(3)]
+    qs = [_q(2, 8, 64, i) for i in range(3)]
+    dev = [(to_cuda(d), q.cuda()) for d, q in zip(ds, qs)]
+    call = lambda i: dm3.ops.paged_attention(dev[i][1], *held(dev[i][0]), dev[i][0]["table"], dev[i][0]["lengths"], dev[i][0]["status"])  # noqa: E731
+    want = [call(i) for i in range(3)]
+    torch.cuda.synchronize()
+    graphs, outs = [], []
+    for i in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(call(i))
+        graphs.append(g)
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    for _ in range(10):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                if i < 2:
+                    graphs[i].replay()
+                else:
+                    out2 = call(2)
+    torch.cuda.synchronize()
+    for got, w in zip([*outs, out2], want):
+        assert torch.equal(got[0], w[0]) and torch.equal(got[1], w[1])

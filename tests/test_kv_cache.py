@@ -1,0 +1,161 @@
+"""The paged cache and rotary positions without a GPU: the frequencies, the page bookkeeping, the oracle's
+quantiser against torch's own e4m3 conversion, shapes under tracing, and every refusal of the C entries and
+the ops (arguments are checked before any device work)."""
+
+import ctypes
+import math
+
+import pytest
+import torch
+
+from oracle import kv_oracle
+
+BF = torch.bfloat16
+P = ctypes.c_void_p(256)  # a non-null, aligned pointer that no refused call reads
+
+
+def test_oracle_quantiser_is_e4m3_of_a_power_of_two():
+    g = torch.Generator().manual_seed(3)
+    x = (torch.randn(40, 64, generator=g) * torch.exp2(torch.randint(-30, 30, (40, 1), generator=g).float())).to(BF)
+    x[3] = 0
+    x[4, 5] = math.inf
+    x[5, 6] = math.nan
+    v, e = kv_oracle.quantise(x)
+    scale = torch.exp2(e.double())[:, None]
+    ref = (x.double() / scale).float().to(torch.float8_e4m3fn).double() * scale
+    ref[~x.isfinite()] = math.nan
+    assert torch.equal(v.nan_to_num(7.0), ref.nan_to_num(7.0)) and int(e[3]) == 0
+    top = torch.where(x.isfinite(), x.double().abs(), 0.0).amax(-1)
+    busy = top > 0
+    assert (top[busy] <= 448 * scale[busy, 0]).all() and (top[busy] > 224 * scale[busy, 0]).all()
+    # a half step of e4m3 at most (2^-4 of the value, or half of the smallest code's step)
+    ok = x.isfinite()
+    assert ((v - x.double()).abs()[ok] <= torch.maximum(x.double().abs() / 16, 2.0**-10 * scale.expand_as(v))[ok]).all()
+
+
+def test_frequencies(dm3):
+    f, factor = dm3.rope_frequencies(64, 1e6)
+    assert f.dtype == torch.float64 and factor == 1.0 and f[0] == 1.0
+    assert torch.allclose(f, torch.tensor([1e6 ** (-2 * i / 64) for i in range(32)], dtype=torch.float64), rtol=1e-14)
+    lin, _ = dm3.rope_frequencies(64, 1e6, "linear", 4.0)
+    assert torch.equal(lin, f / 4)
+    ntk, _ = dm3.rope_frequencies(64, 1e6, "ntk", 4.0)
+    assert ntk[0] == 1.0 and abs(float(ntk[-1] / f[-1]) - 0.25) < 1e-12  # the slowest pair is slowed by stretch
+    yarn, factor = dm3.rope_frequencies(64, 1e6, "yarn", 4.0, 32768)
+    turns = 32768 * f / (2 * math.pi)
+    assert torch.equal(yarn[turns > 32], f[turns > 32]) and torch.equal(yarn[turns < 1], f[turns < 1] / 4)
+    assert ((yarn <= f) & (yarn >= f / 4)).all() and abs(factor - (0.1 * math.log(4) + 1)) < 1e-15
+    assert dm3.rope_frequencies(2, 100.0, "ntk", 2.0)[0].tolist() == [1.0]
+    for bad in (dict(rotary_dim=7), dict(rotary_dim=0), dict(rotary_dim=8, scaling="cubic"), dict(rotary_dim=8, base=0.0),
+                dict(rotary_dim=8, scaling="yarn", stretch=2.0), dict(rotary_dim=8, stretch=0.5)):
+        with pytest.raises(ValueError):
+            dm3.rope_frequencies(**bad)
+
+
+def test_pages_are_reserved_and_released(dm3):
+    c = dm3.KVCache(layers=2, rows=3, tokens_per_row=100, kv_heads=2, head_dim=64, page_size=16, pages=9, device="cpu")
+    assert c.pages_per_row == 7 and c.k.shape == (2, 9, 2, 16, 64) and c.k_exp is None
+    assert (c.table == -1).all()
+    c.reserve(0, 33)
+    first = c.table[0, :3].tolist()
+    c.reserve(0, 48)  # the third page has room
+    assert c.table[0, :4].tolist() == first + [-1]
+    c.reserve(1, 96)
+    assert len(set(first) | set(c.table[1, :6].tolist())) == 9
+    before = c.table.clone()
+    with pytest.raises(RuntimeError, match="free"):
+        c.reserve(2, 1)
+    with pytest.raises(RuntimeError, match="more than its 7 pages"):
+        c.reserve(0, 113)
+    assert torch.equal(c.table, before)
+    c.release(0)
+    assert (c.table[0] == -1).all()
+    c.reserve(2, 40)
+    assert sorted(c.table[2, :3].tolist()) == sorted(first)
+    c.reserve(2, 0)
+    for bad in (dict(page_size=24), dict(page_size=8), dict(head_dim=96), dict(kv_heads=0), dict(pages=0)):
+        with pytest.raises(ValueError):
+            dm3.KVCache(**{**dict(layers=1, rows=1, tokens_per_row=10, kv_heads=1, head_dim=64, device="cpu"), **bad})
+
+
+def _meta_cache(quant, pages=5, heads=2, size=16, dim=64, device="meta"):
+    k = torch.empty(pages, heads, size, dim, dtype=torch.float8_e4m3fn if quant else BF, device=device)
+    e = torch.empty(pages, heads, size, dtype=torch.int8, device=device) if quant else None
+    return k, torch.empty_like(k), e, None if e is None else torch.empty_like(e)
+
+
+def test_fake_impls_trace_on_meta(dm3):
+    m = dict(device="meta")
+    pos, inv = torch.empty(3, dtype=torch.int64, **m), torch.empty(16, dtype=torch.float64, **m)
+    table, status = torch.empty(3, 4, dtype=torch.int32, **m), torch.empty(1, dtype=torch.int32, **m)
+    x = torch.empty(3, 8, 64, dtype=BF, **m)
+    assert torch.ops.dm3.rope(x, pos, inv).shape == x.shape
+    for quant in (False, True):
+        c = _meta_cache(quant)
+        k = torch.empty(3, 2, 64, dtype=BF, **m)
+        assert torch.ops.dm3.kv_write(k, k, pos, table, *c, status).shape == (0,)
+        assert torch.ops.dm3.kv_write(k, k, pos, table, *c, status, None, x, inv).shape == x.shape
+        rk, rv = torch.ops.dm3.kv_read(*c, table, pos, 33, status)
+        assert rk.shape == rv.shape == (3, 2, 33, 64) and rk.dtype == BF
+        out, lse = torch.ops.dm3.paged_attention(x, *c, table, pos, status)
+        assert out.shape == x.shape and out.dtype == BF and lse.shape == (3, 8) and lse.dtype == torch.float32
+
+
+def test_ops_refuse_cpu_tensors(dm3):
+    with pytest.raises(RuntimeError, match="CUDA tensors only"):
+        dm3.ops.rope(torch.zeros(1, 1, 64, dtype=BF), torch.zeros(1, dtype=torch.int64), torch.ones(32, dtype=torch.float64))
+    c = dm3.KVCache(1, 1, 16, 1, 64, device="cpu")
+    n = torch.ones(1, dtype=torch.int64)
+    with pytest.raises(RuntimeError, match="CUDA tensors only"):
+        c.attend(0, torch.zeros(1, 1, 64, dtype=BF), n)
+    with pytest.raises(RuntimeError, match="CUDA tensors only"):
+        c.read(0, n, 4)
+    with pytest.raises(RuntimeError, match="CUDA tensors only"):
+        c.write(0, torch.zeros(1, 1, 64, dtype=BF), torch.zeros(1, 1, 64, dtype=BF), n)
+
+
+# What each C entry is called with, by name; a refusal test changes one of them.
+_CACHE = dict(k_cache=P, v_cache=P, page_stride=2 * 16 * 64, k_exp=None, v_exp=None, exp_stride=0, pages=5, page_size=16)
+_TABLE = dict(table=P, table_stride=4, table_rows=3, per_row=4)
+CALLS = {
+    "dm3_rope": dict(x=P, T=3, heads=2, dim=64, ts=128, hs=64, positions=P, inv_freq=P, rot=32, interleaved=0, factor=1.0, y=P, stream=None),
+    "dm3_kv_write": dict(q=P, q_heads=4, q_ts=256, q_hs=64, k=P, k_ts=128, k_hs=64, v=P, v_ts=128, v_hs=64, T=3, kv_heads=2, dim=64, rows=None,
+                         positions=P, **_TABLE, **_CACHE, inv_freq=P, rot=32, interleaved=0, factor=1.0, q_out=P, status=P, stream=None),
+    "dm3_kv_read": dict(**_CACHE, kv_heads=2, dim=64, **_TABLE, lengths=P, max_length=40, k_out=P, v_out=P, status=P, stream=None),
+    "dm3_paged_attention": dict(q=P, q_rs=256, q_hs=64, q_heads=4, **_CACHE, kv_heads=2, dim=64, **_TABLE, lengths=P, scale=0.125, window=0, out=P,
+                                lse=P, status=P, workspace=P, workspace_bytes=1 << 30, stream=None),
+}
+ODD = ctypes.c_void_p(264)  # not on 16 bytes
+BAD_CACHE = [dict(dim=96), dict(dim=0), dict(kv_heads=0), dict(page_size=8), dict(page_size=40), dict(pages=0), dict(k_cache=None), dict(v_cache=None),
+             dict(k_cache=ODD), dict(v_cache=ODD), dict(status=None), dict(k_exp=P), dict(v_exp=P), dict(page_stride=2 * 16 * 64 - 8),
+             dict(page_stride=2 * 16 * 64 + 4), dict(k_exp=P, v_exp=P, exp_stride=31, page_stride=2 * 16 * 64), dict(table=None),
+             dict(table_stride=3), dict(table_rows=-1), dict(per_row=-1)]
+BAD = {
+    "dm3_rope": [dict(T=-1), dict(heads=0), dict(dim=0), dict(rot=0), dict(rot=7), dict(rot=66), dict(rot=2048, dim=4096), dict(x=None),
+                 dict(positions=None), dict(inv_freq=None), dict(y=None), dict(heads=1 << 20)],
+    "dm3_kv_write": BAD_CACHE + [dict(T=-1), dict(q_heads=-1), dict(rot=24), dict(rot=80), dict(inv_freq=None), dict(k=None), dict(v=None),
+                                 dict(positions=None), dict(q=None), dict(q_out=None), dict(k=ODD), dict(q=ODD), dict(v_ts=129), dict(q_out=ODD)],
+    "dm3_kv_read": BAD_CACHE + [dict(max_length=-1), dict(lengths=None), dict(k_out=None), dict(v_out=ODD), dict(table_rows=40000)],
+    "dm3_paged_attention": BAD_CACHE + [dict(q_heads=3), dict(q_heads=1), dict(q_heads=0), dict(window=-1), dict(scale=math.nan),
+                                        dict(scale=math.inf), dict(q=None), dict(lengths=None), dict(out=None), dict(lse=None), dict(q=ODD),
+                                        dict(q_rs=250), dict(out=ODD), dict(table_rows=70000)],
+}
+
+
+@pytest.mark.parametrize("name", CALLS)
+def test_c_entries_refuse(dm3, name):
+    lib = dm3._lib.load()
+    for change in BAD[name]:
+        args = {**CALLS[name], **change}
+        rc = getattr(lib, name)(*args.values())
+        assert rc == dm3._lib.DM3_EINVAL, (name, change, rc)
+        assert lib.dm3_last_error(), (name, change)
+
+
+@pytest.mark.parametrize("name", CALLS)
+def test_c_entries_with_nothing_to_do(dm3, name):
+    """No tokens or no rows: done without a launch."""
+    lib = dm3._lib.load()
+    change = dict(T=0) if "T" in CALLS[name] else dict(table_rows=0, table=None)
+    assert getattr(lib, name)(*{**CALLS[name], **change}.values()) == 0
+    assert lib.dm3_last_launch_count() == 0
