@@ -123,6 +123,28 @@ bool tensor_map_3d(CUtensorMap* out, const void* base, uint64_t d0, uint64_t d1,
   return true;
 }
 
+bool tensor_map_boxes(CUtensorMap* out, const void* base, uint64_t row_bytes, uint64_t rows, uint64_t pages,
+                      uint64_t page_stride, uint32_t box_bytes, uint32_t box_rows) {
+  EncodeTiled enc = encoder();
+  if (!enc) {
+    set_error("cuTensorMapEncodeTiled is not available from the driver");
+    return false;
+  }
+  const cuuint64_t dims[3] = {row_bytes, rows, pages};
+  const cuuint64_t strides[2] = {row_bytes, page_stride};
+  const cuuint32_t box[3] = {box_bytes, box_rows, 1};
+  const cuuint32_t elem[3] = {1, 1, 1};
+  const CUresult r = enc(out, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void*>(base), dims, strides, box, elem,
+                         CU_TENSOR_MAP_INTERLEAVE_NONE,
+                         box_bytes == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
+                         CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) {
+    set_error("cuTensorMapEncodeTiled failed with code " + std::to_string(static_cast<int>(r)));
+    return false;
+  }
+  return true;
+}
+
 }  // namespace dm3
 
 extern "C" const char* dm3_last_error(void) { return dm3::g_error.c_str(); }
@@ -134,7 +156,7 @@ extern "C" int dm3_last_launch_count(void) { return dm3::g_launches; }
 extern "C" int dm3_set_wait_limit_ns(uint64_t ns) {
   if (ns == 0) return dm3::set_error("the wait limit must be at least 1 ns"), 1;
   int (*setters[])(uint64_t) = {dm3::wait_limit_gemm, dm3::wait_limit_gemv, dm3::wait_limit_gemv_tc, dm3::wait_limit_moe_decode,
-                                dm3::wait_limit_moe_prefill};
+                                dm3::wait_limit_moe_prefill, dm3::wait_limit_attention};
   for (auto fn : setters) {
     const int err = fn(ns);
     if (err != 0)

@@ -35,6 +35,7 @@
 #include "dm3_common.cuh"
 #include "dm3_internal.h"
 #include "dm3_kv.cuh"
+#include "dm3_tc.cuh"
 
 namespace dm3 {
 namespace attn {
@@ -80,17 +81,6 @@ __device__ __forceinline__ Span row_span(const Params& p, int row) {
   s.chunk = (s.tiles + p.splits - 1) / p.splits;
   if (s.chunk < p.min_tiles) s.chunk = p.min_tiles;
   return s;
-}
-
-__device__ __forceinline__ uint4 ld16(const uint8_t* p) {
-  uint4 r;
-  asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "l"(p));
-  return r;
-}
-__device__ __forceinline__ uint2 ld8(const uint8_t* p) {
-  uint2 r;
-  asm volatile("ld.global.L1::no_allocate.v2.u32 {%0, %1}, [%2];" : "=r"(r.x), "=r"(r.y) : "l"(p));
-  return r;
 }
 
 // D[16x8] += A[16x16] B[16x8], fp32 accumulators; lane (g = lane / 4, q = lane % 4) holds A rows g, g + 8 at columns
@@ -139,27 +129,69 @@ __device__ __forceinline__ uint32_t pack_half(float lo, float hi) {
 // kNT: tiles of 8 query heads; kU: token tiles of one step of a warp.
 template <int kDim, bool kQuant, int kNT, int kU>
 struct Shape {
-  static constexpr int kRow = kDim * (kQuant ? 1 : 2);                  // bytes of a cache row
-  static constexpr int kKP = kRow / 64;                                 // 16-byte loads of a key row a lane
-  static constexpr int kVB = kQuant && kDim % 128 ? 8 : 16;             // bytes of one value load a lane
-  static constexpr int kVP = kRow / (8 * kVB), kVW = kVB / 4;           // loads a row, words a load
-  static constexpr int kE = kQuant ? kVB : kVB / 2;                     // values a load
+  static constexpr int kRow = kDim * (kQuant ? 1 : 2);         // bytes of a cache row
+  static constexpr int kKP = kRow / 64;                        // 16-byte copies of a key row a lane
+  static constexpr int kVB = kQuant && kDim % 128 ? 8 : 16;    // bytes of one value copy a lane
+  static constexpr int kVP = kRow / (8 * kVB), kVW = kVB / 4;  // copies a row, words a copy
+  static constexpr int kE = kQuant ? kVB : kVB / 2;            // values a copy
   static constexpr int kHeads = 8 * kNT;
-  static constexpr bool kSharedQ = kRow == 512;  // the registers of keys and values leave none for the queries
-  static constexpr int kPitch = 2 * kDim + 8;  // floats of a head pair in shared memory (8: no bank conflicts)
+  // A tile arrives as boxes of kBox bytes x 16 tokens, swizzled: 16-byte chunk c of token t is at chunk
+  // c ^ (t % 8) of its 128 bytes (c ^ (t / 2 % 4) of 64).
+  static constexpr int kBox = kRow % 128 ? 64 : 128, kBoxes = kRow / kBox;
+  static constexpr int kTileBytes = kTile * kRow;
+  // Shared memory: a ring of kRing units a warp (a step's keys, its values, the next step's keys, ...), the
+  // queries, the units' exponents, ranges and barriers, the join's maxima and sums. The join reuses the ring.
+  static constexpr int kUnit = kU * kTileBytes;
+  static constexpr int kQBytes = kNT * kDim * 16;  // 8 * kNT heads of kDim 16-bit values
+  static constexpr int kSide = (kQuant ? kU * 32 : 0) + kU * 4 + 8 + 4;  // a unit's exponents, ranges and barrier
+  static constexpr int kStats = (2 * kWarps + 1) * kHeads * 4;
+  // Two CTAs an SM: few warps with much to do at once did better than more of them with smaller steps and fewer
+  // registers (96 ragged rows, 16 heads a cache head, e4m3: 74.6 us; three CTAs and half the step 80.6, four 88.6)
+  static constexpr int kRoom = 112 * 1024 - kQBytes - kStats - 1024;  // 1024: aligning the ring
+  static constexpr int kFit = kRoom / kWarps / (kUnit + kSide), kRing = kFit < 6 ? kFit : 6;
+  static constexpr int kPitch = 2 * kDim + 8;  // floats of a head pair in the join (8: no bank conflicts)
+  static constexpr int kRingBytes = kWarps * kRing * kUnit;
+  static constexpr int kShared = 1024 + kRingBytes + kQBytes + kWarps * kRing * kSide + kStats;
+  static_assert(kRing >= 2 && kWarps * kNT * 4 * kPitch * 4 <= kRingBytes, "the ring holds two units and the join");
 };
+// The token that lane group lr's rows of a tile hold (and + 8): with it, the eight lanes of every 16-byte shared
+// memory access, of keys (two lane groups, four chunks) as of values (two chunks, four tokens), fall on
+// different chunks of 128-byte boxes.
+template <int kBox>
+__device__ __forceinline__ int token_of(int lr) {
+  return kBox == 128 ? ((lr ^ lr >> 2) & 1) << 2 | (lr & 2) | lr >> 2 : lr;
+}
 
 template <int kDim, bool kQuant, int kNT, int kU>
-__global__ void __launch_bounds__(kWarps * 32) attend_kernel(const __grid_constant__ Params p) {
+__global__ void __launch_bounds__(kWarps * 32, 2)
+    attend_kernel(const __grid_constant__ Params p, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap) {
   using C = Shape<kDim, kQuant, kNT, kU>;
-  __shared__ __align__(16) float s_o[kWarps][kNT * 4][C::kPitch];
-  __shared__ uint4 s_q[C::kSharedQ ? kNT * C::kKP : 1][32];
-  __shared__ float s_m[kWarps][C::kHeads], s_l[kWarps][C::kHeads];
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* const smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
+  uint4* const s_q = reinterpret_cast<uint4*>(smem + C::kRingBytes);  // [kNT][kDim / 32][32 lanes]
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, lr = lane >> 2, lc = lane & 3;
+  uint8_t* side = smem + C::kRingBytes + C::kQBytes;
+  uint8_t(*const s_exp)[kU][32] = reinterpret_cast<uint8_t(*)[kU][32]>(side) + (kQuant ? warp * C::kRing : 0);  // keys' 16, values' 16
+  side += kQuant ? kWarps * C::kRing * kU * 32 : 0;
+  uint64_t* const full = reinterpret_cast<uint64_t*>(side) + warp * C::kRing;
+  side += kWarps * C::kRing * 8;
+  int(*const s_range)[kU] = reinterpret_cast<int(*)[kU]>(side) + warp * C::kRing;  // rows of a tile that are seen: from | to << 8
+  side += kWarps * C::kRing * kU * 4;
+  float(*const s_m)[C::kHeads] = reinterpret_cast<float(*)[C::kHeads]>(side);
+  float(*const s_l)[C::kHeads] = s_m + kWarps;
+  float* const s_qs = s_m[2 * kWarps];
+  if (lane == 0) {
+#pragma unroll
+    for (int i = 0; i < C::kRing; ++i) mbar_init(&full[i], kU);
+    fence_mbar_init();
+  }
+  __syncwarp();
+
   const int split = blockIdx.x, kvh = blockIdx.y / p.head_tiles, ht = blockIdx.y % p.head_tiles, row = blockIdx.z;
   const int h0 = ht * C::kHeads;  // first head of the group
   griddep_launch();
   griddep_wait();
+  fence_proxy_async();  // the cache's rows may have been written just before; the copies read them
   const Span sp = row_span(p, row);
   const int64_t begin = split * sp.chunk;  // tiles of this CTA, counted from sp.tile0
   const int64_t end = begin + sp.chunk < sp.tiles ? begin + sp.chunk : sp.tiles;
@@ -174,209 +206,223 @@ __global__ void __launch_bounds__(kWarps * 32) attend_kernel(const __grid_consta
     return;
   }
 
-  // queries as B operands, the permutation of dim that 16-byte key loads give
-  uint32_t qf[kNT][C::kSharedQ ? 1 : kDim / 8];
-  float qs[kNT][2];  // logit scale of the lane's two heads of each tile
-#pragma unroll
-  for (int nt = 0; nt < kNT; ++nt) {
-    const int h = h0 + nt * 8 + lr;
-    const __nv_bfloat16* src = p.q + row * p.q_rs + static_cast<int64_t>(kvh * p.group + h) * p.q_hs;
-    const bool on = h < p.group;
-    if (C::kSharedQ) {
-      for (int j = warp; j < C::kKP; j += kWarps)
-        s_q[nt * C::kKP + j][lane] = on ? *reinterpret_cast<const uint4*>(src + j * 32 + lc * 8) : make_uint4(0, 0, 0, 0);
-      qs[nt][0] = qs[nt][1] = p.scale_log2;
-    } else if (!kQuant) {
-#pragma unroll
-      for (int j = 0; j < C::kKP; ++j) {
-        const uint4 w = on ? *reinterpret_cast<const uint4*>(src + j * 32 + lc * 8) : make_uint4(0, 0, 0, 0);
-        qf[nt][4 * j] = w.x, qf[nt][4 * j + 1] = w.y, qf[nt][4 * j + 2] = w.z, qf[nt][4 * j + 3] = w.w;
+  // A warp's steps: kU tiles each, warps in turn. Lane i of a block of 32 tiles knows where the block's tile i lies,
+  // and asks for it.
+  constexpr int kBlock = 32 / kU;  // steps a block
+  int steps = static_cast<int>((end - begin - warp * kU + kWarps * kU - 1) / (kWarps * kU));  // 0 where fewer tiles than warps
+  const int per_page = p.c.page_size / kTile;
+  int page, y, range;  // y: first row of the tile in its page
+  auto find = [&](int step0) {
+    const int64_t t = begin + (static_cast<int64_t>(step0 + lane / kU) * kWarps + warp) * kU + lane % kU;
+    int tile = 0;
+    page = 0, range = 0;
+    if (t < end) {
+      const int64_t g = sp.tile0 + t, nth = g / per_page, t0 = g * kTile;
+      tile = static_cast<int>(g - nth * per_page);
+      page = p.c.table[row * p.c.table_stride + nth];
+      if (page < 0 || page >= p.c.pages) {
+        page = 0;
+        kv::set_status(p.c.status, STATUS_BAD_PAGE);
+      } else {
+        range = (sp.first > t0 ? static_cast<int>(sp.first - t0) : 0) | (sp.n - t0 < kTile ? static_cast<int>(sp.n - t0) : kTile) << 8;
       }
-      qs[nt][0] = qs[nt][1] = p.scale_log2;
-    } else {
-      uint32_t raw[kDim / 8];
+    }
+    y = kvh * p.c.page_size + tile * kTile;
+  };
+  find(0);
+
+  uint8_t* const ring = smem + warp * C::kRing * C::kUnit;
+  auto ask = [&](bool keys, int step, int slot) {
+    if (step >= steps) return;
+    if (keys && step % kBlock == 0 && step > 0) find(step);
+    const int u = lane - (step % kBlock) * kU;
+    if (u >= 0 && u < kU) {
+      uint8_t* const to = ring + slot * C::kUnit + u * C::kTileBytes;
+      s_range[slot][u] = range;
+      mbar_arrive_expect_tx(&full[slot], C::kTileBytes + (kQuant && keys ? 32 : 0));
+#pragma unroll
+      for (int b = 0; b < C::kBoxes; ++b)
+        tc::tma_load_3d(to + b * kTile * C::kBox, keys ? &kmap : &vmap, b * C::kBox, y, page, &full[slot]);
+      if (kQuant && keys) {
+        const int64_t x = page * p.c.exp_stride + y;
+        bulk_g2s(s_exp[slot][u], p.c.k_exp + x, 16, &full[slot]);
+        bulk_g2s(s_exp[slot][u] + 16, p.c.v_exp + x, 16, &full[slot]);
+      }
+    }
+  };
+#pragma unroll
+  for (int i = 0; i < C::kRing; ++i) ask(!(i & 1), i / 2, i);
+
+  // Queries as B operands, in the permutation of dim that 16-byte key copies give; warp nt prepares tile nt.
+  if (warp < kNT) {
+    const int h = h0 + warp * 8 + lr;
+    const __nv_bfloat16* src = p.q + row * p.q_rs + static_cast<int64_t>(kvh * p.group + h) * p.q_hs;
+    uint4 w[kDim / 32];
+#pragma unroll
+    for (int j = 0; j < kDim / 32; ++j) {
+      const int d = kQuant ? j / 2 * 64 + lc * 16 + j % 2 * 8 : j * 32 + lc * 8;
+      w[j] = h < p.group ? *reinterpret_cast<const uint4*>(src + d) : make_uint4(0, 0, 0, 0);
+    }
+    float qs = p.scale_log2;  // logit scale of head h
+    if (kQuant) {
       uint32_t top = 0;  // the largest magnitude's bits
+      auto mag = [](uint32_t x) { return max(x << 16 & 0x7fffffffu, x & 0x7fff0000u); };
 #pragma unroll
-      for (int j = 0; j < C::kKP; ++j)
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const uint4 w = on ? *reinterpret_cast<const uint4*>(src + j * 64 + lc * 16 + i * 8) : make_uint4(0, 0, 0, 0);
-          const uint32_t x[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            raw[j * 8 + i * 4 + k] = x[k];
-            top = max(top, max(x[k] << 16 & 0x7fffffffu, x[k] & 0x7fff0000u));
-          }
-        }
+      for (int j = 0; j < kDim / 32; ++j) top = max(top, max(max(mag(w[j].x), mag(w[j].y)), max(mag(w[j].z), mag(w[j].w))));
       top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
       top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
       const int e = min(max(static_cast<int>(top >> 23) - 127, -112), 126) - 14;  // 2^-e puts the largest in [2^14, 2^15)
       const float up = exp2i(-e);
+      auto half = [up](uint32_t x) { return pack_half(__uint_as_float(x << 16) * up, __uint_as_float(x & 0xffff0000u) * up); };
 #pragma unroll
-      for (int i = 0; i < kDim / 8; ++i)
-        qf[nt][i] = pack_half(__uint_as_float(raw[i] << 16) * up, __uint_as_float(raw[i] & 0xffff0000u) * up);
-      const float down = p.scale_log2 * exp2i(e);  // of head lr; the accumulators' heads are 2 * lc and 2 * lc + 1
-      qs[nt][0] = __shfl_sync(0xffffffffu, down, (2 * lc) * 4);
-      qs[nt][1] = __shfl_sync(0xffffffffu, down, (2 * lc + 1) * 4);
+      for (int j = 0; j < kDim / 32; ++j) w[j] = make_uint4(half(w[j].x), half(w[j].y), half(w[j].z), half(w[j].w));
+      qs *= exp2i(e);
     }
+#pragma unroll
+    for (int j = 0; j < kDim / 32; ++j) s_q[(warp * (kDim / 32) + j) * 32 + lane] = w[j];
+    if (lc == 0) s_qs[warp * 8 + lr] = qs;
   }
-
-  if (C::kSharedQ) __syncthreads();
-
-  // a warp's steps: kU tiles each, warps in turn; lane i of a block of 32 knows the page of the block's tile i
-  constexpr int kBlock = 32 / kU;  // steps a block
-  const int steps = static_cast<int>((end - begin + kWarps * kU - 1) / (kWarps * kU));
-  const int per_page = p.c.page_size / kTile;
-  int pg, off;  // page (-1: not a tile of this CTA, or a bad page) and tile in the page
-  auto find = [&](int step0, int& page, int& tile) {
-    const int64_t t = begin + (static_cast<int64_t>(step0 + lane / kU) * kWarps + warp) * kU + lane % kU;
-    page = -1, tile = 0;
-    if (t < end) {
-      const int64_t g = sp.tile0 + t;
-      const int64_t nth = g / per_page;
-      tile = static_cast<int>(g - nth * per_page);
-      page = p.c.table[row * p.c.table_stride + nth];
-      if (page < 0 || page >= p.c.pages) {
-        page = -1;
-        kv::set_status(p.c.status, STATUS_BAD_PAGE);
-      }
-    }
-  };
-  int next_pg, next_off;
-  find(0, pg, off);
-  find(kBlock, next_pg, next_off);
-
-  const uint8_t* const kbase = static_cast<const uint8_t*>(p.c.k) + lr * C::kRow + lc * 16;
-  const uint8_t* const vbase = static_cast<const uint8_t*>(p.c.v) + lc * 2 * C::kRow + lr * C::kVB;
-  uint4 k[kU][2][C::kKP];
-  uint32_t v[kU][4][C::kVP][C::kVW];
-  int ek[kU][2], ev[kU][2];
-  int64_t at[kU];  // byte offset of a tile's rows in either buffer
-  int lo[kU], hi[kU];  // rows of the tile that are seen
-  auto load_k = [&](int step) {
-    if (step % kBlock == 0 && step > 0) {
-      pg = next_pg, off = next_off;
-      find(step + kBlock, next_pg, next_off);
-    }
-#pragma unroll
-    for (int u = 0; u < kU; ++u) {
-      const int from = (step % kBlock) * kU + u;
-      const int page = __shfl_sync(0xffffffffu, pg, from), tile = __shfl_sync(0xffffffffu, off, from);
-      const int64_t r = static_cast<int64_t>(kvh) * p.c.page_size + tile * kTile, pp = page < 0 ? 0 : page;
-      at[u] = (pp * p.c.page_stride + r * kDim) * (kQuant ? 1 : 2);
-      const int64_t t0 = (sp.tile0 + begin + (static_cast<int64_t>(step) * kWarps + warp) * kU + u) * kTile;
-      lo[u] = sp.first > t0 ? static_cast<int>(sp.first - t0) : 0;
-      hi[u] = page < 0 ? 0 : sp.n - t0 < kTile ? static_cast<int>(sp.n - t0) : kTile;
-#pragma unroll
-      for (int j = 0; j < C::kKP; ++j) {
-        k[u][0][j] = ld16(kbase + at[u] + j * 64);
-        k[u][1][j] = ld16(kbase + at[u] + j * 64 + 8 * C::kRow);
-      }
-      if (kQuant) {
-        const int64_t x = pp * p.c.exp_stride + r + lr;
-        ek[u][0] = p.c.k_exp[x], ek[u][1] = p.c.k_exp[x + 8];
-        ev[u][0] = p.c.v_exp[x], ev[u][1] = p.c.v_exp[x + 8];
-      }
-    }
-  };
-  load_k(0);
+  __syncthreads();
 
   float o[kNT][kDim / 16][4];
-  float m[kNT][2], l[kNT][2];  // of the lane's two heads a tile: m the same in all lanes of a head, l a lane's part
+  // Of the lane's two heads a tile: the maximum m (the same in all lanes of a head), what is subtracted (m, or 0
+  // before any logit was seen, less the lift), and a lane's part of l.
+  float m[kNT][2], sub[kNT][2], l[kNT][2], qs[kNT][2];
 #pragma unroll
   for (int nt = 0; nt < kNT; ++nt) {
 #pragma unroll
     for (int i = 0; i < kDim / 16; ++i)
 #pragma unroll
       for (int j = 0; j < 4; ++j) o[nt][i][j] = 0.f;
-    m[nt][0] = m[nt][1] = -INFINITY;
-    l[nt][0] = l[nt][1] = 0.f;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) m[nt][h] = -INFINITY, sub[nt][h] = 0.f, l[nt][h] = 0.f, qs[nt][h] = s_qs[nt * 8 + 2 * lc + h];
   }
 
+  const int tok = token_of<C::kBox>(lr), sw = C::kBox == 128 ? tok : tok >> 1;  // the lane's token of a key tile, its swizzle
+  int vtok[2];                                                                    // its tokens of a value tile (and + 8)
+#pragma unroll
+  for (int i = 0; i < 2; ++i) vtok[i] = token_of<C::kBox>(2 * lc + i);
+  int slot = 0;
+  uint32_t parity = 0;
+  // The unit in the current slot has landed; when the wait ran out, no more are asked for.
+  auto landed = [&](int step) {
+    if (__any_sync(0xffffffffu, !mbar_wait(&full[slot], parity))) {
+      if (lane == 0) kv::set_status(p.c.status, STATUS_TIMEOUT);
+      steps = min(steps, step + (C::kRing + 1) / 2);
+    }
+  };
+  auto next_slot = [&] {
+    if (++slot == C::kRing) slot = 0, parity ^= 1;
+  };
   for (int step = 0; step < steps; ++step) {
-    // this step's values start loading, then the keys' product
+    landed(step);
+    const uint8_t* unit = ring + slot * C::kUnit;
+    // a product takes the sum of the one before 25 cycles later: two sums side by side where a step has but one tile
+    constexpr int kChains = kU * kNT == 1 ? 2 : 1;
+    float s[kU][kNT][4], part[kChains][kU][kNT][4];
 #pragma unroll
-    for (int u = 0; u < kU; ++u)
+    for (int i = 0; i < kChains; ++i)
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
+      for (int u = 0; u < kU; ++u)
 #pragma unroll
-        for (int j = 0; j < C::kVP; ++j) {
-          const uint8_t* src = vbase + at[u] + ((i & 1) + (i >> 1) * 8) * C::kRow + j * 8 * C::kVB;
-          if (C::kVB == 16) {
-            const uint4 w = ld16(src);
-            v[u][i][j][0] = w.x, v[u][i][j][1] = w.y, v[u][i][j][C::kVW - 2] = w.z, v[u][i][j][C::kVW - 1] = w.w;
-          } else {
-            const uint2 w = ld8(src);
-            v[u][i][j][0] = w.x, v[u][i][j][1] = w.y;
-          }
-        }
-    float s[kU][kNT][4];
+        for (int nt = 0; nt < kNT; ++nt)
 #pragma unroll
-    for (int u = 0; u < kU; ++u) {
+          for (int j = 0; j < 4; ++j) part[i][u][nt][j] = 0.f;
+    auto key = [&](int u, int half, int j) {
+      constexpr int kIn = C::kBox / 64;  // passes a box
+      return *reinterpret_cast<const uint4*>(unit + u * C::kTileBytes + (j / kIn * kTile + tok + half * 8) * C::kBox +
+                                             (((j % kIn) * 4 + lc) ^ (C::kBox == 128 ? sw : sw & 3)) * 16);
+    };
 #pragma unroll
-      for (int nt = 0; nt < kNT; ++nt)
+    for (int j = 0; j < C::kKP; ++j) {
+      if (!kQuant) {
+        uint4 w[kNT];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) s[u][nt][j] = 0.f;
+        for (int nt = 0; nt < kNT; ++nt) w[nt] = s_q[(nt * (kDim / 32) + j) * 32 + lane];
 #pragma unroll
-      for (int j = 0; j < C::kKP; ++j) {
-        const uint32_t a[4] = {k[u][0][j].x, k[u][0][j].y, k[u][0][j].z, k[u][0][j].w};
-        const uint32_t b[4] = {k[u][1][j].x, k[u][1][j].y, k[u][1][j].z, k[u][1][j].w};
-        if (!kQuant) {
+        for (int u = 0; u < kU; ++u) {
+          const uint4 a = key(u, 0, j), b = key(u, 1, j);
 #pragma unroll
           for (int nt = 0; nt < kNT; ++nt) {
-            const uint4 w = C::kSharedQ ? s_q[nt * C::kKP + j][lane]
-                                        : make_uint4(qf[nt][4 * j], qf[nt][4 * j + 1], qf[nt][4 * j + 2], qf[nt][4 * j + 3]);
-            mma<false>(s[u][nt], a[0], b[0], a[1], b[1], w.x, w.y);
-            mma<false>(s[u][nt], a[2], b[2], a[3], b[3], w.z, w.w);
+            mma<false>(part[0][u][nt], a.x, b.x, a.y, b.y, w[nt].x, w[nt].y);
+            mma<false>(part[kChains - 1][u][nt], a.z, b.z, a.w, b.w, w[nt].z, w[nt].w);
           }
-        } else {
+        }
+      } else {
+        uint4 w[kNT][2];
+#pragma unroll
+        for (int nt = 0; nt < kNT; ++nt)
+#pragma unroll
+          for (int i = 0; i < 2; ++i) w[nt][i] = s_q[(nt * (kDim / 32) + 2 * j + i) * 32 + lane];
+#pragma unroll
+        for (int u = 0; u < kU; ++u) {
+          const uint4 x = key(u, 0, j), y = key(u, 1, j);
+          const uint32_t a[4] = {x.x, x.y, x.z, x.w}, b[4] = {y.x, y.y, y.z, y.w};
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const uint32_t x0 = half_pair(a[i]), x1 = half_pair(b[i]), x2 = half_pair_hi(a[i]), x3 = half_pair_hi(b[i]);
 #pragma unroll
-            for (int nt = 0; nt < kNT; ++nt) mma<true>(s[u][nt], x0, x1, x2, x3, qf[nt][8 * j + 2 * i], qf[nt][8 * j + 2 * i + 1]);
+            for (int nt = 0; nt < kNT; ++nt)
+              mma<true>(part[i % kChains][u][nt], x0, x1, x2, x3, i & 1 ? w[nt][i / 2].z : w[nt][i / 2].x,
+                        i & 1 ? w[nt][i / 2].w : w[nt][i / 2].y);
           }
         }
       }
     }
+#pragma unroll
+    for (int u = 0; u < kU; ++u)
+#pragma unroll
+      for (int nt = 0; nt < kNT; ++nt)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          s[u][nt][j] = part[0][u][nt][j];
+#pragma unroll
+          for (int i = 1; i < kChains; ++i) s[u][nt][j] += part[i][u][nt][j];
+        }
     // logits in log2 units (with the value rows' exponents), -inf where nothing is seen
-    float kf[kU][2], vf[kU][2], back[kU][2];
-    int low[kU], high[kU];
+    float back[kU][2];
 #pragma unroll
     for (int u = 0; u < kU; ++u) {
-      low[u] = lo[u], high[u] = hi[u];
+      float kf[2], vf[2];
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
-        kf[u][r] = kQuant ? exp2i(ek[u][r]) : 1.f;
-        vf[u][r] = kQuant ? static_cast<float>(ev[u][r]) : 0.f;
-        back[u][r] = kQuant ? exp2i(-ev[u][r]) : 1.f;
+        const int8_t* x = reinterpret_cast<const int8_t*>(&s_exp[slot][u][r * 8 + tok]);
+        kf[r] = kQuant ? exp2i(x[0]) : 1.f;
+        vf[r] = kQuant ? __uint_as_float(0x4b400000u + x[16]) - 12582912.f : 0.f;  // the exponent as a float, off the conversion pipe
+        back[u][r] = kQuant ? exp2i(-max(static_cast<int>(x[16]), -126)) : 1.f;  // finite in places not seen, too
       }
-    }
-    if (step + 1 < steps) load_k(step + 1);
-    bool above = false;
-#pragma unroll
-    for (int u = 0; u < kU; ++u) {
+      const int seen = s_range[slot][u];
 #pragma unroll
       for (int nt = 0; nt < kNT; ++nt)
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           float z = s[u][nt][j] * qs[nt][j & 1];
-          if (kQuant) z = z * kf[u][j >> 1] + vf[u][j >> 1];
+          if (kQuant) z = z * kf[j >> 1] + vf[j >> 1];
           s[u][nt][j] = z;
         }
-      if (low[u] > 0 || high[u] < kTile)
+      if (seen != kTile << 8)
 #pragma unroll
         for (int nt = 0; nt < kNT; ++nt)
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            const int r = lr + (j >> 1) * 8;
-            if (r < low[u] || r >= high[u]) s[u][nt][j] = -INFINITY;
+            const int r = tok + (j >> 1) * 8;
+            if (r < (seen & 255) || r >= seen >> 8) s[u][nt][j] = -INFINITY;
           }
-#pragma unroll
-      for (int nt = 0; nt < kNT; ++nt)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) above |= s[u][nt][j] > m[nt][j & 1] + kSlack;
     }
+    __syncwarp();  // the unit is read
+    ask(!(C::kRing & 1), step + C::kRing / 2, slot);
+    next_slot();
+
+    bool above = false;
+#pragma unroll
+    for (int nt = 0; nt < kNT; ++nt)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        float x = fmaxf(s[0][nt][h], s[0][nt][2 + h]);
+#pragma unroll
+        for (int u = 1; u < kU; ++u) x = fmaxf(x, fmaxf(s[u][nt][h], s[u][nt][2 + h]));
+        above |= x > m[nt][h] + kSlack;
+      }
     if (__any_sync(0xffffffffu, above)) {
 #pragma unroll
       for (int nt = 0; nt < kNT; ++nt)
@@ -389,6 +435,7 @@ __global__ void __launch_bounds__(kWarps * 32) attend_kernel(const __grid_consta
           for (int w = 4; w < 32; w *= 2) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, w));
           const float f = m[nt][h] == -INFINITY ? 0.f : ex2(m[nt][h] - x);
           m[nt][h] = x;
+          sub[nt][h] = (x == -INFINITY ? 0.f : x) - (kQuant ? kLift : 0.f);
           l[nt][h] *= f;
 #pragma unroll
           for (int i = 0; i < kDim / 16; ++i) o[nt][i][h] *= f, o[nt][i][2 + h] *= f;
@@ -403,9 +450,8 @@ __global__ void __launch_bounds__(kWarps * 32) attend_kernel(const __grid_consta
         float w[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const float mm = m[nt][j & 1] == -INFINITY ? 0.f : m[nt][j & 1];
-          w[j] = ex2(s[u][nt][j] - mm + (kQuant ? kLift : 0.f));
-          l[nt][j & 1] += kQuant ? (w[j] == 0.f ? 0.f : w[j] * back[u][j >> 1]) : w[j];
+          w[j] = ex2(s[u][nt][j] - sub[nt][j & 1]);
+          l[nt][j & 1] += kQuant ? w[j] * back[u][j >> 1] : w[j];
         }
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
@@ -418,24 +464,39 @@ __global__ void __launch_bounds__(kWarps * 32) attend_kernel(const __grid_consta
           }
         }
       }
+
+    landed(step);
+    unit = ring + slot * C::kUnit;
 #pragma unroll
     for (int u = 0; u < kU; ++u) {
-      // what lies in places not seen may be anything: no weight of zero makes a NaN harmless
-      if (low[u] > 0 || high[u] < kTile)
+      const int seen = s_range[slot][u];
+#pragma unroll
+      for (int j = 0; j < C::kVP; ++j) {
+        uint32_t v[4][C::kVW];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const int r = lc * 2 + (i & 1) + (i >> 1) * 8;
-          if (r < low[u] || r >= high[u])
-#pragma unroll
-            for (int j = 0; j < C::kVP; ++j)
-#pragma unroll
-              for (int w = 0; w < C::kVW; ++w) v[u][i][j][w] = 0;
+          const int t = vtok[i & 1], key = C::kBox == 128 ? t : t >> 1 & 3;
+          const uint8_t* src = unit + u * C::kTileBytes + (j * kTile + t + (i >> 1) * 8) * C::kBox;
+          if constexpr (C::kVB == 16) {
+            const uint4 w = *reinterpret_cast<const uint4*>(src + (lr ^ key) * 16);
+            v[i][0] = w.x, v[i][1] = w.y, v[i][2] = w.z, v[i][3] = w.w;
+          } else {
+            const uint2 w = *reinterpret_cast<const uint2*>(src + (lr * 8 ^ key * 16));
+            v[i][0] = w.x, v[i][1] = w.y;
+          }
         }
+        // what lies in places not seen may be anything, and no weight of zero makes a NaN harmless
+        if (seen != kTile << 8)
 #pragma unroll
-      for (int j = 0; j < C::kVP; ++j)
+          for (int i = 0; i < 4; ++i) {
+            const int r = vtok[i & 1] + (i >> 1) * 8;
+            if (r < (seen & 255) || r >= seen >> 8)
+#pragma unroll
+              for (int w = 0; w < C::kVW; ++w) v[i][w] = 0;
+          }
 #pragma unroll
         for (int w = 0; w < C::kVW; ++w) {
-          const uint32_t t0 = v[u][0][j][w], t1 = v[u][1][j][w], t8 = v[u][2][j][w], t9 = v[u][3][j][w];
+          const uint32_t t0 = v[0][w], t1 = v[1][w], t8 = v[2][w], t9 = v[3][w];
           if (!kQuant) {
             const int tile = j * 4 + w;
             const uint32_t a0 = __byte_perm(t0, t1, 0x5410), a1 = __byte_perm(t0, t1, 0x7632);
@@ -449,17 +510,24 @@ __global__ void __launch_bounds__(kWarps * 32) attend_kernel(const __grid_consta
             const int tile = (j * C::kVW + w) * 2;
             const uint32_t x0 = __byte_perm(t0, t1, 0x5140), x1 = __byte_perm(t0, t1, 0x7362);
             const uint32_t y0 = __byte_perm(t8, t9, 0x5140), y1 = __byte_perm(t8, t9, 0x7362);
+            const uint32_t a0 = half_pair(x0), a1 = half_pair_hi(x0), a2 = half_pair(y0), a3 = half_pair_hi(y0);
+            const uint32_t b0 = half_pair(x1), b1 = half_pair_hi(x1), b2 = half_pair(y1), b3 = half_pair_hi(y1);
 #pragma unroll
             for (int nt = 0; nt < kNT; ++nt) {
-              mma<true>(o[nt][tile], half_pair(x0), half_pair_hi(x0), half_pair(y0), half_pair_hi(y0), ph[u][nt][0], ph[u][nt][1]);
-              mma<true>(o[nt][tile + 1], half_pair(x1), half_pair_hi(x1), half_pair(y1), half_pair_hi(y1), ph[u][nt][0], ph[u][nt][1]);
+              mma<true>(o[nt][tile], a0, a1, a2, a3, ph[u][nt][0], ph[u][nt][1]);
+              mma<true>(o[nt][tile + 1], b0, b1, b2, b3, ph[u][nt][0], ph[u][nt][1]);
             }
           }
         }
+      }
     }
+    __syncwarp();  // the unit is read
+    ask(C::kRing & 1, step + (C::kRing + 1) / 2, slot);
+    next_slot();
   }
 
-  // join the warps
+  // join the warps; the ring's place is free once every warp is here (it has waited for all that it asked for)
+  float(*s_o)[kNT * 4][C::kPitch] = reinterpret_cast<float(*)[kNT * 4][C::kPitch]>(smem);
 #pragma unroll
   for (int nt = 0; nt < kNT; ++nt)
 #pragma unroll
@@ -468,62 +536,128 @@ __global__ void __launch_bounds__(kWarps * 32) attend_kernel(const __grid_consta
       for (int w = 4; w < 32; w *= 2) l[nt][h] += __shfl_xor_sync(0xffffffffu, l[nt][h], w);
       if (lr == 0) s_m[warp][nt * 8 + 2 * lc + h] = m[nt][h], s_l[warp][nt * 8 + 2 * lc + h] = l[nt][h];
     }
+  __syncthreads();
+  const bool whole = sp.tiles <= sp.chunk;
+  if (threadIdx.x < C::kHeads) {  // each warp's factor into s_m, 1 / sum (or 1) into s_qs
+    const int h = threadIdx.x;
+    float mm = -INFINITY, ll = 0.f;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) mm = fmaxf(mm, s_m[w][h]);
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      const float f = s_m[w][h] == -INFINITY ? 0.f : ex2(s_m[w][h] - mm);
+      ll += s_l[w][h] * f;
+      s_m[w][h] = f;
+    }
+    s_qs[h] = whole ? (ll == 0.f ? 0.f : 1.f / ll) : 1.f;
+    if (h0 + h < p.group) {
+      if (whole)
+        p.lse[qrow + h] = ll == 0.f ? -INFINITY : (mm - (kQuant ? kLift : 0.f) + log2f(ll)) * 0.69314718055994531f;
+      else
+        p.part_ml[(qrow + h) * p.splits + split] = make_float2(mm, ll);
+    }
+  }
+  // (value d of both heads of a pair) at d with its low bits turned by lr, so that neither these writes (lanes kE
+  // values apart) nor the reads (neighbours) meet on a bank
 #pragma unroll
   for (int nt = 0; nt < kNT; ++nt)
 #pragma unroll
     for (int i = 0; i < kDim / 16; ++i)
 #pragma unroll
-      for (int r = 0; r < 2; ++r)  // (d, both heads) at [head pair][tile][r][lr]
-        *reinterpret_cast<float2*>(&s_o[warp][nt * 4 + lc][(i * 16 + r * 8 + lr) * 2]) = make_float2(o[nt][i][2 * r], o[nt][i][2 * r + 1]);
+      for (int r = 0; r < 2; ++r) {
+        const int d = i / (C::kE / 2) * 8 * C::kE + lr * C::kE + i % (C::kE / 2) * 2 + r;
+        *reinterpret_cast<float2*>(&s_o[warp][nt * 4 + lc][(d ^ (lr & 3)) * 2]) = make_float2(o[nt][i][2 * r], o[nt][i][2 * r + 1]);
+      }
   __syncthreads();
-  const bool whole = sp.tiles <= sp.chunk;
-  for (int i = threadIdx.x; i < C::kHeads * kDim; i += blockDim.x) {
-    const int h = i / kDim, d = i % kDim;
+  for (int i = threadIdx.x; i < C::kHeads / 2 * kDim; i += blockDim.x) {
+    const int hp = i / kDim, d = i % kDim, h = 2 * hp;
     if (h0 + h >= p.group) break;
-    float mm = -INFINITY, ll = 0.f, x = 0.f;
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) mm = fmaxf(mm, s_m[w][h]);
-    // d = pass * 8 * kE + lr * kE + 2 * (tile of the pass) + r
-    const int in = d % (8 * C::kE), tile = d / (8 * C::kE) * (C::kE / 2) + in % C::kE / 2;
-    const int at_ = (tile * 16 + (in & 1) * 8 + in / C::kE) * 2 + (h & 1);
+    float x = 0.f, y = 0.f;
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) {
-      const float f = s_m[w][h] == -INFINITY ? 0.f : ex2(s_m[w][h] - mm);
-      ll += s_l[w][h] * f;
-      x += s_o[w][h >> 1][at_] * f;
+      const float2 v = *reinterpret_cast<const float2*>(&s_o[w][hp][(d ^ (d / C::kE & 3)) * 2]);
+      const float2 f = *reinterpret_cast<const float2*>(&s_m[w][h]);
+      x += v.x * f.x, y += v.y * f.y;
     }
+    x *= s_qs[h], y *= s_qs[h + 1];
+    const bool both = h0 + h + 1 < p.group;
     if (whole) {
-      p.out[(qrow + h) * kDim + d] = __float2bfloat16_rn(ll == 0.f ? 0.f : x / ll);
-      if (d == 0) p.lse[qrow + h] = ll == 0.f ? -INFINITY : (mm - (kQuant ? kLift : 0.f) + log2f(ll)) * 0.69314718055994531f;
+      p.out[(qrow + h) * kDim + d] = __float2bfloat16_rn(x);
+      if (both) p.out[(qrow + h + 1) * kDim + d] = __float2bfloat16_rn(y);
     } else {
-      const int64_t to = (qrow + h) * p.splits + split;
-      p.part_o[to * kDim + d] = x;
-      if (d == 0) p.part_ml[to] = make_float2(mm, ll);
+      float* to = p.part_o + ((qrow + h) * p.splits + split) * kDim + d;
+      to[0] = x;
+      if (both) to[static_cast<int64_t>(p.splits) * kDim] = y;
     }
   }
 }
 
-// Joins the splits of one query head: blockIdx = (head, row), a thread a value.
-__global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ Params p, int dim, float lift) {
+// Joins the splits. 16 lanes hold 64 values of one query head (4 each); `groups` of them take its splits in turn,
+// each with a running maximum of its own, and meet in shared memory: 16 / groups pieces of 64 values a CTA.
+constexpr int kJoinThreads = 256, kJoinBatch = 4;
+__global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constant__ Params p, int dim, int groups, float lift) {
+  __shared__ float s_m[kJoinThreads / 16], s_l[kJoinThreads / 16];
+  __shared__ float4 s_x[kJoinThreads / 16][16];
   griddep_launch();
   griddep_wait();
-  const int row = blockIdx.y;
-  const Span sp = row_span(p, row);
-  if (sp.tiles <= sp.chunk) return;  // written whole, or nothing to see
-  const int n = static_cast<int>((sp.tiles + sp.chunk - 1) / sp.chunk);
-  const int64_t head = static_cast<int64_t>(row) * p.q_heads + blockIdx.x;
-  const float2* ml = p.part_ml + head * p.splits;
-  const float* po = p.part_o + head * p.splits * dim + threadIdx.x;
-  float mm = -INFINITY, ll = 0.f, x = 0.f;
-  for (int i = 0; i < n; ++i) mm = fmaxf(mm, ml[i].x);
-  for (int i = 0; i < n; ++i) {
-    const float2 a = ml[i];
-    const float f = a.x == -INFINITY ? 0.f : ex2(a.x - mm);
-    ll += a.y * f;
-    x += po[static_cast<int64_t>(i) * dim] * f;
+  const int team = threadIdx.x / 16, c = threadIdx.x % 16, g = team % groups, pieces = dim / 64;
+  const int64_t piece = static_cast<int64_t>(blockIdx.x) * (16 / groups) + team / groups, head = piece / pieces;
+  const int64_t row = head / p.q_heads;
+  bool on = row < p.c.rows;
+  int n = 0;
+  if (on) {
+    const Span sp = row_span(p, static_cast<int>(row));
+    on = sp.tiles > sp.chunk;  // else written whole, or nothing to see
+    if (on) n = static_cast<int>((sp.tiles + sp.chunk - 1) / sp.chunk);
   }
-  p.out[head * dim + threadIdx.x] = __float2bfloat16_rn(ll == 0.f ? 0.f : x / ll);
-  if (threadIdx.x == 0) p.lse[head] = ll == 0.f ? -INFINITY : (mm - lift + log2f(ll)) * 0.69314718055994531f;
+  const int at = static_cast<int>(piece % pieces) * 16 + c;  // of the head's float4s
+  const float2* ml = p.part_ml + head * p.splits;
+  const float4* po = reinterpret_cast<const float4*>(p.part_o + head * p.splits * dim) + at;
+  float m = -INFINITY, l = 0.f;
+  float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int i0 = g; i0 < n; i0 += groups * kJoinBatch) {
+    float2 a[kJoinBatch];
+    float4 y[kJoinBatch];
+#pragma unroll
+    for (int b = 0; b < kJoinBatch; ++b) {
+      const int i = i0 + b * groups;
+      a[b] = i < n ? ml[i] : make_float2(-INFINITY, 0.f);
+      y[b] = i < n ? po[static_cast<int64_t>(i) * (dim / 4)] : make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+    float mm = m;
+#pragma unroll
+    for (int b = 0; b < kJoinBatch; ++b) mm = fmaxf(mm, a[b].x);
+    const float back = m == -INFINITY ? 0.f : ex2(m - mm);
+    l *= back, x.x *= back, x.y *= back, x.z *= back, x.w *= back;
+#pragma unroll
+    for (int b = 0; b < kJoinBatch; ++b) {
+      const float f = a[b].x == -INFINITY ? 0.f : ex2(a[b].x - mm);
+      l += a[b].y * f;
+      x.x += y[b].x * f, x.y += y[b].y * f, x.z += y[b].z * f, x.w += y[b].w * f;
+    }
+    m = mm;
+  }
+  if (groups > 1) {
+    if (c == 0) s_m[team] = m, s_l[team] = l;
+    s_x[team][c] = x;
+    __syncthreads();
+    if (g) return;
+    float mm = m;
+    for (int i = 1; i < groups; ++i) mm = fmaxf(mm, s_m[team + i]);
+    const float f0 = m == -INFINITY ? 0.f : ex2(m - mm);
+    l *= f0, x.x *= f0, x.y *= f0, x.z *= f0, x.w *= f0;
+    for (int i = 1; i < groups; ++i) {
+      const float f = s_m[team + i] == -INFINITY ? 0.f : ex2(s_m[team + i] - mm);
+      const float4 y = s_x[team + i][c];
+      l += s_l[team + i] * f;
+      x.x += y.x * f, x.y += y.y * f, x.z += y.z * f, x.w += y.w * f;
+    }
+    m = mm;
+  }
+  if (!on) return;
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  *reinterpret_cast<uint2*>(p.out + head * dim + at * 4) = make_uint2(pack_bf16(x.x * inv, x.y * inv), pack_bf16(x.z * inv, x.w * inv));
+  if (at == 0) p.lse[head] = l == 0.f ? -INFINITY : (m - lift + log2f(l)) * 0.69314718055994531f;
 }
 
 // ------------------------------------------------------------------ host side
@@ -537,47 +671,65 @@ static int sms() {
   return sm_count(dev);
 }
 
-static int tile_heads(int group, int dim) { return group > 8 && dim <= 128 ? 16 : 8; }
+static int tile_heads(int group) { return group > 8 ? 16 : 8; }
 
 static Plan plan(int rows, int q_heads, int kv_heads, int dim, bool quant, int64_t tiles) {
   Plan r;
-  const int group = q_heads / kv_heads, heads = tile_heads(group, dim);
+  const int group = q_heads / kv_heads, heads = tile_heads(group);
   r.head_tiles = (group + heads - 1) / heads;
   const int64_t units = static_cast<int64_t>(rows) * kv_heads * r.head_tiles;
-  r.min_tiles = 8;
-  int64_t s = (static_cast<int64_t>(sms()) * 8 + units - 1) / units;
+  r.min_tiles = kWarps;
+  int64_t s = (static_cast<int64_t>(sms()) * 4 + units - 1) / units;
   const int64_t most = (tiles + r.min_tiles - 1) / r.min_tiles;
   if (s > most) s = most;
+  if (s > 65535) s = 65535;
   r.splits = static_cast<int>(s < 1 ? 1 : s);
   return r;
 }
 
 template <typename... A>
-static cudaError_t start(void (*kernel)(A...), dim3 grid, int threads, void* stream, A... args) {
+static cudaError_t start(void (*kernel)(A...), dim3 grid, int threads, int shared, void* stream, A... args) {
+  if (shared > 48 * 1024) {
+    const cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, shared);
+    if (err != cudaSuccess) return err;
+  }
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = pdl_enabled() ? 1 : 0;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = grid;
   cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = shared;
   cfg.stream = static_cast<cudaStream_t>(stream);
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   return cudaLaunchKernelEx(&cfg, kernel, args...);
 }
 
+template <int kDim, bool kQuant, int kNT, int kU>
+static int attend(const Params& p, dim3 grid, void* stream) {
+  using C = Shape<kDim, kQuant, kNT, kU>;
+  CUtensorMap maps[2];
+  for (int i = 0; i < 2; ++i)
+    if (!tensor_map_boxes(&maps[i], i ? p.c.v : p.c.k, C::kRow, static_cast<uint64_t>(p.kv_heads) * p.c.page_size, p.c.pages,
+                          static_cast<uint64_t>(p.c.page_stride) * (kQuant ? 1 : 2), C::kBox, kTile))
+      return DM3_EINVAL;
+  const cudaError_t err = start(attend_kernel<kDim, kQuant, kNT, kU>, grid, kWarps * 32, C::kShared, stream, p, maps[0], maps[1]);
+  if (err != cudaSuccess) return set_error(std::string("paged_attention launch: ") + cudaGetErrorString(err)), DM3_ECUDA;
+  return DM3_OK;
+}
+
 template <int kDim, bool kQuant>
-static cudaError_t attend(const Params& p, dim3 grid, void* stream) {
-  // token tiles a step: 32 registers of keys a lane (64 for 512-byte rows)
-  constexpr int kRow = kDim * (kQuant ? 1 : 2), kU = kRow <= 64 ? 4 : kRow <= 128 ? 2 : 1;
-  if constexpr (kDim <= 128) {
-    if (tile_heads(p.group, kDim) == 16) return start(attend_kernel<kDim, kQuant, 2, kU>, grid, kWarps * 32, stream, p);
-  }
-  return start(attend_kernel<kDim, kQuant, 1, kU>, grid, kWarps * 32, stream, p);
+static int attend(const Params& p, dim3 grid, void* stream) {
+  // token tiles a step: 8 KB of keys, one unit of the ring (6 KB for 384-byte rows)
+  constexpr int kRow = kDim * (kQuant ? 1 : 2), kU = kRow <= 64 ? 8 : kRow <= 128 ? 4 : kRow <= 256 ? 2 : 1;
+  return tile_heads(p.group) == 16 ? attend<kDim, kQuant, 2, kU>(p, grid, stream) : attend<kDim, kQuant, 1, kU>(p, grid, stream);
 }
 
 }  // namespace attn
 }  // namespace dm3
+
+int dm3::wait_limit_attention(uint64_t ns) { return static_cast<int>(set_wait_limit_here(ns)); }
 
 // ------------------------------------------------------------------ C ABI
 extern "C" size_t dm3_paged_attention_workspace_bytes(int rows, int q_heads, int kv_heads, int dim, int page_size,
@@ -623,16 +775,21 @@ extern "C" int dm3_paged_attention(const void* q, int64_t q_rs, int64_t q_hs, in
     p.part_ml = reinterpret_cast<float2*>(p.part_o + parts * dim);
   }
   const dim3 grid(plan.splits, kv_heads * plan.head_tiles, rows);
-  cudaError_t err;
+  int rc;
   switch (dim) {
-    case 64: err = k_exp ? attn::attend<64, true>(p, grid, stream) : attn::attend<64, false>(p, grid, stream); break;
-    case 128: err = k_exp ? attn::attend<128, true>(p, grid, stream) : attn::attend<128, false>(p, grid, stream); break;
-    case 192: err = k_exp ? attn::attend<192, true>(p, grid, stream) : attn::attend<192, false>(p, grid, stream); break;
-    default: err = k_exp ? attn::attend<256, true>(p, grid, stream) : attn::attend<256, false>(p, grid, stream); break;
+    case 64: rc = k_exp ? attn::attend<64, true>(p, grid, stream) : attn::attend<64, false>(p, grid, stream); break;
+    case 128: rc = k_exp ? attn::attend<128, true>(p, grid, stream) : attn::attend<128, false>(p, grid, stream); break;
+    case 192: rc = k_exp ? attn::attend<192, true>(p, grid, stream) : attn::attend<192, false>(p, grid, stream); break;
+    default: rc = k_exp ? attn::attend<256, true>(p, grid, stream) : attn::attend<256, false>(p, grid, stream); break;
   }
-  if (err == cudaSuccess && plan.splits > 1)
-    err = attn::start(attn::join_kernel, dim3(q_heads, rows), dim, stream, p, dim, k_exp ? attn::kLift : 0.f);
-  if (err != cudaSuccess) return set_error(std::string("paged_attention launch: ") + cudaGetErrorString(err)), DM3_ECUDA;
+  if (rc) return rc;
+  if (plan.splits > 1) {
+    const int groups = plan.splits <= 4 ? 1 : plan.splits <= 24 ? 4 : 16;  // teams that share a head's splits
+    const int64_t pieces = static_cast<int64_t>(rows) * q_heads * (dim / 64);
+    const cudaError_t err = attn::start(attn::join_kernel, dim3(static_cast<unsigned>((pieces * groups + 15) / 16)), attn::kJoinThreads, 0,
+                                        stream, p, dim, groups, k_exp ? attn::kLift : 0.f);
+    if (err != cudaSuccess) return set_error(std::string("paged_attention launch: ") + cudaGetErrorString(err)), DM3_ECUDA;
+  }
   note_launches(plan.splits > 1 ? 2 : 1);
   return DM3_OK;
 }

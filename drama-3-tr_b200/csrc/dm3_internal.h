@@ -39,4 +39,11 @@ int wait_limit_moe_prefill(uint64_t ns);
 bool tensor_map_3d(CUtensorMap* out, const void* base, uint64_t d0, uint64_t d1, uint64_t d2, uint64_t stride1,
                    uint64_t stride2, uint32_t box_rows);
 
+// A 3-D uint8 tensor map over [pages][rows][row_bytes] (rows adjacent, page stride in bytes) whose box is box_bytes
+// (128 or 64, swizzled over as many bytes) x box_rows x 1. Encoded for every call. False (with the error set) when
+// the driver rejects it.
+bool tensor_map_boxes(CUtensorMap* out, const void* base, uint64_t row_bytes, uint64_t rows, uint64_t pages,
+                      uint64_t page_stride, uint32_t box_bytes, uint32_t box_rows);
+int wait_limit_attention(uint64_t ns);
+
 }  // namespace dm3

@@ -364,9 +364,10 @@ bool kv_cache_ok(const kv::Cache& c, int kv_heads, int dim) {
     return set_error("bad page table"), false;
   const int64_t row = static_cast<int64_t>(kv_heads) * c.page_size;
   const int unit = c.k_exp ? 16 : 8;  // elements in 16 bytes
-  if (c.page_stride < row * dim || c.page_stride % unit || (c.k_exp && c.exp_stride < row))
+  if (c.page_stride < row * dim || c.page_stride % unit || (c.k_exp && (c.exp_stride < row || c.exp_stride % 16)))
     return set_error("cache: pages overlap, or do not start on 16 bytes"), false;
-  if (reinterpret_cast<uintptr_t>(c.k) % 16 || reinterpret_cast<uintptr_t>(c.v) % 16)
+  if (reinterpret_cast<uintptr_t>(c.k) % 16 || reinterpret_cast<uintptr_t>(c.v) % 16 ||
+      reinterpret_cast<uintptr_t>(c.k_exp) % 16 || reinterpret_cast<uintptr_t>(c.v_exp) % 16)
     return set_error("cache: the buffers must be 16-byte aligned"), false;
   return true;
 }

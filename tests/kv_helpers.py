@@ -33,7 +33,7 @@ def paged(lengths, kv_heads, dim, size, quant, seed, capacity=None, like=None):
             v, e = kv_oracle.quantise(x)
             code = (v * torch.exp2(-e.double())[..., None]).float().to(torch.float8_e4m3fn)
             code.view(torch.uint8)[hole] = 0x7F
-            e[hole] = 127
+            e[hole] = torch.where(torch.rand(e[hole].shape, generator=g) < 0.5, 127, -128).to(torch.int8)
             d[name], d[name + "_exp"] = code, e
         else:
             x[hole] = torch.nan
