@@ -27,6 +27,7 @@
 // sizes, and l sums w_t * 2^-e_t. Codes are exact in fp16; queries are scaled by a power of two to
 // [2^14, 2^15), where fp16 holds a bf16 row to 2^-40 of its largest value; a weight is rounded once to 11 bits.
 // With a bf16 cache a weight goes to the tensor cores as a bf16 pair (high and low part, 16 bits).
+#include <atomic>
 #include <cmath>
 #include <cstdint>
 #include <string>
@@ -689,10 +690,6 @@ static Plan plan(int rows, int q_heads, int kv_heads, int dim, bool quant, int64
 
 template <typename... A>
 static cudaError_t start(void (*kernel)(A...), dim3 grid, int threads, int shared, void* stream, A... args) {
-  if (shared > 48 * 1024) {
-    const cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, shared);
-    if (err != cudaSuccess) return err;
-  }
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = pdl_enabled() ? 1 : 0;
@@ -714,6 +711,16 @@ static int attend(const Params& p, dim3 grid, void* stream) {
     if (!tensor_map_boxes(&maps[i], i ? p.c.v : p.c.k, C::kRow, static_cast<uint64_t>(p.kv_heads) * p.c.page_size, p.c.pages,
                           static_cast<uint64_t>(p.c.page_stride) * (kQuant ? 1 : 2), C::kBox, kTile))
       return DM3_EINVAL;
+  // once a device (a second thread setting it again does no harm)
+  static std::atomic<uint64_t> allowed{0};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  const uint64_t bit = uint64_t(1) << (dev & 63);
+  if (!(allowed.load(std::memory_order_relaxed) & bit)) {
+    const cudaError_t err = cudaFuncSetAttribute(attend_kernel<kDim, kQuant, kNT, kU>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kShared);
+    if (err != cudaSuccess) return set_error(std::string("paged_attention: ") + cudaGetErrorString(err)), DM3_ECUDA;
+    allowed.fetch_or(bit, std::memory_order_relaxed);
+  }
   const cudaError_t err = start(attend_kernel<kDim, kQuant, kNT, kU>, grid, kWarps * 32, C::kShared, stream, p, maps[0], maps[1]);
   if (err != cudaSuccess) return set_error(std::string("paged_attention launch: ") + cudaGetErrorString(err)), DM3_ECUDA;
   return DM3_OK;

@@ -27,7 +27,9 @@ namespace dm3 {
 namespace kv {
 
 constexpr int kThreads = 256;
-constexpr int kMaxRot = 1024;  // angles of one token in shared memory
+constexpr int kMaxRot = 1024;
+constexpr int kBlockTokens = 8;   // most tokens of one CTA
+constexpr int kAngles = 1024;     // most (token, pair) angles of one CTA: 8 tokens of a 256-value head, or 2 of 1024
 
 struct Heads {  // [tokens][heads][dim] bf16, unit stride in dim
   const __nv_bfloat16* p;
@@ -38,31 +40,20 @@ struct Heads {  // [tokens][heads][dim] bf16, unit stride in dim
 struct RopeParams {
   Heads x;
   __nv_bfloat16* y;  // [T][heads][dim]
-  int T, dim;
+  int T, dim, block;  // block: tokens of a CTA
   const int64_t* positions;
   const double* inv_freq;
   int rot, interleaved;
   double factor;
 };
 
-// (cos, sin) of position * inv_freq, times factor. In 64 bits up to the reduced angle; `T` is the type
-// of what follows: double where a rotated key is quantised next.
-template <typename T>
-__device__ __forceinline__ void angle(int64_t pos, double inv_freq, double factor, T& c, T& s) {
-  double t = static_cast<double>(pos) * inv_freq * 0.31830988618379067154;  // 1 / pi
-  t -= 2.0 * rint(t * 0.5);
-  if (sizeof(T) == 8) {
-    double cd, sd;
-    sincospi(t, &sd, &cd);
-    c = static_cast<T>(cd * factor);
-    s = static_cast<T>(sd * factor);
-  } else {
-    float cf, sf;
-    sincospif(static_cast<float>(t), &sf, &cf);
-    c = static_cast<T>(cf * static_cast<float>(factor));
-    s = static_cast<T>(sf * static_cast<float>(factor));
-  }
-}
+// Division by a fixed n < 2^16 of values below 2^16: (x * ceil(2^32 / n)) >> 32 is exact there.
+struct Div {
+  uint32_t n, m;
+  explicit Div(int d) : n(d), m(d > 1 ? static_cast<uint32_t>(((uint64_t(1) << 32) + d - 1) / d) : 0) {}
+  Div() : n(1), m(0) {}
+  __device__ __forceinline__ int operator()(int x) const { return n > 1 ? static_cast<int>(__umulhi(static_cast<uint32_t>(x), m)) : x; }
+};
 
 struct Chunk {
   float v[8];
@@ -87,63 +78,138 @@ __device__ __forceinline__ uint4 pack(const Chunk& c) {
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-// Turns the 8 values of chunk `at` (of dim / 8) of the row at `row`; `own` is that chunk. cs holds the
-// token's (cos, sin). rot is a multiple of 16, so a chunk's partners are one chunk.
-template <typename T>
-__device__ __forceinline__ Chunk turn(const __nv_bfloat16* row, uint4 own, int at, const T* cosv, const T* sinv, int rot,
-                                      int interleaved) {
-  Chunk x = unpack(own);
-  if (at * 8 >= rot) return x;
-  Chunk y;
-  if (interleaved) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const T c = cosv[at * 4 + i], s = sinv[at * 4 + i], a = x.v[2 * i], b = x.v[2 * i + 1];
-      y.v[2 * i] = static_cast<float>(a * c - b * s);
-      y.v[2 * i + 1] = static_cast<float>(b * c + a * s);
-    }
+// (cos, sin) of position * inv_freq, times factor: reduced in 64 bits, then 32 (kLow false) or 64 bits as a
+// pair of floats each, high and low part.
+template <bool kLow>
+__device__ __forceinline__ void angle(int64_t pos, double inv_freq, double factor, float2& high, float2& low) {
+  double t = static_cast<double>(pos) * inv_freq * 0.31830988618379067154;  // 1 / pi
+  t -= 2.0 * rint(t * 0.5);
+  if (kLow) {
+    double c, s;
+    sincospi(t, &s, &c);
+    c *= factor, s *= factor;
+    high = make_float2(static_cast<float>(c), static_cast<float>(s));
+    low = make_float2(static_cast<float>(c - high.x), static_cast<float>(s - high.y));
   } else {
-    const int half = rot / 16;
-    const bool second = at >= half;
-    const int j = second ? at - half : at;
-    const Chunk z = unpack(*reinterpret_cast<const uint4*>(row + (second ? j : at + half) * 8));
+    float c, s;
+    sincospif(static_cast<float>(t), &s, &c);
+    high = make_float2(c * static_cast<float>(factor), s * static_cast<float>(factor));
+  }
+}
+
+// A thread works on 16 values of a row: pairs 8 * i .. 8 * i + 7. In the half layout they lie in the 8-value chunks i
+// and i + rot / 16, in the interleaved one in 2i and 2i + 1, as do the values past rot in both.
+struct Where {
+  int a, b;
+  bool turned;
+};
+__device__ __forceinline__ Where where(int i, int rot, int interleaved) {
+  const bool turned = i * 16 < rot;
+  return turned && !interleaved ? Where{i, i + rot / 16, true} : Where{2 * i, 2 * i + 1, turned};
+}
+
+// The angles of a CTA's tokens: pair 8i + 2k + e of token t at [t][k][i][e], so neighbouring threads read
+// neighbouring 16 bytes.
+template <bool kLow>
+__device__ __forceinline__ void fill_angles(float2* high, float2* low, int tokens, const int64_t* positions,
+                                            const double* inv_freq, int rot, double factor) {
+  const int half = rot / 2, units = rot / 16;
+  for (int x = threadIdx.x; x < tokens * half; x += blockDim.x) {
+    const int t = x / half, f = x - t * half, at = t * half + (((f & 7) >> 1) * units + (f >> 3)) * 2 + (f & 1);
+    float2 h, l;
+    angle<kLow>(positions[t], inv_freq[f], factor, h, l);
+    high[at] = h;
+    if (kLow) low[at] = l;
+  }
+}
+
+// a cos - b sin to about 2^-46 of |a| + |b|: products and the sum with their rounding errors carried along
+__device__ __forceinline__ float exact_turn(float a, float b, float ch, float cl, float sh, float sl) {
+  const float p = __fmul_rn(a, ch), q = __fmul_rn(-b, sh);  // _rn: not to be contracted
+  const float pe = fmaf(a, ch, -p), qe = fmaf(-b, sh, -q);
+  const float d = __fadd_rn(p, q), z = __fsub_rn(d, p);
+  const float de = __fadd_rn(__fsub_rn(p, __fsub_rn(d, z)), __fsub_rn(q, z));
+  return __fadd_rn(d, __fadd_rn(__fadd_rn(de, __fadd_rn(pe, qe)), fmaf(a, cl, -b * sl)));
+}
+
+// Turns the 16 values of unit i in place. angles: of the token.
+template <bool kExact>
+__device__ __forceinline__ void turn(Chunk& x, Chunk& y, int i, const float2* high, const float2* low, int rot, int interleaved) {
+  const int units = rot / 16;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const T c = cosv[j * 8 + i], s = second ? sinv[j * 8 + i] : -sinv[j * 8 + i];
-      y.v[i] = static_cast<float>(static_cast<T>(x.v[i]) * c + static_cast<T>(z.v[i]) * s);
+  for (int k = 0; k < 4; ++k) {
+    const float4 h = *reinterpret_cast<const float4*>(high + (k * units + i) * 2);
+    float4 l = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (kExact) l = *reinterpret_cast<const float4*>(low + (k * units + i) * 2);
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const float ch = e ? h.z : h.x, sh = e ? h.w : h.y, cl = e ? l.z : l.x, sl = e ? l.w : l.y;
+      auto pair = [&](float& a, float& b) {
+        const float a0 = a, b0 = b;
+        a = kExact ? exact_turn(a0, b0, ch, cl, sh, sl) : a0 * ch - b0 * sh;
+        b = kExact ? exact_turn(b0, -a0, ch, cl, sh, sl) : b0 * ch + a0 * sh;
+      };
+      const int j = 2 * k + e;
+      if (!interleaved)
+        pair(x.v[j], y.v[j]);
+      else if (k < 2)
+        pair(x.v[2 * j], x.v[2 * j + 1]);
+      else
+        pair(y.v[2 * j - 8], y.v[2 * j - 7]);
     }
   }
-  return y;
 }
 
 // ------------------------------------------------------------------ rope
-// One CTA a token (and a share of its heads, blockIdx.y, when there are few tokens).
-__global__ void __launch_bounds__(kThreads) rope_kernel(const __grid_constant__ RopeParams p) {
-  __shared__ float cosv[kMaxRot / 2], sinv[kMaxRot / 2];
+// A CTA takes a block of tokens (and a share of their rows, blockIdx.y, when there are few tokens), a thread 16
+// values of a row at a time, two rows' loads in flight.
+__global__ void __launch_bounds__(kThreads) rope_kernel(const __grid_constant__ RopeParams p, const Div per, const Div heads) {
+  __shared__ __align__(16) float2 cs[kAngles];
   griddep_launch();
   griddep_wait();
-  const int t = blockIdx.x;
-  const int64_t pos = p.positions[t];
-  for (int i = threadIdx.x; i < p.rot / 2; i += blockDim.x) angle(pos, p.inv_freq[i], p.factor, cosv[i], sinv[i]);
+  const int64_t t0 = static_cast<int64_t>(blockIdx.x) * p.block;
+  const int tokens = p.T - t0 < p.block ? static_cast<int>(p.T - t0) : p.block;
+  fill_angles<false>(cs, nullptr, tokens, p.positions + t0, p.inv_freq, p.rot, p.factor);
   __syncthreads();
-  const int per = p.dim / 8, n = p.x.n * per;
-  for (int i = blockIdx.y * blockDim.x + threadIdx.x; i < n; i += gridDim.y * blockDim.x) {
-    const int h = i / per, c = i - h * per;
-    const __nv_bfloat16* row = p.x.p + t * p.x.ts + h * p.x.hs;
-    const uint4 own = *reinterpret_cast<const uint4*>(row + c * 8);
-    *reinterpret_cast<uint4*>(p.y + (static_cast<int64_t>(t) * p.x.n + h) * p.dim + c * 8) =
-        pack(turn(row, own, c, cosv, sinv, p.rot, p.interleaved));
+  constexpr int kBatch = 2;
+  const int total = tokens * p.x.n * (p.dim / 16), step = blockDim.x * gridDim.y;
+  for (int u0 = blockIdx.y * blockDim.x + threadIdx.x; u0 < total; u0 += step * kBatch) {
+    uint4 ra[kBatch], rb[kBatch];
+    Where w[kBatch];
+    int t[kBatch], i[kBatch], row[kBatch];
+#pragma unroll
+    for (int b = 0; b < kBatch; ++b) {
+      const int u = u0 + b * step;
+      if (u >= total) break;
+      row[b] = per(u);
+      i[b] = u - row[b] * per.n;
+      t[b] = heads(row[b]);
+      const __nv_bfloat16* src = p.x.p + (t0 + t[b]) * p.x.ts + (row[b] - t[b] * static_cast<int>(heads.n)) * p.x.hs;
+      w[b] = where(i[b], p.rot, p.interleaved);
+      ra[b] = __ldcs(reinterpret_cast<const uint4*>(src + w[b].a * 8));
+      rb[b] = __ldcs(reinterpret_cast<const uint4*>(src + w[b].b * 8));
+    }
+#pragma unroll
+    for (int b = 0; b < kBatch; ++b) {
+      if (u0 + b * step >= total) break;
+      Chunk x = unpack(ra[b]), y = unpack(rb[b]);
+      if (w[b].turned) turn<false>(x, y, i[b], cs + t[b] * (p.rot / 2), nullptr, p.rot, p.interleaved);
+      __nv_bfloat16* dst = p.y + (t0 * p.x.n + row[b]) * p.dim;
+      *reinterpret_cast<uint4*>(dst + w[b].a * 8) = pack(x);
+      *reinterpret_cast<uint4*>(dst + w[b].b * 8) = pack(y);
+    }
   }
 }
 
-// Any dim, rot, stride and alignment: one value at a time.
+// Any dim, rot, stride and alignment: one token a CTA, one value a thread at a time.
 __global__ void __launch_bounds__(kThreads) rope_any_kernel(const __grid_constant__ RopeParams p) {
-  __shared__ float cosv[kMaxRot / 2], sinv[kMaxRot / 2];
+  __shared__ float2 cs[kMaxRot / 2];
   griddep_launch();
   griddep_wait();
   const int t = blockIdx.x;
   const int64_t pos = p.positions[t];
-  for (int i = threadIdx.x; i < p.rot / 2; i += blockDim.x) angle(pos, p.inv_freq[i], p.factor, cosv[i], sinv[i]);
+  float2 none;
+  for (int i = threadIdx.x; i < p.rot / 2; i += blockDim.x) angle<false>(pos, p.inv_freq[i], p.factor, cs[i], none);
   __syncthreads();
   const int n = p.x.n * p.dim, half = p.rot / 2;
   for (int i = blockIdx.y * blockDim.x + threadIdx.x; i < n; i += gridDim.y * blockDim.x) {
@@ -154,7 +220,7 @@ __global__ void __launch_bounds__(kThreads) rope_any_kernel(const __grid_constan
       const bool second = p.interleaved ? (d & 1) : d >= half;
       const int j = p.interleaved ? d >> 1 : (second ? d - half : d);
       const float z = __bfloat162float(row[p.interleaved ? d ^ 1 : (second ? j : d + half)]);
-      y = y * cosv[j] + z * (second ? sinv[j] : -sinv[j]);
+      y = y * cs[j].x + z * (second ? cs[j].y : -cs[j].y);
     }
     p.y[(static_cast<int64_t>(t) * p.x.n + h) * p.dim + d] = __float2bfloat16_rn(y);
   }
@@ -164,7 +230,7 @@ __global__ void __launch_bounds__(kThreads) rope_any_kernel(const __grid_constan
 struct WriteParams {
   Heads q, k, v;     // q.n = 0: none
   __nv_bfloat16* y;  // the turned queries, [T][q.n][dim]
-  int T, dim;
+  int T, dim, block;
   const int64_t* rows;  // table row of each token; null: token i is row i
   const int64_t* positions;
   Cache c;
@@ -173,9 +239,8 @@ struct WriteParams {
   double factor;
 };
 
-// The 8 values as e4m3 codes of 2^-e; what is not finite becomes NaN.
-__device__ __forceinline__ uint2 encode(const Chunk& x, int e) {
-  const float s = exp2i(-e);
+// 8 values as e4m3 codes of 2^-e; what is not finite becomes NaN.
+__device__ __forceinline__ uint2 encode(const Chunk& x, float scale) {
   uint32_t w[2];
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
@@ -183,7 +248,7 @@ __device__ __forceinline__ uint2 encode(const Chunk& x, int e) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const float a = x.v[4 * i + j];
-      f[j] = isfinite(a) ? a * s : NAN;
+      f[j] = isfinite(a) ? a * scale : NAN;
     }
     w[i] = pack_e4m3x2(f[0], f[1]) | static_cast<uint32_t>(pack_e4m3x2(f[2], f[3])) << 16;
   }
@@ -199,71 +264,102 @@ __device__ __forceinline__ int row_exponent(float amax) {
   return min(max(e, -110), 119);
 }
 
-// One CTA a token (and a share of its rows, blockIdx.y). A row (one head of q, k or v) belongs to
-// kSeg neighbouring lanes, 8 values each, so the amax of a quantised row is a few shuffles.
+// As rope_kernel, over the rows of q, k and v. A row belongs to kSeg neighbouring lanes, so the amax of a quantised
+// row is a few shuffles. A quantised key is turned to 2^-46: it is the code of the exactly turned key, whichever call
+// wrote it (in 32 bits about one value in 10^6 would fall on the other side of a code's border).
 template <int kSeg, bool kQuant>
-__global__ void __launch_bounds__(kThreads) write_kernel(const __grid_constant__ WriteParams p) {
-  using T = typename std::conditional<kQuant, double, float>::type;
-  __shared__ T cosv[kMaxDim / 2], sinv[kMaxDim / 2];
+__global__ void __launch_bounds__(kThreads) write_kernel(const __grid_constant__ WriteParams p, const Div rows_of) {
+  __shared__ __align__(16) float2 high[kAngles], low[kQuant ? kAngles : 1];
+  __shared__ int64_t s_at[kBlockTokens], s_exp[kBlockTokens];  // place of a token's row of head 0; -1: not cached
+  __shared__ bool s_pad[kBlockTokens];
   griddep_launch();
   griddep_wait();
-  const int t = blockIdx.x;
-  const int64_t pos = p.positions[t];
-  const int64_t r = p.rows ? p.rows[t] : t;
-  const bool padding = pos < 0 || r < 0;
-  for (int i = threadIdx.x; i < p.rot / 2; i += blockDim.x) angle(pos, p.inv_freq[i], p.factor, cosv[i], sinv[i]);
-  __syncthreads();
-  int64_t page = -1;
-  int in_page = 0;
-  if (!padding) {
-    const int64_t nth = pos / p.c.page_size;
-    if (r < p.c.rows && nth < p.c.per_row) page = p.c.table[r * p.c.table_stride + nth];
-    in_page = static_cast<int>(pos - nth * p.c.page_size);
-    if (page < 0 || page >= p.c.pages) {
-      page = -1;
-      if (threadIdx.x == 0) set_status(p.c.status, STATUS_BAD_PAGE);
-    }
-  }
-  const int seg = threadIdx.x / kSeg, c = threadIdx.x % kSeg, segs = blockDim.x / kSeg, per = p.dim / 8;
-  const int n = p.q.n + 2 * p.k.n;
-  // all lanes of a warp make the same number of rounds: the shuffles need them
-  for (int h0 = blockIdx.y * segs; h0 < n; h0 += gridDim.y * segs) {
-    const int h = h0 + seg;
-    const bool on = h < n && c < per;
-    Chunk x{};
-    int side = 0, head = h;  // 0: query, 1: key, 2: value
-    if (on) {
-      if (head >= p.q.n) head -= p.q.n, side = 1;
-      if (side == 1 && head >= p.k.n) head -= p.k.n, side = 2;
-      const Heads& in = side == 0 ? p.q : side == 1 ? p.k : p.v;
-      const __nv_bfloat16* row = in.p + t * in.ts + head * in.hs;
-      const uint4 own = *reinterpret_cast<const uint4*>(row + c * 8);
-      if (side == 2 || p.rot == 0)
-        x = unpack(own);
+  const int64_t t0 = static_cast<int64_t>(blockIdx.x) * p.block;
+  const int tokens = p.T - t0 < p.block ? static_cast<int>(p.T - t0) : p.block;
+  // a place is found by the last threads, while the first ones are at the angles
+  if (const int t = kThreads - 1 - threadIdx.x; t < tokens) {
+    const int64_t pos = p.positions[t0 + t], r = p.rows ? p.rows[t0 + t] : t0 + t;
+    const bool padding = pos < 0 || r < 0;
+    int64_t at = -1, x = 0;
+    if (!padding) {
+      const int64_t nth = pos / p.c.page_size, in = pos - nth * p.c.page_size;
+      const int64_t page = r < p.c.rows && nth < p.c.per_row ? p.c.table[r * p.c.table_stride + nth] : -1;
+      if (page >= 0 && page < p.c.pages)
+        at = page * p.c.page_stride + in * p.dim, x = page * p.c.exp_stride + in;
       else
-        x = turn(row, own, c, cosv, sinv, p.rot, p.interleaved);
+        set_status(p.c.status, STATUS_BAD_PAGE);
     }
-    if (on && side == 0)
-      *reinterpret_cast<uint4*>(p.y + (static_cast<int64_t>(t) * p.q.n + head) * p.dim + c * 8) =
-          padding ? make_uint4(0, 0, 0, 0) : pack(x);
-    if (!kQuant) {
-      if (on && side != 0 && page >= 0)
-        *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(side == 1 ? p.c.k : p.c.v) + page * p.c.page_stride +
-                                  (static_cast<int64_t>(head) * p.c.page_size + in_page) * p.dim + c * 8) = pack(x);
-      continue;
+    s_at[t] = at, s_exp[t] = x, s_pad[t] = padding;
+  }
+  if (p.rot) fill_angles<kQuant>(high, low, tokens, p.positions + t0, p.inv_freq, p.rot, p.factor);
+  __syncthreads();
+  constexpr int kSegs = kThreads / kSeg, kBatch = 2;
+  const int i = threadIdx.x % kSeg, n = p.q.n + 2 * p.k.n, total = tokens * n;
+  const Where w = where(i, p.rot, p.interleaved);
+  const bool mine = i < p.dim / 16;
+  // all lanes of a warp make the same number of rounds: the shuffles need them
+  for (int base = blockIdx.y * kSegs * kBatch; base < total; base += gridDim.y * kSegs * kBatch) {
+    uint4 ra[kBatch], rb[kBatch];
+    int t[kBatch], head[kBatch], side[kBatch];  // side 0: query, 1: key, 2: value, -1: none
+#pragma unroll
+    for (int b = 0; b < kBatch; ++b) {
+      const int r = base + b * kSegs + threadIdx.x / kSeg;
+      side[b] = -1;
+      ra[b] = rb[b] = make_uint4(0, 0, 0, 0);
+      if (r < total && mine) {
+        t[b] = rows_of(r);
+        int h = r - t[b] * n;
+        side[b] = 0;
+        if (h >= p.q.n) h -= p.q.n, side[b] = 1;
+        if (side[b] == 1 && h >= p.k.n) h -= p.k.n, side[b] = 2;
+        head[b] = h;
+        const Heads& in = side[b] == 0 ? p.q : side[b] == 1 ? p.k : p.v;
+        const __nv_bfloat16* row = in.p + (t0 + t[b]) * in.ts + h * in.hs;
+        ra[b] = __ldcs(reinterpret_cast<const uint4*>(row + w.a * 8));
+        rb[b] = __ldcs(reinterpret_cast<const uint4*>(row + w.b * 8));
+      }
     }
-    if (side == 1) x = unpack(pack(x));  // the key as a bf16 cache would hold it
-    float amax = 0.f;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) amax = fmaxf(amax, isfinite(x.v[i]) ? fabsf(x.v[i]) : 0.f);
+    for (int b = 0; b < kBatch; ++b) {
+      Chunk x = unpack(ra[b]), y = unpack(rb[b]);
+      if (w.turned && (side[b] == 0 || side[b] == 1)) {
+        const int at = t[b] * (p.rot / 2);
+        if (kQuant && side[b] == 1)
+          turn<kQuant>(x, y, i, high + at, low + at, p.rot, p.interleaved);
+        else
+          turn<false>(x, y, i, high + at, nullptr, p.rot, p.interleaved);
+      }
+      const uint4 px = pack(x), py = pack(y);
+      if (side[b] == 0) {
+        __nv_bfloat16* dst = p.y + ((t0 + t[b]) * p.q.n + head[b]) * p.dim;
+        const uint4 zero = make_uint4(0, 0, 0, 0);
+        *reinterpret_cast<uint4*>(dst + w.a * 8) = s_pad[t[b]] ? zero : px;
+        *reinterpret_cast<uint4*>(dst + w.b * 8) = s_pad[t[b]] ? zero : py;
+      }
+      const int64_t place = side[b] > 0 ? s_at[t[b]] : -1;
+      if (!kQuant) {
+        if (place >= 0) {
+          __nv_bfloat16* dst = static_cast<__nv_bfloat16*>(side[b] == 1 ? p.c.k : p.c.v) + place +
+                               static_cast<int64_t>(head[b]) * p.c.page_size * p.dim;
+          *reinterpret_cast<uint4*>(dst + w.a * 8) = px;
+          *reinterpret_cast<uint4*>(dst + w.b * 8) = py;
+        }
+        continue;
+      }
+      x = unpack(px), y = unpack(py);  // the key as a bf16 cache would hold it
+      float amax = 0.f;
 #pragma unroll
-    for (int o = kSeg / 2; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-    if (on && side != 0 && page >= 0) {
-      const int e = row_exponent(amax);
-      const int64_t at = static_cast<int64_t>(head) * p.c.page_size + in_page;
-      *reinterpret_cast<uint2*>(static_cast<uint8_t*>(side == 1 ? p.c.k : p.c.v) + page * p.c.page_stride + at * p.dim +
-                                c * 8) = encode(x, e);
-      if (c == 0) (side == 1 ? p.c.k_exp : p.c.v_exp)[page * p.c.exp_stride + at] = static_cast<int8_t>(e);
+      for (int j = 0; j < 8; ++j)
+        amax = fmaxf(amax, fmaxf(isfinite(x.v[j]) ? fabsf(x.v[j]) : 0.f, isfinite(y.v[j]) ? fabsf(y.v[j]) : 0.f));
+#pragma unroll
+      for (int o = kSeg / 2; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+      if (place >= 0) {
+        const int e = row_exponent(amax);
+        uint8_t* dst = static_cast<uint8_t*>(side[b] == 1 ? p.c.k : p.c.v) + place + static_cast<int64_t>(head[b]) * p.c.page_size * p.dim;
+        *reinterpret_cast<uint2*>(dst + w.a * 8) = encode(x, exp2i(-e));
+        *reinterpret_cast<uint2*>(dst + w.b * 8) = encode(y, exp2i(-e));
+        if (i == 0) (side[b] == 1 ? p.c.k_exp : p.c.v_exp)[s_exp[t[b]] + static_cast<int64_t>(head[b]) * p.c.page_size] = static_cast<int8_t>(e);
+      }
     }
   }
 }
@@ -271,60 +367,92 @@ __global__ void __launch_bounds__(kThreads) write_kernel(const __grid_constant__
 // ------------------------------------------------------------------ kv_read
 struct ReadParams {
   Cache c;
-  int heads, dim;
+  int heads;
   const int64_t* lengths;
   int64_t L;           // tokens a row of the outputs
   __nv_bfloat16* out[2];  // [rows][heads][L][dim]
 };
 
-// blockIdx = (tile of a row's 16-byte output chunks, head, 2 * row + side).
-template <bool kQuant>
+// blockIdx = (64 tokens, head, row): where their four tiles of 16 lie is looked up once, then a thread moves 16 output
+// bytes at a time, dim / 32 of them in flight.
+template <int kDim, bool kQuant>
 __global__ void __launch_bounds__(kThreads) read_kernel(const __grid_constant__ ReadParams p) {
+  constexpr int kTokens = 64, kTiles = kTokens / 16, kPer = kDim / 8, kRounds = kTokens * kPer / kThreads;
+  __shared__ int64_t s_at[kTiles];  // place of a tile's rows; -1: none
+  __shared__ float s_scale[2][kQuant ? kTokens : 1];
   griddep_launch();
   griddep_wait();
-  const int row = blockIdx.z >> 1, side = blockIdx.z & 1, head = blockIdx.y, per = p.dim / 8;
+  const int row = blockIdx.z, head = blockIdx.y, tid = threadIdx.x;
+  const int64_t first = static_cast<int64_t>(blockIdx.x) * kTokens, span = static_cast<int64_t>(p.c.per_row) * p.c.page_size;
   int64_t n = p.lengths[row];
-  const int64_t span = static_cast<int64_t>(p.c.per_row) * p.c.page_size;
   if (n > span) {
     n = span;
-    if (threadIdx.x == 0) set_status(p.c.status, STATUS_BAD_PAGE);
+    if (tid == 0) set_status(p.c.status, STATUS_BAD_PAGE);
   }
-  const int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
-  const int64_t tok = i / per;
-  const int c = static_cast<int>(i - tok * per);
-  if (tok >= p.L) return;
-  uint4 r = make_uint4(0, 0, 0, 0);
-  if (tok < n) {
-    const int64_t nth = tok / p.c.page_size;
-    const int in_page = static_cast<int>(tok - nth * p.c.page_size);
-    const int64_t page = p.c.table[row * p.c.table_stride + nth];
-    if (page < 0 || page >= p.c.pages) {
-      set_status(p.c.status, STATUS_BAD_PAGE);
-    } else {
-      const int64_t at = static_cast<int64_t>(head) * p.c.page_size + in_page;
-      const void* base = side == 0 ? p.c.k : p.c.v;
+  if (n > p.L) n = p.L;
+  // every thread of a tile's 16 finds the tile; one of them notes it
+  if (tid < (kQuant ? 2 : 1) * kTokens) {
+    const int side = tid / kTokens, in = tid % kTokens;
+    const int64_t tok = first + in;
+    int64_t at = -1;
+    float scale = 0.f;
+    if (tok - in % 16 < n) {
+      const int64_t nth = tok / p.c.page_size;
+      const int64_t page = p.c.table[row * p.c.table_stride + nth];
+      if (page < 0 || page >= p.c.pages) {
+        set_status(p.c.status, STATUS_BAD_PAGE);
+      } else {
+        const int64_t r = static_cast<int64_t>(head) * p.c.page_size + (tok - nth * p.c.page_size);
+        at = page * p.c.page_stride + (r - in % 16) * kDim;
+        if (kQuant && tok < n) scale = exp2i((side ? p.c.v_exp : p.c.k_exp)[page * p.c.exp_stride + r]);
+      }
+    }
+    if (side == 0 && in % 16 == 0) s_at[in / 16] = at;
+    if (kQuant) s_scale[side][in] = scale;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int side = 0; side < 2; ++side) {
+    uint4 r[kRounds];
+#pragma unroll
+    for (int i = 0; i < kRounds; ++i) {
+      const int u = i * kThreads + tid, tok = u / kPer, c = u % kPer;
+      const int64_t at = s_at[tok / 16];
+      r[i] = make_uint4(0, 0, 0, 0);
+      if (at >= 0 && first + tok < n) {
+        const int64_t x = at + tok % 16 * kDim + c * 8;
+        if (kQuant) {
+          const uint2 w = __ldcs(reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(side ? p.c.v : p.c.k) + x));
+          r[i].x = w.x, r[i].y = w.y;
+        } else {
+          r[i] = __ldcs(reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(side ? p.c.v : p.c.k) + x));
+        }
+      }
+    }
+    __nv_bfloat16* const out = p.out[side] + ((static_cast<int64_t>(row) * p.heads + head) * p.L + first) * kDim;
+#pragma unroll
+    for (int i = 0; i < kRounds; ++i) {
+      const int u = i * kThreads + tid, tok = u / kPer;
+      if (first + tok >= p.L) break;
       if (kQuant) {
-        const uint2 w = *reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(base) + page * p.c.page_stride + at * p.dim + c * 8);
-        const float s = exp2i((side == 0 ? p.c.k_exp : p.c.v_exp)[page * p.c.exp_stride + at]);
+        const float s = s_scale[side][tok];
         Chunk x;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const float2 f = unpack_e4m3x2(static_cast<uint16_t>((j < 2 ? w.x : w.y) >> (16 * (j & 1))));
+          const float2 f = unpack_e4m3x2(static_cast<uint16_t>((j < 2 ? r[i].x : r[i].y) >> (16 * (j & 1))));
           x.v[2 * j] = f.x * s;
           x.v[2 * j + 1] = f.y * s;
         }
-        r = pack(x);
-      } else {
-        r = *reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(base) + page * p.c.page_stride + at * p.dim + c * 8);
+        r[i] = pack(x);
       }
+      *reinterpret_cast<uint4*>(out + u * 8) = r[i];
     }
   }
-  *reinterpret_cast<uint4*>(p.out[side] + ((static_cast<int64_t>(row) * p.heads + head) * p.L + tok) * p.dim + c * 8) = r;
 }
 
 // ------------------------------------------------------------------ host side
-template <typename K, typename P>
-static int launch(K kernel, dim3 grid, int threads, const P& p, void* stream, const char* what) {
+template <typename... A>
+static int launch(void (*kernel)(A...), dim3 grid, int threads, void* stream, const char* what, A... args) {
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = pdl_enabled() ? 1 : 0;
@@ -334,7 +462,7 @@ static int launch(K kernel, dim3 grid, int threads, const P& p, void* stream, co
   cfg.stream = static_cast<cudaStream_t>(stream);
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  const cudaError_t err = cudaLaunchKernelEx(&cfg, kernel, p);
+  const cudaError_t err = cudaLaunchKernelEx(&cfg, kernel, args...);
   if (err != cudaSuccess) return set_error(std::string(what) + " launch: " + cudaGetErrorString(err)), DM3_ECUDA;
   note_launches(1);
   return DM3_OK;
@@ -344,12 +472,21 @@ static bool aligned(const Heads& h) {
   return reinterpret_cast<uintptr_t>(h.p) % 16 == 0 && h.ts % 8 == 0 && h.hs % 8 == 0;
 }
 
-// CTAs a token: enough that few tokens still spread over the machine, at most one a round of rows.
-static int shares(int64_t tokens, int rounds) {
+// Tokens of a CTA: eight a CTA of each SM's eight at most, so that a token's angles and places cost little beside its
+// rows, but no fewer CTAs than that. And CTAs that share a block's rows when there are few tokens.
+struct Blocks {
+  int tokens, shares;
+};
+static Blocks blocks(int64_t T, int rot, int64_t rounds_a_token) {
   int dev = 0;
   cudaGetDevice(&dev);
-  const int64_t want = (2 * sm_count(dev) + tokens - 1) / tokens;
-  return static_cast<int>(want < rounds ? want : rounds);
+  const int64_t ctas = 8 * sm_count(dev);
+  Blocks b;
+  b.tokens = static_cast<int>(T / ctas < 1 ? 1 : T / ctas < kBlockTokens ? T / ctas : kBlockTokens);
+  while (b.tokens * (rot / 2) > kAngles) --b.tokens;
+  const int64_t want = (ctas / 4 + T - 1) / T;
+  b.shares = static_cast<int>(b.tokens > 1 ? 1 : want < rounds_a_token ? want : rounds_a_token);
+  return b;
 }
 
 }  // namespace kv
@@ -387,14 +524,19 @@ extern "C" int dm3_rope(const void* x, int T, int heads, int dim, int64_t ts, in
     return set_error("rope: the rotated part must be even, at most the head and at most 1024"), DM3_EINVAL;
   if (T == 0) return DM3_OK;
   if (!x || !positions || !inv_freq || !y) return set_error("rope: null pointer"), DM3_EINVAL;
-  RopeParams p{{static_cast<const __nv_bfloat16*>(x), ts, hs, heads}, static_cast<__nv_bfloat16*>(y), T, dim, positions,
+  RopeParams p{{static_cast<const __nv_bfloat16*>(x), ts, hs, heads}, static_cast<__nv_bfloat16*>(y), T, dim, 1, positions,
                inv_freq, rot, interleaved, factor};
-  // 16 bytes a thread where rows and pairs fall on them
-  const bool wide = dim % 8 == 0 && rot % 16 == 0 && aligned(p.x) && reinterpret_cast<uintptr_t>(y) % 16 == 0;
-  const int units = wide ? heads * (dim / 8) : heads * dim;
-  const int threads = units < kThreads ? (units + 31) / 32 * 32 : kThreads;
-  const dim3 grid(T, shares(T, (units + threads - 1) / threads));
-  return wide ? launch(rope_kernel, grid, threads, p, stream, "rope") : launch(rope_any_kernel, grid, threads, p, stream, "rope");
+  // 16 bytes a thread at a time where rows and pairs fall on them, and a block's rows are counted in 16 bits
+  const int units = dim / 16 * heads;
+  const bool wide = dim % 16 == 0 && rot % 16 == 0 && units < 65536 / kBlockTokens && aligned(p.x) && reinterpret_cast<uintptr_t>(y) % 16 == 0;
+  if (wide) {
+    const Blocks b = blocks(T, rot, (units + 2 * kThreads - 1) / (2 * kThreads));
+    p.block = b.tokens;
+    const int threads = b.tokens > 1 || units >= kThreads ? kThreads : (units + 31) / 32 * 32;
+    return launch(rope_kernel, dim3((T + b.tokens - 1) / b.tokens, b.shares), threads, stream, "rope", p, Div(dim / 16), Div(heads));
+  }
+  const Blocks b = blocks(T, 0, (heads * dim + kThreads - 1) / kThreads);
+  return launch(rope_any_kernel, dim3(T, b.shares), kThreads, stream, "rope", p);
 }
 
 extern "C" int dm3_kv_write(const void* q, int q_heads, int64_t q_ts, int64_t q_hs, const void* k, int64_t k_ts, int64_t k_hs,
@@ -420,11 +562,14 @@ extern "C" int dm3_kv_write(const void* q, int q_heads, int64_t q_ts, int64_t q_
   p.y = static_cast<__nv_bfloat16*>(q_out);
   p.T = T, p.dim = dim, p.rows = rows, p.positions = positions;
   p.inv_freq = inv_freq, p.rot = rot, p.interleaved = interleaved, p.factor = factor;
-  const int seg = dim == 64 ? 8 : dim == 128 ? 16 : 32, per_round = kThreads / seg, n = q_heads + 2 * kv_heads;
-  const dim3 grid(T, shares(T, (n + per_round - 1) / per_round));
-  auto go = [&](auto kernel) { return launch(kernel, grid, kThreads, p, stream, "kv_write"); };
-  if (k_exp) return seg == 8 ? go(write_kernel<8, true>) : seg == 16 ? go(write_kernel<16, true>) : go(write_kernel<32, true>);
-  return seg == 8 ? go(write_kernel<8, false>) : seg == 16 ? go(write_kernel<16, false>) : go(write_kernel<32, false>);
+  const int seg = dim == 64 ? 4 : dim == 128 ? 8 : 16, round = 2 * kThreads / seg, n = q_heads + 2 * kv_heads;
+  if (n > 65535 / kBlockTokens) return set_error("kv_write: too many heads"), DM3_EINVAL;
+  const Blocks b = blocks(T, rot, (n + round - 1) / round);
+  p.block = b.tokens;
+  const dim3 grid((T + b.tokens - 1) / b.tokens, b.shares);
+  auto go = [&](auto kernel) { return launch(kernel, grid, kThreads, stream, "kv_write", p, Div(n)); };
+  if (k_exp) return seg == 4 ? go(write_kernel<4, true>) : seg == 8 ? go(write_kernel<8, true>) : go(write_kernel<16, true>);
+  return seg == 4 ? go(write_kernel<4, false>) : seg == 8 ? go(write_kernel<8, false>) : go(write_kernel<16, false>);
 }
 
 extern "C" int dm3_kv_read(const void* k_cache, const void* v_cache, int64_t page_stride, const int8_t* k_exp,
@@ -436,15 +581,19 @@ extern "C" int dm3_kv_read(const void* k_cache, const void* v_cache, int64_t pag
   p.c = {const_cast<void*>(k_cache), const_cast<void*>(v_cache), const_cast<int8_t*>(k_exp), const_cast<int8_t*>(v_exp),
          page_stride, exp_stride, pages, page_size, table, table_stride, table_rows, per_row, status};
   if (!kv_cache_ok(p.c, kv_heads, dim)) return DM3_EINVAL;
-  if (table_rows > 32767) return set_error("kv_read: at most 32767 rows"), DM3_EINVAL;
+  if (table_rows > 65535) return set_error("kv_read: at most 65535 rows"), DM3_EINVAL;
   if (max_length < 0 || max_length > (int64_t(1) << 31)) return set_error("kv_read: bad max_length"), DM3_EINVAL;
   if (table_rows == 0 || max_length == 0) return DM3_OK;
   if (!lengths || !k_out || !v_out || reinterpret_cast<uintptr_t>(k_out) % 16 || reinterpret_cast<uintptr_t>(v_out) % 16)
     return set_error("kv_read: null or misaligned pointer"), DM3_EINVAL;
-  p.heads = kv_heads, p.dim = dim, p.lengths = lengths, p.L = max_length;
+  p.heads = kv_heads, p.lengths = lengths, p.L = max_length;
   p.out[0] = static_cast<__nv_bfloat16*>(k_out), p.out[1] = static_cast<__nv_bfloat16*>(v_out);
-  const int64_t chunks = max_length * (dim / 8);
-  const dim3 grid(static_cast<unsigned>((chunks + kThreads - 1) / kThreads), kv_heads, 2 * table_rows);
-  return k_exp ? launch(read_kernel<true>, grid, kThreads, p, stream, "kv_read")
-               : launch(read_kernel<false>, grid, kThreads, p, stream, "kv_read");
+  const dim3 grid(static_cast<unsigned>((max_length + 63) / 64), kv_heads, table_rows);
+  auto go = [&](auto kernel) { return launch(kernel, grid, kThreads, stream, "kv_read", p); };
+  switch (dim) {
+    case 64: return k_exp ? go(read_kernel<64, true>) : go(read_kernel<64, false>);
+    case 128: return k_exp ? go(read_kernel<128, true>) : go(read_kernel<128, false>);
+    case 192: return k_exp ? go(read_kernel<192, true>) : go(read_kernel<192, false>);
+    default: return k_exp ? go(read_kernel<256, true>) : go(read_kernel<256, false>);
+  }
 }

@@ -524,22 +524,41 @@ def _(logits, lse, token, eos_id, semantic_begin, score):
 
 
 # ----------------------------------------------------------------------------- rotary positions and the paged cache
-def _same_device(first: Tensor, *ts: Optional[Tensor]) -> None:
-    _require_cuda(first, *ts)
+# These ops take a few microseconds on the device, less than torch.library's dispatch of a Python op (20 us, 45 us with
+# mutated arguments). So `rope`, `kv_write`, `kv_read` and `paged_attention` call their kernels directly where nothing
+# has to see the call as an operator, and go through torch.ops.dm3.* under tracing, for tensor subclasses (fake
+# tensors among them) and where autograd would have to be told that there is no gradient.
+def _plain(*ts: Optional[Tensor]) -> bool:
+    if torch.compiler.is_compiling():
+        return False
     for t in ts:
-        if t is not None and t.device != first.device:
-            raise RuntimeError(f"tensors on {first.device} and {t.device} in one call")
+        if t is not None and (type(t) is not Tensor or t.requires_grad):
+            return False
+    return True
 
 
-def _launch(device: torch.device, name: str, *args) -> None:
+def _same_device(first: Tensor, *ts: Optional[Tensor]) -> int:
+    d = first.get_device()
+    for t in ts:
+        if t is not None and t.get_device() != d:
+            raise RuntimeError("drama3_b200 ops run on CUDA tensors only (no CPU fallback), all on one device: got "
+                               f"{first.device} and {t.device}")
+    if d < 0:
+        raise RuntimeError("drama3_b200 ops run on CUDA tensors only (no CPU fallback)")
+    return d
+
+
+def _launch(device: int, name: str, *args) -> None:
     """Calls a C entry point on the device's current stream, with that device current."""
     fn = getattr(_lib.load(), name)
-    if device.index == torch.cuda.current_device():
-        rc = fn(*args, _stream(device))
+    stream = torch._C._cuda_getCurrentRawStream(device)
+    if device == torch._C._cuda_getDevice():
+        rc = fn(*args, stream)
     else:
         with torch.cuda.device(device):
-            rc = fn(*args, _stream(device))
-    _lib.check(rc, name)
+            rc = fn(*args, stream)
+    if rc:
+        _lib.check(rc, name)
 
 
 def _heads(t: Tensor, name: str) -> Tensor:
@@ -547,13 +566,14 @@ def _heads(t: Tensor, name: str) -> Tensor:
     they are, other layouts are copied."""
     if t.dtype != BF16 or t.dim() != 3:
         raise RuntimeError(f"{name} must be bf16 [tokens, heads, dim]")
-    if t.stride(2) != 1 or t.stride(0) % 8 or t.stride(1) % 8 or t.data_ptr() % 16:
+    a, b, c = t.stride()
+    if c != 1 or a % 8 or b % 8 or t.data_ptr() % 16:
         t = t.clone(memory_format=torch.contiguous_format)
     return t
 
 
 def _int64(t: Tensor, n: int, name: str) -> Tensor:
-    if t.dtype != torch.int64 or t.dim() != 1 or t.shape[0] != n:
+    if t.dtype != torch.int64 or t.shape != (n,):
         raise RuntimeError(f"{name} must be int64 [{n}]")
     return t.contiguous()
 
@@ -567,40 +587,41 @@ def _angles(inv_freq: Tensor) -> Tensor:
 def _cache_args(k_cache: Tensor, v_cache: Tensor, k_exp: Optional[Tensor], v_exp: Optional[Tensor], table: Tensor,
                 status: Tensor):
     """((k, v, page stride, k_exp, v_exp, exp stride), (pages, page_size), (kv_heads, dim), table arguments)."""
-    if k_cache.dim() != 4 or k_cache.shape != v_cache.shape or k_cache.dtype != v_cache.dtype:
+    shape, strides = k_cache.shape, k_cache.stride()
+    if len(shape) != 4 or shape != v_cache.shape or k_cache.dtype != v_cache.dtype:
         raise RuntimeError("the cache must be two [pages, kv_heads, page_size, dim] buffers of one type")
-    pages, heads, size, dim = k_cache.shape
-    inner = (size * dim, dim, 1)
-    if k_cache.stride() != v_cache.stride() or k_cache.stride()[1:] != inner:
+    pages, heads, size, dim = shape
+    if strides != v_cache.stride() or strides[1:] != (size * dim, dim, 1):
         raise RuntimeError("each page of the cache must be contiguous, with the same strides for keys and values")
+    k_at = v_at = None
+    exp_stride = 0
     if k_exp is None and v_exp is None:
         if k_cache.dtype != BF16:
             raise RuntimeError("a cache without exponents must be bf16")
-        exp_stride = 0
     else:
         if k_exp is None or v_exp is None or k_cache.dtype not in (E4M3, torch.uint8):
             raise RuntimeError("a quantised cache is float8_e4m3fn (or uint8) with exponents for keys and values")
         for e in (k_exp, v_exp):
-            if e.dtype != torch.int8 or e.shape != k_cache.shape[:3] or e.stride()[1:] != (size, 1):
+            if e.dtype != torch.int8 or e.shape != shape[:3] or e.stride()[1:] != (size, 1):
                 raise RuntimeError("exponents must be int8 [pages, kv_heads, page_size], each page contiguous")
-        if k_exp.stride(0) != v_exp.stride(0):
-            raise RuntimeError("key and value exponents must have the same strides")
         exp_stride = k_exp.stride(0)
-    if table.dtype != torch.int32 or table.dim() != 2 or (table.shape[1] > 1 and table.stride(1) != 1):
+        if exp_stride != v_exp.stride(0):
+            raise RuntimeError("key and value exponents must have the same strides")
+        k_at, v_at = k_exp.data_ptr(), v_exp.data_ptr()
+    if table.dtype != torch.int32 or table.dim() != 2:
+        raise RuntimeError("the page table must be int32 [rows, pages a row] with unit column stride")
+    rows, per_row = table.shape
+    step, col = table.stride()
+    if per_row > 1 and col != 1:
         raise RuntimeError("the page table must be int32 [rows, pages a row] with unit column stride")
     if status.dtype != torch.int32 or status.numel() != 1:
         raise RuntimeError("status must be one int32")
-    rows, per_row = table.shape
-    return ((_ptr(k_cache), _ptr(v_cache), k_cache.stride(0), _ptr(k_exp), _ptr(v_exp), exp_stride), (pages, size),
-            (heads, dim), (_ptr(table), max(table.stride(0), per_row), rows, per_row))
+    return ((k_cache.data_ptr(), v_cache.data_ptr(), strides[0], k_at, v_at, exp_stride), (pages, size), (heads, dim),
+            (table.data_ptr(), step if step > per_row else per_row, rows, per_row))
 
 
-@torch.library.custom_op("dm3::rope", mutates_args=())
-def rope(x: Tensor, positions: Tensor, inv_freq: Tensor, interleaved: bool = False, factor: float = 1.0) -> Tensor:
-    """Rotary positions: x bf16 [T, heads, dim] with the first 2 * len(inv_freq) values of every head turned
-    in pairs by positions[t] * inv_freq[i] (formed in 64 bits), times factor. Pair i is (2i, 2i + 1) when
-    interleaved, else (i, i + len(inv_freq)). positions int64 [T], inv_freq float64 (see `Rope`)."""
-    _same_device(x, positions, inv_freq)
+def _rope(x: Tensor, positions: Tensor, inv_freq: Tensor, interleaved: bool = False, factor: float = 1.0) -> Tensor:
+    dev = _same_device(x, positions, inv_freq)
     if x.dtype != BF16 or x.dim() != 3:
         raise RuntimeError("x must be bf16 [tokens, heads, dim]")
     if x.stride(2) != 1:
@@ -608,17 +629,70 @@ def rope(x: Tensor, positions: Tensor, inv_freq: Tensor, interleaved: bool = Fal
     T, heads, dim = x.shape
     positions, inv_freq = _int64(positions, T, "positions"), _angles(inv_freq)
     y = torch.empty((T, heads, dim), dtype=BF16, device=x.device)
-    _launch(x.device, "dm3_rope", _ptr(x), T, heads, dim, x.stride(0), x.stride(1), _ptr(positions), _ptr(inv_freq),
-            2 * inv_freq.shape[0], 1 if interleaved else 0, factor, _ptr(y))
+    _launch(dev, "dm3_rope", x.data_ptr(), T, heads, dim, x.stride(0), x.stride(1), positions.data_ptr(),
+            inv_freq.data_ptr(), 2 * inv_freq.shape[0], 1 if interleaved else 0, factor, y.data_ptr())
     return y
 
 
-@rope.register_fake
+_rope_op = torch.library.custom_op("dm3::rope", _rope, mutates_args=())
+
+
+@_rope_op.register_fake
 def _(x, positions, inv_freq, interleaved=False, factor=1.0):
     return x.new_empty(x.shape)
 
 
-@torch.library.custom_op("dm3::kv_write", mutates_args=("k_cache", "v_cache", "k_exp", "v_exp", "status"))
+def rope(x: Tensor, positions: Tensor, inv_freq: Tensor, interleaved: bool = False, factor: float = 1.0) -> Tensor:
+    """Rotary positions: x bf16 [T, heads, dim] with the first 2 * len(inv_freq) values of every head turned
+    in pairs by positions[t] * inv_freq[i] (formed in 64 bits), times factor. Pair i is (2i, 2i + 1) when
+    interleaved, else (i, i + len(inv_freq)). positions int64 [T], inv_freq float64 (see `Rope`)."""
+    return (_rope if _plain(x, positions, inv_freq) else _rope_op)(x, positions, inv_freq, interleaved, factor)
+
+
+def _kv_write(k: Tensor, v: Tensor, positions: Tensor, table: Tensor, k_cache: Tensor, v_cache: Tensor,
+              k_exp: Optional[Tensor], v_exp: Optional[Tensor], status: Tensor, rows: Optional[Tensor] = None,
+              q: Optional[Tensor] = None, inv_freq: Optional[Tensor] = None, interleaved: bool = False,
+              factor: float = 1.0) -> Tensor:
+    dev = _same_device(k, v, positions, table, k_cache, v_cache, k_exp, v_exp, status, rows, q, inv_freq)
+    held, (pages, size), (heads, dim), tab = _cache_args(k_cache, v_cache, k_exp, v_exp, table, status)
+    k, v = _heads(k, "k"), _heads(v, "v")
+    T = k.shape[0]
+    if k.shape != (T, heads, dim) or v.shape != k.shape:
+        raise RuntimeError(f"k and v must be [T, {heads}, {dim}] as the cache")
+    positions = _int64(positions, T, "positions")
+    q_at = rows_at = inv_at = None
+    q_heads = q_ts = q_hs = rot = 0
+    if rows is not None:
+        rows = _int64(rows, T, "rows")
+        rows_at = rows.data_ptr()
+    if q is not None:
+        q = _heads(q, "q")
+        q_heads = q.shape[1]
+        if q.shape != (T, q_heads, dim):
+            raise RuntimeError(f"q must be [{T}, heads, {dim}]")
+        out = torch.empty((T, q_heads, dim), dtype=BF16, device=k.device)
+        q_at, (q_ts, q_hs, _) = q.data_ptr(), q.stride()
+    else:
+        out = torch.empty((0,), dtype=BF16, device=k.device)
+    if inv_freq is not None:
+        inv_freq = _angles(inv_freq)
+        inv_at, rot = inv_freq.data_ptr(), 2 * inv_freq.shape[0]
+    _launch(dev, "dm3_kv_write", q_at, q_heads, q_ts, q_hs, k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(),
+            v.stride(0), v.stride(1), T, heads, dim, rows_at, positions.data_ptr(), *tab, *held, pages, size, inv_at, rot,
+            1 if interleaved else 0, factor, out.data_ptr(), status.data_ptr())
+    return out
+
+
+_kv_write_op = torch.library.custom_op("dm3::kv_write", _kv_write,
+                                       mutates_args=("k_cache", "v_cache", "k_exp", "v_exp", "status"))
+
+
+@_kv_write_op.register_fake
+def _(k, v, positions, table, k_cache, v_cache, k_exp, v_exp, status, rows=None, q=None, inv_freq=None, interleaved=False,
+      factor=1.0):
+    return k.new_empty((0,)) if q is None else q.new_empty(q.shape)
+
+
 def kv_write(k: Tensor, v: Tensor, positions: Tensor, table: Tensor, k_cache: Tensor, v_cache: Tensor,
              k_exp: Optional[Tensor], v_exp: Optional[Tensor], status: Tensor, rows: Optional[Tensor] = None,
              q: Optional[Tensor] = None, inv_freq: Optional[Tensor] = None, interleaved: bool = False,
@@ -629,66 +703,71 @@ def kv_write(k: Tensor, v: Tensor, positions: Tensor, table: Tensor, k_cache: Te
     multiple of 16 values). A token with a negative row or position is padding: it is not cached and its
     query is zeros. Two tokens of one call must not share a place. See `KVCache` for the buffers; status
     collects skipped tokens (bit 4) whose place or page lies outside the table or the cache."""
-    _same_device(k, v, positions, table, k_cache, v_cache, k_exp, v_exp, status, rows, q, inv_freq)
+    return (_kv_write if _plain(k, v, q, k_cache, v_cache) else _kv_write_op)(
+        k, v, positions, table, k_cache, v_cache, k_exp, v_exp, status, rows, q, inv_freq, interleaved, factor)
+
+
+def _kv_read(k_cache: Tensor, v_cache: Tensor, k_exp: Optional[Tensor], v_exp: Optional[Tensor], table: Tensor,
+             lengths: Tensor, max_length: int, status: Tensor) -> tuple[Tensor, Tensor]:
+    dev = _same_device(k_cache, v_cache, k_exp, v_exp, table, lengths, status)
     held, (pages, size), (heads, dim), tab = _cache_args(k_cache, v_cache, k_exp, v_exp, table, status)
-    k, v = _heads(k, "k"), _heads(v, "v")
-    T = k.shape[0]
-    if tuple(k.shape) != (T, heads, dim) or v.shape != k.shape:
-        raise RuntimeError(f"k and v must be [T, {heads}, {dim}] as the cache")
-    positions = _int64(positions, T, "positions")
-    if rows is not None:
-        rows = _int64(rows, T, "rows")
-    q_heads = 0
-    if q is not None:
-        q = _heads(q, "q")
-        q_heads = q.shape[1]
-        if q.shape[0] != T or q.shape[2] != dim:
-            raise RuntimeError(f"q must be [{T}, heads, {dim}]")
-        out = torch.empty((T, q_heads, dim), dtype=BF16, device=k.device)
-    else:
-        out = torch.empty((0,), dtype=BF16, device=k.device)
-    rot = 0
-    if inv_freq is not None:
-        inv_freq = _angles(inv_freq)
-        rot = 2 * inv_freq.shape[0]
-    _launch(k.device, "dm3_kv_write", _ptr(q), q_heads, q.stride(0) if q_heads else 0, q.stride(1) if q_heads else 0,
-            _ptr(k), k.stride(0), k.stride(1), _ptr(v), v.stride(0), v.stride(1), T, heads, dim, _ptr(rows),
-            _ptr(positions), *tab, *held, pages, size, _ptr(inv_freq), rot, 1 if interleaved else 0, factor, _ptr(out),
-            _ptr(status))
-    return out
-
-
-@kv_write.register_fake
-def _(k, v, positions, table, k_cache, v_cache, k_exp, v_exp, status, rows=None, q=None, inv_freq=None, interleaved=False,
-      factor=1.0):
-    return k.new_empty((0,)) if q is None else q.new_empty(q.shape)
-
-
-@torch.library.custom_op("dm3::kv_read", mutates_args=("status",))
-def kv_read(k_cache: Tensor, v_cache: Tensor, k_exp: Optional[Tensor], v_exp: Optional[Tensor], table: Tensor,
-            lengths: Tensor, max_length: int, status: Tensor) -> tuple[Tensor, Tensor]:
-    """The first min(lengths[r], max_length) tokens of every row of a paged cache as dense bf16 (keys, values)
-    [rows, kv_heads, max_length, dim], exactly the values that the cache stands for, and zeros behind them."""
-    _same_device(k_cache, v_cache, k_exp, v_exp, table, lengths, status)
-    held, (pages, size), (heads, dim), tab = _cache_args(k_cache, v_cache, k_exp, v_exp, table, status)
-    rows = table.shape[0]
+    rows = tab[2]
     if max_length < 0:
         raise RuntimeError("max_length must not be negative")
     lengths = _int64(lengths, rows, "lengths")
     k = torch.empty((rows, heads, max_length, dim), dtype=BF16, device=k_cache.device)
     v = torch.empty_like(k)
-    _launch(k.device, "dm3_kv_read", *held, pages, size, heads, dim, *tab, _ptr(lengths), max_length, _ptr(k), _ptr(v),
-            _ptr(status))
+    _launch(dev, "dm3_kv_read", *held, pages, size, heads, dim, *tab, lengths.data_ptr(), max_length, k.data_ptr(),
+            v.data_ptr(), status.data_ptr())
     return k, v
 
 
-@kv_read.register_fake
+_kv_read_op = torch.library.custom_op("dm3::kv_read", _kv_read, mutates_args=("status",))
+
+
+@_kv_read_op.register_fake
 def _(k_cache, v_cache, k_exp, v_exp, table, lengths, max_length, status):
     shape = (table.shape[0], k_cache.shape[1], max_length, k_cache.shape[3])
     return k_cache.new_empty(shape, dtype=BF16), k_cache.new_empty(shape, dtype=BF16)
 
 
-@torch.library.custom_op("dm3::paged_attention", mutates_args=("status",))
+def kv_read(k_cache: Tensor, v_cache: Tensor, k_exp: Optional[Tensor], v_exp: Optional[Tensor], table: Tensor,
+            lengths: Tensor, max_length: int, status: Tensor) -> tuple[Tensor, Tensor]:
+    """The first min(lengths[r], max_length) tokens of every row of a paged cache as dense bf16 (keys, values)
+    [rows, kv_heads, max_length, dim], exactly the values that the cache stands for, and zeros behind them."""
+    return (_kv_read if _plain(k_cache, v_cache) else _kv_read_op)(k_cache, v_cache, k_exp, v_exp, table, lengths,
+                                                                   max_length, status)
+
+
+def _paged_attention(q: Tensor, k_cache: Tensor, v_cache: Tensor, k_exp: Optional[Tensor], v_exp: Optional[Tensor],
+                     table: Tensor, lengths: Tensor, status: Tensor, scale: Optional[float] = None,
+                     window: int = 0) -> tuple[Tensor, Tensor]:
+    dev = _same_device(q, k_cache, v_cache, k_exp, v_exp, table, lengths, status)
+    held, (pages, size), (heads, dim), tab = _cache_args(k_cache, v_cache, k_exp, v_exp, table, status)
+    q = _heads(q, "q")
+    rows, q_heads = tab[2], q.shape[1]
+    if q.shape != (rows, q_heads, dim):
+        raise RuntimeError(f"q must be [{rows}, heads, {dim}]")
+    lengths = _int64(lengths, rows, "lengths")
+    out = torch.empty((rows, q_heads, dim), dtype=BF16, device=q.device)
+    lse = torch.empty((rows, q_heads), dtype=torch.float32, device=q.device)
+    # scratch from the caller's allocator: calls on other streams and in other graphs have their own
+    nbytes = _lib.load().dm3_paged_attention_workspace_bytes(rows, q_heads, heads, dim, size, tab[3])
+    ws = torch.empty((nbytes,), dtype=torch.uint8, device=q.device) if nbytes else None
+    _launch(dev, "dm3_paged_attention", q.data_ptr(), q.stride(0), q.stride(1), q_heads, *held, pages, size, heads, dim, *tab,
+            lengths.data_ptr(), dim ** -0.5 if scale is None else scale, window, out.data_ptr(), lse.data_ptr(),
+            status.data_ptr(), None if ws is None else ws.data_ptr(), nbytes)
+    return out, lse
+
+
+_paged_attention_op = torch.library.custom_op("dm3::paged_attention", _paged_attention, mutates_args=("status",))
+
+
+@_paged_attention_op.register_fake
+def _(q, k_cache, v_cache, k_exp, v_exp, table, lengths, status, scale=None, window=0):
+    return q.new_empty(q.shape), q.new_empty(q.shape[:2], dtype=torch.float32)
+
+
 def paged_attention(q: Tensor, k_cache: Tensor, v_cache: Tensor, k_exp: Optional[Tensor], v_exp: Optional[Tensor],
                     table: Tensor, lengths: Tensor, status: Tensor, scale: Optional[float] = None,
                     window: int = 0) -> tuple[Tensor, Tensor]:
@@ -698,23 +777,5 @@ def paged_attention(q: Tensor, k_cache: Tensor, v_cache: Tensor, k_exp: Optional
     Returns (out bf16 [rows, q_heads, dim], lse fp32 [rows, q_heads], the natural log of the sum of exp).
     A row that sees nothing gives zeros and -inf. The launch is laid out for the table's width, so a
     narrower view of it (table[:, :n]) makes a shorter call."""
-    _same_device(q, k_cache, v_cache, k_exp, v_exp, table, lengths, status)
-    held, (pages, size), (heads, dim), tab = _cache_args(k_cache, v_cache, k_exp, v_exp, table, status)
-    q = _heads(q, "q")
-    rows, q_heads = table.shape[0], q.shape[1]
-    if q.shape[0] != rows or q.shape[2] != dim:
-        raise RuntimeError(f"q must be [{rows}, heads, {dim}]")
-    lengths = _int64(lengths, rows, "lengths")
-    out = torch.empty((rows, q_heads, dim), dtype=BF16, device=q.device)
-    lse = torch.empty((rows, q_heads), dtype=torch.float32, device=q.device)
-    nbytes = _lib.load().dm3_paged_attention_workspace_bytes(rows, q_heads, heads, dim, size, tab[3])
-    ws = torch.empty((nbytes,), dtype=torch.uint8, device=q.device) if nbytes else None
-    _launch(q.device, "dm3_paged_attention", _ptr(q), q.stride(0), q.stride(1), q_heads, *held, pages, size, heads, dim,
-            *tab, _ptr(lengths), dim ** -0.5 if scale is None else scale, window, _ptr(out), _ptr(lse), _ptr(status),
-            _ptr(ws), nbytes)
-    return out, lse
-
-
-@paged_attention.register_fake
-def _(q, k_cache, v_cache, k_exp, v_exp, table, lengths, status, scale=None, window=0):
-    return q.new_empty(q.shape), q.new_empty(q.shape[:2], dtype=torch.float32)
+    return (_paged_attention if _plain(q, k_cache, v_cache) else _paged_attention_op)(
+        q, k_cache, v_cache, k_exp, v_exp, table, lengths, status, scale, window)

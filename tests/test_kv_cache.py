@@ -135,7 +135,7 @@ BAD = {
                  dict(positions=None), dict(inv_freq=None), dict(y=None), dict(heads=1 << 20)],
     "dm3_kv_write": BAD_CACHE + [dict(T=-1), dict(q_heads=-1), dict(rot=24), dict(rot=80), dict(inv_freq=None), dict(k=None), dict(v=None),
                                  dict(positions=None), dict(q=None), dict(q_out=None), dict(k=ODD), dict(q=ODD), dict(v_ts=129), dict(q_out=ODD)],
-    "dm3_kv_read": BAD_CACHE + [dict(max_length=-1), dict(lengths=None), dict(k_out=None), dict(v_out=ODD), dict(table_rows=40000)],
+    "dm3_kv_read": BAD_CACHE + [dict(max_length=-1), dict(lengths=None), dict(k_out=None), dict(v_out=ODD), dict(table_rows=70000)],
     "dm3_paged_attention": BAD_CACHE + [dict(q_heads=3), dict(q_heads=1), dict(q_heads=0), dict(window=-1), dict(scale=math.nan),
                                         dict(scale=math.inf), dict(q=None), dict(lengths=None), dict(out=None), dict(lse=None), dict(q=ODD),
                                         dict(q_rs=250), dict(out=ODD), dict(table_rows=70000)],
