@@ -17,6 +17,7 @@
 #include <cmath>
 #include <cstdint>
 #include <string>
+#include <type_traits>
 
 #include "dm3.h"
 #include "dm3_common.cuh"
@@ -103,9 +104,10 @@ struct Where {
   int a, b;
   bool turned;
 };
-__device__ __forceinline__ Where where(int i, int rot, int interleaved) {
+template <bool kInter>
+__device__ __forceinline__ Where where(int i, int rot) {
   const bool turned = i * 16 < rot;
-  return turned && !interleaved ? Where{i, i + rot / 16, true} : Where{2 * i, 2 * i + 1, turned};
+  return turned && !kInter ? Where{i, i + rot / 16, true} : Where{2 * i, 2 * i + 1, turned};
 }
 
 // The angles of a CTA's tokens: pair 8i + 2k + e of token t at [t][k][i][e], so neighbouring threads read
@@ -133,8 +135,8 @@ __device__ __forceinline__ float exact_turn(float a, float b, float ch, float cl
 }
 
 // Turns the 16 values of unit i in place. angles: of the token.
-template <bool kExact>
-__device__ __forceinline__ void turn(Chunk& x, Chunk& y, int i, const float2* high, const float2* low, int rot, int interleaved) {
+template <bool kExact, bool kInter>
+__device__ __forceinline__ void turn(Chunk& x, Chunk& y, int i, const float2* high, const float2* low, int rot) {
   const int units = rot / 16;
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
@@ -150,7 +152,7 @@ __device__ __forceinline__ void turn(Chunk& x, Chunk& y, int i, const float2* hi
         b = kExact ? exact_turn(b0, -a0, ch, cl, sh, sl) : b0 * ch + a0 * sh;
       };
       const int j = 2 * k + e;
-      if (!interleaved)
+      if (!kInter)
         pair(x.v[j], y.v[j]);
       else if (k < 2)
         pair(x.v[2 * j], x.v[2 * j + 1]);
@@ -163,41 +165,47 @@ __device__ __forceinline__ void turn(Chunk& x, Chunk& y, int i, const float2* hi
 // ------------------------------------------------------------------ rope
 // A CTA takes a block of tokens (and a share of their rows, blockIdx.y, when there are few tokens), a thread 16
 // values of a row at a time, two rows' loads in flight.
-__global__ void __launch_bounds__(kThreads) rope_kernel(const __grid_constant__ RopeParams p, const Div per, const Div heads) {
+// A row belongs to 2^shift neighbouring lanes (dim / 16 of them at work), so a thread keeps its place in the row.
+template <bool kInter>
+__global__ void __launch_bounds__(kThreads, 4) rope_kernel(const __grid_constant__ RopeParams p, const int shift, const Div heads) {
   __shared__ __align__(16) float2 cs[kAngles];
   griddep_launch();
   griddep_wait();
   const int64_t t0 = static_cast<int64_t>(blockIdx.x) * p.block;
   const int tokens = p.T - t0 < p.block ? static_cast<int>(p.T - t0) : p.block;
+  constexpr int kBatch = 2;
+  const int i = threadIdx.x & ((1 << shift) - 1), segs = kThreads >> shift, total = tokens * p.x.n;
+  const Where w = where<kInter>(i, p.rot);
+  const bool mine = i < p.dim / 16;
+  uint4 ra[kBatch], rb[kBatch];
+  int t[kBatch], row[kBatch];
+  auto load = [&](int base) {
+#pragma unroll
+    for (int b = 0; b < kBatch; ++b) {
+      row[b] = base + b * segs + (threadIdx.x >> shift);
+      if (row[b] < total && mine) {
+        t[b] = heads(row[b]);
+        const __nv_bfloat16* src = p.x.p + (t0 + t[b]) * p.x.ts + (row[b] - t[b] * p.x.n) * p.x.hs;
+        ra[b] = __ldcs(reinterpret_cast<const uint4*>(src + w.a * 8));
+        rb[b] = __ldcs(reinterpret_cast<const uint4*>(src + w.b * 8));
+      }
+    }
+  };
+  load(blockIdx.y * segs * kBatch);  // on its way while the angles are found
   fill_angles<false>(cs, nullptr, tokens, p.positions + t0, p.inv_freq, p.rot, p.factor);
   __syncthreads();
-  constexpr int kBatch = 2;
-  const int total = tokens * p.x.n * (p.dim / 16), step = blockDim.x * gridDim.y;
-  for (int u0 = blockIdx.y * blockDim.x + threadIdx.x; u0 < total; u0 += step * kBatch) {
-    uint4 ra[kBatch], rb[kBatch];
-    Where w[kBatch];
-    int t[kBatch], i[kBatch], row[kBatch];
+  for (int base = blockIdx.y * segs * kBatch; base < total;) {
 #pragma unroll
     for (int b = 0; b < kBatch; ++b) {
-      const int u = u0 + b * step;
-      if (u >= total) break;
-      row[b] = per(u);
-      i[b] = u - row[b] * per.n;
-      t[b] = heads(row[b]);
-      const __nv_bfloat16* src = p.x.p + (t0 + t[b]) * p.x.ts + (row[b] - t[b] * static_cast<int>(heads.n)) * p.x.hs;
-      w[b] = where(i[b], p.rot, p.interleaved);
-      ra[b] = __ldcs(reinterpret_cast<const uint4*>(src + w[b].a * 8));
-      rb[b] = __ldcs(reinterpret_cast<const uint4*>(src + w[b].b * 8));
-    }
-#pragma unroll
-    for (int b = 0; b < kBatch; ++b) {
-      if (u0 + b * step >= total) break;
+      if (row[b] >= total || !mine) break;
       Chunk x = unpack(ra[b]), y = unpack(rb[b]);
-      if (w[b].turned) turn<false>(x, y, i[b], cs + t[b] * (p.rot / 2), nullptr, p.rot, p.interleaved);
+      if (w.turned) turn<false, kInter>(x, y, i, cs + t[b] * (p.rot / 2), nullptr, p.rot);
       __nv_bfloat16* dst = p.y + (t0 * p.x.n + row[b]) * p.dim;
-      *reinterpret_cast<uint4*>(dst + w[b].a * 8) = pack(x);
-      *reinterpret_cast<uint4*>(dst + w[b].b * 8) = pack(y);
+      *reinterpret_cast<uint4*>(dst + w.a * 8) = pack(x);
+      *reinterpret_cast<uint4*>(dst + w.b * 8) = pack(y);
     }
+    base += gridDim.y * segs * kBatch;
+    if (base < total) load(base);
   }
 }
 
@@ -235,24 +243,27 @@ struct WriteParams {
   const int64_t* positions;
   Cache c;
   const double* inv_freq;
-  int rot, interleaved;  // rot = 0: no rotary positions
+  int rot;  // 0: no rotary positions
   double factor;
 };
 
-// 8 values as e4m3 codes of 2^-e; what is not finite becomes NaN.
+// 8 values as e4m3 codes of 1 / scale.
 __device__ __forceinline__ uint2 encode(const Chunk& x, float scale) {
   uint32_t w[2];
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    float f[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const float a = x.v[4 * i + j];
-      f[j] = isfinite(a) ? a * scale : NAN;
-    }
-    w[i] = pack_e4m3x2(f[0], f[1]) | static_cast<uint32_t>(pack_e4m3x2(f[2], f[3])) << 16;
-  }
+  for (int i = 0; i < 2; ++i)
+    w[i] = pack_e4m3x2(x.v[4 * i] * scale, x.v[4 * i + 1] * scale) |
+           static_cast<uint32_t>(pack_e4m3x2(x.v[4 * i + 2] * scale, x.v[4 * i + 3] * scale)) << 16;
   return make_uint2(w[0], w[1]);
+}
+
+// The largest magnitude's bits of 16 bf16 values (magnitudes order as their bits do).
+__device__ __forceinline__ uint32_t max_magnitude(uint4 a, uint4 b) {
+  const uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+  uint32_t m = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) m = __vmaxu2(m, w[i] & 0x7fff7fffu);
+  return max(m & 0xffffu, m >> 16);
 }
 
 // The exponent of a row whose largest finite magnitude is amax: the smallest e with amax <= 448 * 2^e
@@ -267,8 +278,8 @@ __device__ __forceinline__ int row_exponent(float amax) {
 // As rope_kernel, over the rows of q, k and v. A row belongs to kSeg neighbouring lanes, so the amax of a quantised
 // row is a few shuffles. A quantised key is turned to 2^-46: it is the code of the exactly turned key, whichever call
 // wrote it (in 32 bits about one value in 10^6 would fall on the other side of a code's border).
-template <int kSeg, bool kQuant>
-__global__ void __launch_bounds__(kThreads) write_kernel(const __grid_constant__ WriteParams p, const Div rows_of) {
+template <int kSeg, bool kQuant, bool kInter>
+__global__ void __launch_bounds__(kThreads, 4) write_kernel(const __grid_constant__ WriteParams p, const Div rows_of) {
   __shared__ __align__(16) float2 high[kAngles], low[kQuant ? kAngles : 1];
   __shared__ int64_t s_at[kBlockTokens], s_exp[kBlockTokens];  // place of a token's row of head 0; -1: not cached
   __shared__ bool s_pad[kBlockTokens];
@@ -276,31 +287,13 @@ __global__ void __launch_bounds__(kThreads) write_kernel(const __grid_constant__
   griddep_wait();
   const int64_t t0 = static_cast<int64_t>(blockIdx.x) * p.block;
   const int tokens = p.T - t0 < p.block ? static_cast<int>(p.T - t0) : p.block;
-  // a place is found by the last threads, while the first ones are at the angles
-  if (const int t = kThreads - 1 - threadIdx.x; t < tokens) {
-    const int64_t pos = p.positions[t0 + t], r = p.rows ? p.rows[t0 + t] : t0 + t;
-    const bool padding = pos < 0 || r < 0;
-    int64_t at = -1, x = 0;
-    if (!padding) {
-      const int64_t nth = pos / p.c.page_size, in = pos - nth * p.c.page_size;
-      const int64_t page = r < p.c.rows && nth < p.c.per_row ? p.c.table[r * p.c.table_stride + nth] : -1;
-      if (page >= 0 && page < p.c.pages)
-        at = page * p.c.page_stride + in * p.dim, x = page * p.c.exp_stride + in;
-      else
-        set_status(p.c.status, STATUS_BAD_PAGE);
-    }
-    s_at[t] = at, s_exp[t] = x, s_pad[t] = padding;
-  }
-  if (p.rot) fill_angles<kQuant>(high, low, tokens, p.positions + t0, p.inv_freq, p.rot, p.factor);
-  __syncthreads();
   constexpr int kSegs = kThreads / kSeg, kBatch = 2;
   const int i = threadIdx.x % kSeg, n = p.q.n + 2 * p.k.n, total = tokens * n;
-  const Where w = where(i, p.rot, p.interleaved);
+  const Where w = where<kInter>(i, p.rot);
   const bool mine = i < p.dim / 16;
-  // all lanes of a warp make the same number of rounds: the shuffles need them
-  for (int base = blockIdx.y * kSegs * kBatch; base < total; base += gridDim.y * kSegs * kBatch) {
-    uint4 ra[kBatch], rb[kBatch];
-    int t[kBatch], head[kBatch], side[kBatch];  // side 0: query, 1: key, 2: value, -1: none
+  uint4 ra[kBatch], rb[kBatch];
+  int t[kBatch], head[kBatch], side[kBatch];  // side 0: query, 1: key, 2: value, -1: none
+  auto load = [&](int base) {
 #pragma unroll
     for (int b = 0; b < kBatch; ++b) {
       const int r = base + b * kSegs + threadIdx.x / kSeg;
@@ -319,15 +312,36 @@ __global__ void __launch_bounds__(kThreads) write_kernel(const __grid_constant__
         rb[b] = __ldcs(reinterpret_cast<const uint4*>(row + w.b * 8));
       }
     }
+  };
+  load(blockIdx.y * kSegs * kBatch);  // on its way while the angles and places are found
+  // a place is found by the last threads, while the first ones are at the angles
+  if (const int t = kThreads - 1 - threadIdx.x; t < tokens) {
+    const int64_t pos = p.positions[t0 + t], r = p.rows ? p.rows[t0 + t] : t0 + t;
+    const bool padding = pos < 0 || r < 0;
+    int64_t at = -1, x = 0;
+    if (!padding) {
+      const int64_t nth = pos / p.c.page_size, in = pos - nth * p.c.page_size;
+      const int64_t page = r < p.c.rows && nth < p.c.per_row ? p.c.table[r * p.c.table_stride + nth] : -1;
+      if (page >= 0 && page < p.c.pages)
+        at = page * p.c.page_stride + in * p.dim, x = page * p.c.exp_stride + in;
+      else
+        set_status(p.c.status, STATUS_BAD_PAGE);
+    }
+    s_at[t] = at, s_exp[t] = x, s_pad[t] = padding;
+  }
+  if (p.rot) fill_angles<kQuant>(high, low, tokens, p.positions + t0, p.inv_freq, p.rot, p.factor);
+  __syncthreads();
+  // all lanes of a warp make the same number of rounds: the shuffles need them
+  for (int base = blockIdx.y * kSegs * kBatch; base < total;) {
 #pragma unroll
     for (int b = 0; b < kBatch; ++b) {
       Chunk x = unpack(ra[b]), y = unpack(rb[b]);
       if (w.turned && (side[b] == 0 || side[b] == 1)) {
         const int at = t[b] * (p.rot / 2);
         if (kQuant && side[b] == 1)
-          turn<kQuant>(x, y, i, high + at, low + at, p.rot, p.interleaved);
+          turn<kQuant, kInter>(x, y, i, high + at, low + at, p.rot);
         else
-          turn<false>(x, y, i, high + at, nullptr, p.rot, p.interleaved);
+          turn<false, kInter>(x, y, i, high + at, nullptr, p.rot);
       }
       const uint4 px = pack(x), py = pack(y);
       if (side[b] == 0) {
@@ -346,21 +360,33 @@ __global__ void __launch_bounds__(kThreads) write_kernel(const __grid_constant__
         }
         continue;
       }
+      if (!__any_sync(0xffffffffu, side[b] > 0)) continue;
+      uint32_t top = max_magnitude(px, py);
+#pragma unroll
+      for (int o = kSeg / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
       x = unpack(px), y = unpack(py);  // the key as a bf16 cache would hold it
-      float amax = 0.f;
+      if (__any_sync(0xffffffffu, top >= 0x7f80u)) {  // infinities and NaN: not counted, and NaN in the cache
+        float amax = 0.f;
 #pragma unroll
-      for (int j = 0; j < 8; ++j)
-        amax = fmaxf(amax, fmaxf(isfinite(x.v[j]) ? fabsf(x.v[j]) : 0.f, isfinite(y.v[j]) ? fabsf(y.v[j]) : 0.f));
+        for (int j = 0; j < 8; ++j) {
+          amax = fmaxf(amax, fmaxf(isfinite(x.v[j]) ? fabsf(x.v[j]) : 0.f, isfinite(y.v[j]) ? fabsf(y.v[j]) : 0.f));
+          if (!isfinite(x.v[j])) x.v[j] = NAN;
+          if (!isfinite(y.v[j])) y.v[j] = NAN;
+        }
 #pragma unroll
-      for (int o = kSeg / 2; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+        for (int o = kSeg / 2; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+        top = __float_as_uint(amax) >> 16;
+      }
       if (place >= 0) {
-        const int e = row_exponent(amax);
+        const int e = row_exponent(__uint_as_float(top << 16));
         uint8_t* dst = static_cast<uint8_t*>(side[b] == 1 ? p.c.k : p.c.v) + place + static_cast<int64_t>(head[b]) * p.c.page_size * p.dim;
         *reinterpret_cast<uint2*>(dst + w.a * 8) = encode(x, exp2i(-e));
         *reinterpret_cast<uint2*>(dst + w.b * 8) = encode(y, exp2i(-e));
         if (i == 0) (side[b] == 1 ? p.c.k_exp : p.c.v_exp)[s_exp[t[b]] + static_cast<int64_t>(head[b]) * p.c.page_size] = static_cast<int8_t>(e);
       }
     }
+    base += gridDim.y * kSegs * kBatch;
+    if (base < total) load(base);
   }
 }
 
@@ -373,13 +399,12 @@ struct ReadParams {
   __nv_bfloat16* out[2];  // [rows][heads][L][dim]
 };
 
-// blockIdx = (64 tokens, head, row): where their four tiles of 16 lie is looked up once, then a thread moves 16 output
-// bytes at a time, dim / 32 of them in flight.
-template <int kDim, bool kQuant>
+// blockIdx = (kTokens tokens, head, row): where their tiles of 16 lie is looked up once, then a thread moves 16 output
+// bytes at a time, kTokens * dim / 2048 of them in flight.
+template <int kDim, bool kQuant, int kTokens>
 __global__ void __launch_bounds__(kThreads) read_kernel(const __grid_constant__ ReadParams p) {
-  constexpr int kTokens = 64, kTiles = kTokens / 16, kPer = kDim / 8, kRounds = kTokens * kPer / kThreads;
-  __shared__ int64_t s_at[kTiles];  // place of a tile's rows; -1: none
-  __shared__ float s_scale[2][kQuant ? kTokens : 1];
+  constexpr int kTiles = kTokens / 16, kPer = kDim / 8, kRounds = (kTokens * kPer + kThreads - 1) / kThreads;
+  __shared__ int64_t s_at[kTiles], s_exp[kQuant ? kTiles : 1];  // place of a tile's rows (-1: none) and exponents
   griddep_launch();
   griddep_wait();
   const int row = blockIdx.z, head = blockIdx.y, tid = threadIdx.x;
@@ -390,25 +415,21 @@ __global__ void __launch_bounds__(kThreads) read_kernel(const __grid_constant__ 
     if (tid == 0) set_status(p.c.status, STATUS_BAD_PAGE);
   }
   if (n > p.L) n = p.L;
-  // every thread of a tile's 16 finds the tile; one of them notes it
-  if (tid < (kQuant ? 2 : 1) * kTokens) {
-    const int side = tid / kTokens, in = tid % kTokens;
-    const int64_t tok = first + in;
-    int64_t at = -1;
-    float scale = 0.f;
-    if (tok - in % 16 < n) {
+  if (tid < kTiles) {
+    const int64_t tok = first + tid * 16;
+    int64_t at = -1, x = 0;
+    if (tok < n) {
       const int64_t nth = tok / p.c.page_size;
       const int64_t page = p.c.table[row * p.c.table_stride + nth];
       if (page < 0 || page >= p.c.pages) {
         set_status(p.c.status, STATUS_BAD_PAGE);
       } else {
         const int64_t r = static_cast<int64_t>(head) * p.c.page_size + (tok - nth * p.c.page_size);
-        at = page * p.c.page_stride + (r - in % 16) * kDim;
-        if (kQuant && tok < n) scale = exp2i((side ? p.c.v_exp : p.c.k_exp)[page * p.c.exp_stride + r]);
+        at = page * p.c.page_stride + r * kDim, x = page * p.c.exp_stride + r;
       }
     }
-    if (side == 0 && in % 16 == 0) s_at[in / 16] = at;
-    if (kQuant) s_scale[side][in] = scale;
+    s_at[tid] = at;
+    if (kQuant) s_exp[tid] = x;
   }
   __syncthreads();
 #pragma unroll
@@ -417,13 +438,13 @@ __global__ void __launch_bounds__(kThreads) read_kernel(const __grid_constant__ 
 #pragma unroll
     for (int i = 0; i < kRounds; ++i) {
       const int u = i * kThreads + tid, tok = u / kPer, c = u % kPer;
-      const int64_t at = s_at[tok / 16];
+      const int64_t at = tok < kTokens ? s_at[tok / 16] : -1;
       r[i] = make_uint4(0, 0, 0, 0);
       if (at >= 0 && first + tok < n) {
         const int64_t x = at + tok % 16 * kDim + c * 8;
         if (kQuant) {
           const uint2 w = __ldcs(reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(side ? p.c.v : p.c.k) + x));
-          r[i].x = w.x, r[i].y = w.y;
+          r[i] = make_uint4(w.x, w.y, static_cast<uint32_t>((side ? p.c.v_exp : p.c.k_exp)[s_exp[tok / 16] + tok % 16]), 0);
         } else {
           r[i] = __ldcs(reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(side ? p.c.v : p.c.k) + x));
         }
@@ -433,9 +454,9 @@ __global__ void __launch_bounds__(kThreads) read_kernel(const __grid_constant__ 
 #pragma unroll
     for (int i = 0; i < kRounds; ++i) {
       const int u = i * kThreads + tid, tok = u / kPer;
-      if (first + tok >= p.L) break;
+      if (tok >= kTokens || first + tok >= p.L) break;
       if (kQuant) {
-        const float s = s_scale[side][tok];
+        const float s = exp2i(static_cast<int>(r[i].z));
         Chunk x;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
@@ -526,14 +547,17 @@ extern "C" int dm3_rope(const void* x, int T, int heads, int dim, int64_t ts, in
   if (!x || !positions || !inv_freq || !y) return set_error("rope: null pointer"), DM3_EINVAL;
   RopeParams p{{static_cast<const __nv_bfloat16*>(x), ts, hs, heads}, static_cast<__nv_bfloat16*>(y), T, dim, 1, positions,
                inv_freq, rot, interleaved, factor};
-  // 16 bytes a thread at a time where rows and pairs fall on them, and a block's rows are counted in 16 bits
-  const int units = dim / 16 * heads;
-  const bool wide = dim % 16 == 0 && rot % 16 == 0 && units < 65536 / kBlockTokens && aligned(p.x) && reinterpret_cast<uintptr_t>(y) % 16 == 0;
+  // 16 bytes a thread at a time where rows and pairs fall on them, a row has at most a CTA's lanes, and a block's rows
+  // are counted in 16 bits
+  const bool wide = dim % 16 == 0 && rot % 16 == 0 && dim <= 16 * kThreads && heads <= 65535 / kBlockTokens && aligned(p.x) &&
+                    reinterpret_cast<uintptr_t>(y) % 16 == 0;
   if (wide) {
-    const Blocks b = blocks(T, rot, (units + 2 * kThreads - 1) / (2 * kThreads));
+    int shift = 0;
+    while (16 << shift < dim) ++shift;
+    const int round = 2 * (kThreads >> shift);
+    const Blocks b = blocks(T, rot, (heads + round - 1) / round);
     p.block = b.tokens;
-    const int threads = b.tokens > 1 || units >= kThreads ? kThreads : (units + 31) / 32 * 32;
-    return launch(rope_kernel, dim3((T + b.tokens - 1) / b.tokens, b.shares), threads, stream, "rope", p, Div(dim / 16), Div(heads));
+    return launch(interleaved ? rope_kernel<true> : rope_kernel<false>, dim3((T + b.tokens - 1) / b.tokens, b.shares), kThreads, stream, "rope", p, shift, Div(heads));
   }
   const Blocks b = blocks(T, 0, (heads * dim + kThreads - 1) / kThreads);
   return launch(rope_any_kernel, dim3(T, b.shares), kThreads, stream, "rope", p);
@@ -561,15 +585,21 @@ extern "C" int dm3_kv_write(const void* q, int q_heads, int64_t q_ts, int64_t q_
     return set_error("kv_write: rows must start on 16 bytes"), DM3_EINVAL;
   p.y = static_cast<__nv_bfloat16*>(q_out);
   p.T = T, p.dim = dim, p.rows = rows, p.positions = positions;
-  p.inv_freq = inv_freq, p.rot = rot, p.interleaved = interleaved, p.factor = factor;
+  p.inv_freq = inv_freq, p.rot = rot, p.factor = factor;
   const int seg = dim == 64 ? 4 : dim == 128 ? 8 : 16, round = 2 * kThreads / seg, n = q_heads + 2 * kv_heads;
   if (n > 65535 / kBlockTokens) return set_error("kv_write: too many heads"), DM3_EINVAL;
   const Blocks b = blocks(T, rot, (n + round - 1) / round);
   p.block = b.tokens;
   const dim3 grid((T + b.tokens - 1) / b.tokens, b.shares);
   auto go = [&](auto kernel) { return launch(kernel, grid, kThreads, stream, "kv_write", p, Div(n)); };
-  if (k_exp) return seg == 4 ? go(write_kernel<4, true>) : seg == 8 ? go(write_kernel<8, true>) : go(write_kernel<16, true>);
-  return seg == 4 ? go(write_kernel<4, false>) : seg == 8 ? go(write_kernel<8, false>) : go(write_kernel<16, false>);
+  auto pick = [&](auto lanes) {
+    constexpr int kSeg = decltype(lanes)::value;
+    if (k_exp) return interleaved ? go(write_kernel<kSeg, true, true>) : go(write_kernel<kSeg, true, false>);
+    return interleaved ? go(write_kernel<kSeg, false, true>) : go(write_kernel<kSeg, false, false>);
+  };
+  return seg == 4   ? pick(std::integral_constant<int, 4>{})
+         : seg == 8 ? pick(std::integral_constant<int, 8>{})
+                    : pick(std::integral_constant<int, 16>{});
 }
 
 extern "C" int dm3_kv_read(const void* k_cache, const void* v_cache, int64_t page_stride, const int8_t* k_exp,
@@ -588,12 +618,21 @@ extern "C" int dm3_kv_read(const void* k_cache, const void* v_cache, int64_t pag
     return set_error("kv_read: null or misaligned pointer"), DM3_EINVAL;
   p.heads = kv_heads, p.lengths = lengths, p.L = max_length;
   p.out[0] = static_cast<__nv_bfloat16*>(k_out), p.out[1] = static_cast<__nv_bfloat16*>(v_out);
-  const dim3 grid(static_cast<unsigned>((max_length + 63) / 64), kv_heads, table_rows);
+  // 64 tokens a CTA; 16 where that leaves SMs idle (5 rows of 1,237 tokens, 2 heads of 256: 5.9 and 4.7 us)
+  int dev = 0;
+  cudaGetDevice(&dev);
+  const bool few = (max_length + 63) / 64 * kv_heads * table_rows < 2 * sm_count(dev);
+  const dim3 grid(static_cast<unsigned>(few ? (max_length + 15) / 16 : (max_length + 63) / 64), kv_heads, table_rows);
   auto go = [&](auto kernel) { return launch(kernel, grid, kThreads, stream, "kv_read", p); };
+  auto pick = [&](auto d) {
+    constexpr int kDim = decltype(d)::value;
+    if (k_exp) return few ? go(read_kernel<kDim, true, 16>) : go(read_kernel<kDim, true, 64>);
+    return few ? go(read_kernel<kDim, false, 16>) : go(read_kernel<kDim, false, 64>);
+  };
   switch (dim) {
-    case 64: return k_exp ? go(read_kernel<64, true>) : go(read_kernel<64, false>);
-    case 128: return k_exp ? go(read_kernel<128, true>) : go(read_kernel<128, false>);
-    case 192: return k_exp ? go(read_kernel<192, true>) : go(read_kernel<192, false>);
-    default: return k_exp ? go(read_kernel<256, true>) : go(read_kernel<256, false>);
+    case 64: return pick(std::integral_constant<int, 64>{});
+    case 128: return pick(std::integral_constant<int, 128>{});
+    case 192: return pick(std::integral_constant<int, 192>{});
+    default: return pick(std::integral_constant<int, 256>{});
   }
 }
