@@ -68,7 +68,7 @@ SIGNATURES = {
     "dm3_kv_write": (_i, [_p, _i, _i64, _i64, _p, _i64, _i64, _p, _i64, _i64, _i, _i, _i, _p, _p, _p, _i64, _i, _i, _p,
                           _p, _i64, _p, _p, _i64, _i, _i, _p, _i, _i, _f64, _p, _p, _p]),
     "dm3_kv_read": (_i, [_p, _p, _i64, _p, _p, _i64, _i, _i, _i, _i, _p, _i64, _i, _i, _p, _i64, _p, _p, _p, _p]),
-    "dm3_paged_attention_workspace_bytes": (_sz, [_i, _i, _i, _i, _i, _i]),
+    "dm3_paged_attention_workspace_bytes": (_sz, [_i, _i, _i, _i, _i, _i, _i, _i64]),
     "dm3_paged_attention": (_i, [_p, _i64, _i64, _i, _p, _p, _i64, _p, _p, _i64, _i, _i, _i, _i, _p, _i64, _i, _i, _p,
                                  _f32, _i64, _p, _p, _p, _p, _sz, _p]),
     "dm3_last_launch_count": (_i, []),

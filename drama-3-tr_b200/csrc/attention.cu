@@ -18,9 +18,12 @@
 // Every warp walks its own 16-token tiles, the next keys loading while the softmax and the values' product
 // run; the warps of a CTA join in shared memory at the end.
 //
-// Long rows are split: `splits` CTAs share a row's tiles evenly (the device reads the length, so one captured
-// graph serves all lengths), each leaves (M, l, O) in fp32, and a second kernel joins them in order: no atomics,
-// the same answer every time.
+// Rows are split over CTAs by the lengths that the device reads, so one captured graph serves all lengths, in one of two
+// ways (plan() says when); neither uses atomics, and the order of every sum is fixed by the lengths alone.
+//   * Clusters: `splits` CTAs of a cluster share a row's tiles and join over distributed shared memory: one launch,
+//     for short rows.
+//   * Stream: the tiles of all rows and heads are one sequence, cut into equal shares for two CTAs an SM whatever the
+//     rows' lengths; a CTA leaves (M, l, O) in fp32 of a row that it shares, and a second kernel joins them.
 //
 // An e4m3 row is code * 2^e. For keys 2^e joins the logit's scale. For values it joins the weight's exponent:
 // w_t = 2^(s_t + e_t - M) with M the running maximum of s_t + e_t, so weights are in fp16's range whatever the rows'
@@ -44,6 +47,7 @@ namespace attn {
 using kv::Cache;
 
 constexpr int kWarps = 4;
+constexpr int kMaxCluster = 8;
 constexpr int kTile = 16;  // tokens of one tile; pages hold whole tiles
 // The maximum is raised only when a logit exceeds it by more than kSlack (log2): weights reach 2^kSlack. fp16
 // weights carry 2^kLift besides, so that they stay normal down to 2^-(14 + kLift).
@@ -57,31 +61,43 @@ struct Params {
   const int64_t* lengths;
   float scale_log2;  // scale * log2(e)
   int64_t window;
-  int splits, min_tiles;
+  int splits;          // CTAs of a cluster; 0: stream
   __nv_bfloat16* out;  // [rows][q_heads][dim]
   float* lse;          // [rows][q_heads]
-  float* part_o;       // [rows][q_heads][splits][dim]
-  float2* part_ml;     // [rows][q_heads][splits]
+  // stream: the first tile of each row in the sequence and their number ([rows + 1], a tile counted once a head unit),
+  // and what a CTA leaves of the row that it starts in ([2 * cta]) and of the one that it ends in ([2 * cta + 1])
+  int64_t* row_at;
+  float* part_o;    // [2 * ctas][heads of a unit][dim]
+  float2* part_ml;  // [2 * ctas][heads of a unit]
 };
 
-// The tiles that a row sees, and how many of them each split takes.
+// The tokens and tiles that a row sees.
 struct Span {
   int64_t first, n;  // tokens seen: [first, n)
   int64_t tile0;     // tile of the first one
-  int64_t tiles, chunk;
+  int64_t tiles;
+  bool cut;  // the length lies behind the table
 };
-__device__ __forceinline__ Span row_span(const Params& p, int row) {
+__device__ __forceinline__ Span row_span(const Params& p, int64_t row) {
   Span s;
   const int64_t cap = static_cast<int64_t>(p.c.per_row) * p.c.page_size;
   s.n = p.lengths[row];
+  s.cut = s.n > cap;
   if (s.n > cap) s.n = cap;
   if (s.n < 0) s.n = 0;
   s.first = p.window > 0 && s.n > p.window ? s.n - p.window : 0;
   s.tile0 = s.first / kTile;
   s.tiles = (s.n + kTile - 1) / kTile - s.tile0;
-  s.chunk = (s.tiles + p.splits - 1) / p.splits;
-  if (s.chunk < p.min_tiles) s.chunk = p.min_tiles;
   return s;
+}
+// Quotients of what hardly ever needs 64 bits
+__device__ __forceinline__ int64_t div(int64_t a, int64_t b) {
+  return ((a | b) >> 32) == 0 ? static_cast<int64_t>(static_cast<uint32_t>(a) / static_cast<uint32_t>(b)) : a / b;
+}
+// Tiles of a CTA's share of the sequence: equal ones, but a tile for each warp, or a whole unit where units are shorter.
+__device__ __forceinline__ int64_t share_of(int64_t tiles, int rows, int units, int ctas) {
+  const int64_t q = div(tiles * units + ctas - 1, ctas), unit = div(tiles, rows), least = unit < 1 ? 1 : unit < kWarps ? unit : kWarps;
+  return q < least ? least : q;
 }
 
 // D[16x8] += A[16x16] B[16x8], fp32 accumulators; lane (g = lane / 4, q = lane % 4) holds A rows g, g + 8 at columns
@@ -141,11 +157,11 @@ struct Shape {
   static constexpr int kBox = kRow % 128 ? 64 : 128, kBoxes = kRow / kBox;
   static constexpr int kTileBytes = kTile * kRow;
   // Shared memory: a ring of kRing units a warp (a step's keys, its values, the next step's keys, ...), the
-  // queries, the units' exponents, ranges and barriers, the join's maxima and sums. The join reuses the ring.
+  // queries, the units' exponents, ranges and barriers, the join's maxima, sums and factors. The join reuses the ring.
   static constexpr int kUnit = kU * kTileBytes;
   static constexpr int kQBytes = kNT * kDim * 16;  // 8 * kNT heads of kDim 16-bit values
   static constexpr int kSide = (kQuant ? kU * 32 : 0) + kU * 4 + 8 + 4;  // a unit's exponents, ranges and barrier
-  static constexpr int kStats = (2 * kWarps + 1) * kHeads * 4;
+  static constexpr int kStats = (2 * kWarps + 1 + kMaxCluster) * kHeads * 4;
   // Two CTAs an SM: few warps with much to do at once did better than more of them with smaller steps and fewer
   // registers (96 ragged rows, 16 heads a cache head, e4m3: 74.6 us; three CTAs and half the step 80.6, four 88.6)
   static constexpr int kRoom = 112 * 1024 - kQBytes - kStats - 1024;  // 1024: aligning the ring
@@ -161,6 +177,87 @@ struct Shape {
 template <int kBox>
 __device__ __forceinline__ int token_of(int lr) {
   return kBox == 128 ? ((lr ^ lr >> 2) & 1) << 2 | (lr & 2) | lr >> 2 : lr;
+}
+
+__device__ __forceinline__ float lse_of(float m, float l, bool quant) {  // natural log of the sum, from log2 units
+  return l == 0.f ? -INFINITY : (m - (quant ? kLift : 0.f) + log2f(l)) * 0.69314718055994531f;
+}
+
+__device__ __forceinline__ bool elect_one() {  // true in one lane of the warp
+  uint32_t r;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
+  return r != 0;
+}
+
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ uint32_t in_cta(const float* p, int rank) {  // the place of p in another CTA of the cluster
+  uint32_t r;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_u32(p)), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ float ld_cluster(const float* p, int rank) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(in_cta(p, rank)) : "memory");
+  return v;
+}
+__device__ __forceinline__ float2 ld_cluster2(const float* p, int rank) {
+  float2 v;
+  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(in_cta(p, rank)) : "memory");
+  return v;
+}
+
+// Stream: counts the rows' tiles and finds where this CTA's share of the sequence begins; CTA 0 leaves the rows' places for
+// the join. All threads call it; scratch: 11 words. False when the CTA has no share.
+__device__ __forceinline__ bool find_share(const Params& p, int units, int64_t* scratch, int64_t& row, int& unit, int64_t& begin,
+                                           int64_t& left) {
+  constexpr int kThreads = kWarps * 32;
+  int64_t *const s_sum = scratch, *const s_hit = scratch + kWarps;  // s_hit: the row found, its place, its tiles
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, rows = p.c.rows;
+  int64_t total = 0, mine = 0, upto = 0;  // this thread's row of a block of 128: its tiles, and the sum up to it
+  if (threadIdx.x == 0) s_hit[0] = -1;
+  auto scan = [&](int r0) {
+    mine = r0 + static_cast<int>(threadIdx.x) < rows ? row_span(p, r0 + threadIdx.x).tiles : 0;
+    upto = mine;
+#pragma unroll
+    for (int w = 1; w < 32; w *= 2) {
+      const int64_t x = __shfl_up_sync(0xffffffffu, upto, w);
+      if (lane >= w) upto += x;
+    }
+    __syncthreads();
+    if (lane == 31) s_sum[warp] = upto;
+    __syncthreads();
+    upto += total;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      if (w < warp) upto += s_sum[w];
+      total += s_sum[w];
+    }
+  };
+  for (int r0 = 0; r0 < rows; r0 += kThreads) {
+    scan(r0);
+    if (blockIdx.x == 0 && r0 + threadIdx.x < rows) p.row_at[r0 + threadIdx.x] = upto - mine;
+  }
+  if (blockIdx.x == 0 && threadIdx.x == 0) p.row_at[rows] = total;
+  const int64_t share = share_of(total, rows, units, gridDim.x), from = blockIdx.x * share;
+  if (from >= total * units) return false;
+  left = min(share, total * units - from);
+  if (rows > kThreads) total = 0;  // block by block again, up to the one that holds `from`
+  for (int r0 = 0; r0 < rows; r0 += kThreads) {
+    if (rows > kThreads) scan(r0);
+    const int64_t at = (upto - mine) * units;
+    if (mine > 0 && from >= at && from < upto * units) s_hit[0] = r0 + threadIdx.x, s_hit[1] = at, s_hit[2] = mine;
+    if (from < total * units) break;
+  }
+  __syncthreads();
+  row = s_hit[0];
+  if (row < 0) return false;
+  const int64_t in = from - s_hit[1];
+  unit = static_cast<int>(div(in, s_hit[2]));
+  begin = in - unit * s_hit[2];
+  __syncthreads();  // the scratch is free
+  return true;
 }
 
 template <int kDim, bool kQuant, int kNT, int kU>
@@ -183,76 +280,124 @@ __global__ void __launch_bounds__(kWarps * 32, 2)
   float* const s_qs = s_m[2 * kWarps];
   if (lane == 0) {
 #pragma unroll
-    for (int i = 0; i < C::kRing; ++i) mbar_init(&full[i], kU);
+    for (int i = 0; i < C::kRing; ++i) mbar_init(&full[i], 1);
     fence_mbar_init();
   }
   __syncwarp();
 
-  const int split = blockIdx.x, kvh = blockIdx.y / p.head_tiles, ht = blockIdx.y % p.head_tiles, row = blockIdx.z;
-  const int h0 = ht * C::kHeads;  // first head of the group
   griddep_launch();
   griddep_wait();
   fence_proxy_async();  // the cache's rows may have been written just before; the copies read them
-  const Span sp = row_span(p, row);
-  const int64_t begin = split * sp.chunk;  // tiles of this CTA, counted from sp.tile0
-  const int64_t end = begin + sp.chunk < sp.tiles ? begin + sp.chunk : sp.tiles;
-  const int64_t qrow = static_cast<int64_t>(row) * p.q_heads + kvh * p.group + h0;  // output row of head 0
-  if (p.lengths[row] > sp.n && threadIdx.x == 0) kv::set_status(p.c.status, STATUS_BAD_PAGE);
-  if (begin >= end) {
-    if (split == 0) {  // a row that sees nothing
-      for (int i = threadIdx.x; i < C::kHeads * kDim; i += blockDim.x)
-        if (h0 + i / kDim < p.group) p.out[qrow * kDim + i] = __float2bfloat16_rn(0.f);
-      if (threadIdx.x < C::kHeads && h0 + threadIdx.x < p.group) p.lse[qrow + threadIdx.x] = -INFINITY;
+  const int units = p.kv_heads * p.head_tiles;  // of a row
+  // The segment at hand: tiles [begin, end) of a row and unit, counted from the row's first tile seen.
+  int64_t row, begin, end;
+  int unit;
+  Span sp;
+  int64_t left = 0;             // stream: tiles of this CTA's share from the segment on
+  int part = 0;                 // stream: segments done
+  if (p.splits) {
+    row = blockIdx.z, unit = blockIdx.y;
+    sp = row_span(p, row);
+    const int64_t chunk = max((sp.tiles + p.splits - 1) / p.splits, static_cast<int64_t>(kWarps));
+    begin = min(blockIdx.x * chunk, sp.tiles);
+    end = min(begin + chunk, sp.tiles);
+    if (sp.cut && threadIdx.x == 0) kv::set_status(p.c.status, STATUS_BAD_PAGE);
+  } else {
+    // CTAs take the rows in turn to write what one without tokens gives, and to report lengths behind the table
+    for (row = blockIdx.x; row < p.c.rows; row += gridDim.x) {
+      sp = row_span(p, row);
+      if (sp.cut && threadIdx.x == 0) kv::set_status(p.c.status, STATUS_BAD_PAGE);
+      if (sp.tiles) continue;
+      const int64_t at = row * p.q_heads;
+      for (int i = threadIdx.x; i < p.q_heads * kDim; i += blockDim.x) p.out[at * kDim + i] = __float2bfloat16_rn(0.f);
+      for (int i = threadIdx.x; i < p.q_heads; i += blockDim.x) p.lse[at + i] = -INFINITY;
     }
-    return;
+    if (!find_share(p, units, reinterpret_cast<int64_t*>(s_m), row, unit, begin, left)) return;
+    sp = row_span(p, row);
+    end = min(begin + left, sp.tiles);
   }
-
-  // A warp's steps: kU tiles each, warps in turn. Lane i of a block of 32 tiles knows where the block's tile i lies,
-  // and asks for it.
-  constexpr int kBlock = 32 / kU;  // steps a block
-  int steps = static_cast<int>((end - begin - warp * kU + kWarps * kU - 1) / (kWarps * kU));  // 0 where fewer tiles than warps
+  uint8_t* const ring = smem + warp * C::kRing * C::kUnit;
+  int slot = 0;  // of the ring's next unit, and its barrier's parity
+  uint32_t parity = 0;
+  const int tok = token_of<C::kBox>(lr), sw = C::kBox == 128 ? tok : tok >> 1;  // the lane's token of a key tile, its swizzle
+  int vtok[2];                                                                    // its tokens of a value tile (and + 8)
+#pragma unroll
+  for (int i = 0; i < 2; ++i) vtok[i] = token_of<C::kBox>(2 * lc + i);
   const int per_page = p.c.page_size / kTile;
+
+  for (;;) {
+  const int kvh = unit / p.head_tiles, h0 = unit % p.head_tiles * C::kHeads;  // h0: first head of the group
+  const int64_t qrow = row * p.q_heads + kvh * p.group + h0;                   // output row of head h0
+  // A warp's steps: kU tiles each, tiles going to the warps in turn. Lane i of a block of 32 tiles knows where the
+  // block's tile i lies, and asks for it.
+  constexpr int kBlock = 32 / kU;  // steps a block
+  const int mine = static_cast<int>((end - begin - warp + kWarps - 1) / kWarps);  // tiles of this warp
+  int steps = mine > 0 ? (mine + kU - 1) / kU : 0;
   int page, y, range;  // y: first row of the tile in its page
   auto find = [&](int step0) {
-    const int64_t t = begin + (static_cast<int64_t>(step0 + lane / kU) * kWarps + warp) * kU + lane % kU;
+    const int64_t t = begin + (static_cast<int64_t>(step0) * kU + lane) * kWarps + warp;
     int tile = 0;
     page = 0, range = 0;
-    if (t < end) {
-      const int64_t g = sp.tile0 + t, nth = g / per_page, t0 = g * kTile;
+    if (t < end && lane < kBlock * kU) {
+      const int64_t g = sp.tile0 + t, nth = div(g, per_page), t0 = g * kTile;
       tile = static_cast<int>(g - nth * per_page);
       page = p.c.table[row * p.c.table_stride + nth];
-      if (page < 0 || page >= p.c.pages) {
-        page = 0;
+      if (page < 0 || page >= p.c.pages)
         kv::set_status(p.c.status, STATUS_BAD_PAGE);
-      } else {
+      else
         range = (sp.first > t0 ? static_cast<int>(sp.first - t0) : 0) | (sp.n - t0 < kTile ? static_cast<int>(sp.n - t0) : kTile) << 8;
-      }
     }
     y = kvh * p.c.page_size + tile * kTile;
   };
   find(0);
 
-  uint8_t* const ring = smem + warp * C::kRing * C::kUnit;
-  auto ask = [&](bool keys, int step, int slot) {
+  auto ask = [&](bool keys, int step, int to_slot) {
     if (step >= steps) return;
     if (keys && step % kBlock == 0 && step > 0) find(step);
-    const int u = lane - (step % kBlock) * kU;
-    if (u >= 0 && u < kU) {
-      uint8_t* const to = ring + slot * C::kUnit + u * C::kTileBytes;
-      s_range[slot][u] = range;
-      mbar_arrive_expect_tx(&full[slot], C::kTileBytes + (kQuant && keys ? 32 : 0));
+    int pg[kU], yy[kU], rg[kU];
 #pragma unroll
-      for (int b = 0; b < C::kBoxes; ++b)
-        tc::tma_load_3d(to + b * kTile * C::kBox, keys ? &kmap : &vmap, b * C::kBox, y, page, &full[slot]);
-      if (kQuant && keys) {
-        const int64_t x = page * p.c.exp_stride + y;
-        bulk_g2s(s_exp[slot][u], p.c.k_exp + x, 16, &full[slot]);
-        bulk_g2s(s_exp[slot][u] + 16, p.c.v_exp + x, 16, &full[slot]);
+    for (int u = 0; u < kU; ++u) {
+      const int from = step % kBlock * kU + u;
+      pg[u] = __shfl_sync(0xffffffffu, page, from), yy[u] = __shfl_sync(0xffffffffu, y, from), rg[u] = __shfl_sync(0xffffffffu, range, from);
+    }
+    if (elect_one()) {
+      int tiles = 0;
+#pragma unroll
+      for (int u = 0; u < kU; ++u) {
+        s_range[to_slot][u] = rg[u];
+        tiles += rg[u] != 0;
+      }
+      mbar_arrive_expect_tx(&full[to_slot], tiles * (C::kTileBytes + (kQuant && keys ? 32 : 0)));
+#pragma unroll
+      for (int u = 0; u < kU; ++u) {
+        if (rg[u] == 0) continue;  // nothing there: no copy, the place keeps what it held, to be masked
+        uint8_t* const to = ring + to_slot * C::kUnit + u * C::kTileBytes;
+#pragma unroll
+        for (int b = 0; b < C::kBoxes; ++b)
+          tc::tma_load_3d(to + b * kTile * C::kBox, keys ? &kmap : &vmap, b * C::kBox, yy[u], pg[u], &full[to_slot]);
+        if (kQuant && keys) {
+          const int64_t x = pg[u] * p.c.exp_stride + yy[u];
+          bulk_g2s(s_exp[to_slot][u], p.c.k_exp + x, 16, &full[to_slot]);
+          bulk_g2s(s_exp[to_slot][u] + 16, p.c.v_exp + x, 16, &full[to_slot]);
+        }
       }
     }
+    __syncwarp();
   };
 #pragma unroll
-  for (int i = 0; i < C::kRing; ++i) ask(!(i & 1), i / 2, i);
+  for (int i = 0; i < C::kRing; ++i) ask(!(i & 1), i / 2, slot + i < C::kRing ? slot + i : slot + i - C::kRing);
+
+  // Stream: the unit behind this one, its length on its way while this one is worked on (the share ends before the rows do)
+  int64_t next_row = row;
+  int next_unit = unit + 1;
+  Span next_sp = sp;
+  if (left > end - begin && next_unit == units) {
+    next_unit = 0;
+    do {
+      if (++next_row >= p.c.rows) return;
+      next_sp = row_span(p, next_row);
+    } while (next_sp.tiles == 0);
+  }
 
   // Queries as B operands, in the permutation of dim that 16-byte key copies give; warp nt prepares tile nt.
   if (warp < kNT) {
@@ -299,12 +444,6 @@ __global__ void __launch_bounds__(kWarps * 32, 2)
     for (int h = 0; h < 2; ++h) m[nt][h] = -INFINITY, sub[nt][h] = 0.f, l[nt][h] = 0.f, qs[nt][h] = s_qs[nt * 8 + 2 * lc + h];
   }
 
-  const int tok = token_of<C::kBox>(lr), sw = C::kBox == 128 ? tok : tok >> 1;  // the lane's token of a key tile, its swizzle
-  int vtok[2];                                                                    // its tokens of a value tile (and + 8)
-#pragma unroll
-  for (int i = 0; i < 2; ++i) vtok[i] = token_of<C::kBox>(2 * lc + i);
-  int slot = 0;
-  uint32_t parity = 0;
   // The unit in the current slot has landed; when the wait ran out, no more are asked for.
   auto landed = [&](int step) {
     if (__any_sync(0xffffffffu, !mbar_wait(&full[slot], parity))) {
@@ -538,8 +677,9 @@ __global__ void __launch_bounds__(kWarps * 32, 2)
       if (lr == 0) s_m[warp][nt * 8 + 2 * lc + h] = m[nt][h], s_l[warp][nt * 8 + 2 * lc + h] = l[nt][h];
     }
   __syncthreads();
-  const bool whole = sp.tiles <= sp.chunk;
-  if (threadIdx.x < C::kHeads) {  // each warp's factor into s_m, 1 / sum (or 1) into s_qs
+  const bool whole = p.splits ? p.splits == 1 : begin == 0 && end == sp.tiles;
+  const int64_t to = 2 * static_cast<int64_t>(blockIdx.x) + (part ? 1 : 0);  // stream: where a shared row's part goes
+  if (threadIdx.x < C::kHeads) {  // each warp's factor into s_m, the joined sum and maximum into s_l[0], s_l[1]
     const int h = threadIdx.x;
     float mm = -INFINITY, ll = 0.f;
 #pragma unroll
@@ -550,12 +690,12 @@ __global__ void __launch_bounds__(kWarps * 32, 2)
       ll += s_l[w][h] * f;
       s_m[w][h] = f;
     }
+    s_l[0][h] = ll, s_l[1][h] = mm;
     s_qs[h] = whole ? (ll == 0.f ? 0.f : 1.f / ll) : 1.f;
-    if (h0 + h < p.group) {
-      if (whole)
-        p.lse[qrow + h] = ll == 0.f ? -INFINITY : (mm - (kQuant ? kLift : 0.f) + log2f(ll)) * 0.69314718055994531f;
-      else
-        p.part_ml[(qrow + h) * p.splits + split] = make_float2(mm, ll);
+    if (whole) {
+      if (h0 + h < p.group) p.lse[qrow + h] = lse_of(mm, ll, kQuant);
+    } else if (!p.splits) {
+      p.part_ml[to * C::kHeads + h] = make_float2(mm, ll);
     }
   }
   // (value d of both heads of a pair) at d with its low bits turned by lr, so that neither these writes (lanes kE
@@ -570,60 +710,103 @@ __global__ void __launch_bounds__(kWarps * 32, 2)
         *reinterpret_cast<float2*>(&s_o[warp][nt * 4 + lc][(d ^ (lr & 3)) * 2]) = make_float2(o[nt][i][2 * r], o[nt][i][2 * r + 1]);
       }
   __syncthreads();
+  auto place = [&](int d) { return (d ^ (d / C::kE & 3)) * 2; };
+  auto put = [&](int h, int d, float x, float y) {
+    if (h0 + h < p.group) p.out[(qrow + h) * kDim + d] = __float2bfloat16_rn(x);
+    if (h0 + h + 1 < p.group) p.out[(qrow + h + 1) * kDim + d] = __float2bfloat16_rn(y);
+  };
   for (int i = threadIdx.x; i < C::kHeads / 2 * kDim; i += blockDim.x) {
     const int hp = i / kDim, d = i % kDim, h = 2 * hp;
-    if (h0 + h >= p.group) break;
     float x = 0.f, y = 0.f;
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) {
-      const float2 v = *reinterpret_cast<const float2*>(&s_o[w][hp][(d ^ (d / C::kE & 3)) * 2]);
+      const float2 v = *reinterpret_cast<const float2*>(&s_o[w][hp][place(d)]);
       const float2 f = *reinterpret_cast<const float2*>(&s_m[w][h]);
       x += v.x * f.x, y += v.y * f.y;
     }
     x *= s_qs[h], y *= s_qs[h + 1];
-    const bool both = h0 + h + 1 < p.group;
     if (whole) {
-      p.out[(qrow + h) * kDim + d] = __float2bfloat16_rn(x);
-      if (both) p.out[(qrow + h + 1) * kDim + d] = __float2bfloat16_rn(y);
+      put(h, d, x, y);
+    } else if (p.splits) {
+      *reinterpret_cast<float2*>(&s_o[0][hp][place(d)]) = make_float2(x, y);  // read by this thread alone so far
     } else {
-      float* to = p.part_o + ((qrow + h) * p.splits + split) * kDim + d;
-      to[0] = x;
-      if (both) to[static_cast<int64_t>(p.splits) * kDim] = y;
+      float* dst = p.part_o + (to * C::kHeads + h) * kDim + d;
+      dst[0] = x, dst[kDim] = y;
     }
+  }
+  if (p.splits) {
+    if (p.splits == 1) return;
+    // every CTA of the cluster joins its part of the values
+    const int rank = blockIdx.x;
+    float(*const s_f)[C::kHeads] = s_m + 2 * kWarps + 1;  // [splits]
+    cluster_sync();
+    if (threadIdx.x < C::kHeads) {
+      const int h = threadIdx.x;
+      float mm = -INFINITY, ll = 0.f;
+      for (int r = 0; r < p.splits; ++r) {
+        s_f[r][h] = ld_cluster(&s_l[1][h], r);
+        mm = fmaxf(mm, s_f[r][h]);
+      }
+      for (int r = 0; r < p.splits; ++r) {
+        const float f = s_f[r][h] == -INFINITY ? 0.f : ex2(s_f[r][h] - mm);
+        ll += ld_cluster(&s_l[0][h], r) * f;
+        s_f[r][h] = f;
+      }
+      s_qs[h] = ll == 0.f ? 0.f : 1.f / ll;
+      if (rank == 0 && h0 + h < p.group) p.lse[qrow + h] = lse_of(mm, ll, kQuant);
+    }
+    __syncthreads();
+    for (int i = rank * blockDim.x + threadIdx.x; i < C::kHeads / 2 * kDim; i += p.splits * blockDim.x) {
+      const int hp = i / kDim, d = i % kDim, h = 2 * hp;
+      float x = 0.f, y = 0.f;
+#pragma unroll 4
+      for (int r = 0; r < p.splits; ++r) {
+        const float2 v = ld_cluster2(&s_o[0][hp][place(d)], r);
+        x += v.x * s_f[r][h], y += v.y * s_f[r][h + 1];
+      }
+      put(h, d, x * s_qs[h], y * s_qs[h + 1]);
+    }
+    cluster_sync();  // no CTA leaves while another reads its shared memory
+    return;
+  }
+  left -= end - begin;
+  if (left <= 0) return;
+  ++part;
+  row = next_row, unit = next_unit, sp = next_sp;
+  begin = 0, end = min(left, sp.tiles);
+  tc::fence_proxy_async_smem();  // the join's reads and writes of the ring come before the next copies into it
+  __syncthreads();
   }
 }
 
-// Joins the splits. 16 lanes hold 64 values of one query head (4 each); `groups` of them take its splits in turn,
-// each with a running maximum of its own, and meet in shared memory: 16 / groups pieces of 64 values a CTA.
+// Joins the parts of a shared row's unit: blockIdx = (row and unit, slice of its heads' values). A thread holds 4 values;
+// `groups` threads take their parts in turn, each with a running maximum of its own, and meet in shared memory.
 constexpr int kJoinThreads = 256, kJoinBatch = 4;
-__global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constant__ Params p, int dim, int groups, float lift) {
-  __shared__ float s_m[kJoinThreads / 16], s_l[kJoinThreads / 16];
-  __shared__ float4 s_x[kJoinThreads / 16][16];
+__global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constant__ Params p, int dim, int ctas, int heads, int groups, bool quant) {
+  __shared__ float s_m[kJoinThreads], s_l[kJoinThreads];
+  __shared__ float4 s_x[kJoinThreads];
   griddep_launch();
   griddep_wait();
-  const int team = threadIdx.x / 16, c = threadIdx.x % 16, g = team % groups, pieces = dim / 64;
-  const int64_t piece = static_cast<int64_t>(blockIdx.x) * (16 / groups) + team / groups, head = piece / pieces;
-  const int64_t row = head / p.q_heads;
-  bool on = row < p.c.rows;
-  int n = 0;
-  if (on) {
-    const Span sp = row_span(p, static_cast<int>(row));
-    on = sp.tiles > sp.chunk;  // else written whole, or nothing to see
-    if (on) n = static_cast<int>((sp.tiles + sp.chunk - 1) / sp.chunk);
-  }
-  const int at = static_cast<int>(piece % pieces) * 16 + c;  // of the head's float4s
-  const float2* ml = p.part_ml + head * p.splits;
-  const float4* po = reinterpret_cast<const float4*>(p.part_o + head * p.splits * dim) + at;
+  const int units = p.kv_heads * p.head_tiles, row = blockIdx.x / units, unit = blockIdx.x % units;
+  const int64_t at = p.row_at[row], tiles = p.row_at[row + 1] - at, share = share_of(p.row_at[p.c.rows], p.c.rows, units, ctas);
+  const int64_t from = at * units + unit * tiles, first = div(from, share), last = div(from + tiles - 1, share);
+  if (tiles == 0 || last == first) return;  // nothing to see, or written whole
+  const int n = static_cast<int>(last - first + 1), skip = from > first * share;  // skip: the row is not its first CTA's first
+  const int per = kJoinThreads / groups, g = threadIdx.x / per, i4 = blockIdx.y * per + threadIdx.x % per;
+  const int h = i4 * 4 / dim, in_group = unit % p.head_tiles * heads + h;
+  const bool on = h < heads && in_group < p.group;
+  const float2* const ml = p.part_ml + 2 * first * heads + h;
+  const float4* const po = reinterpret_cast<const float4*>(p.part_o + 2 * first * heads * dim) + i4;
   float m = -INFINITY, l = 0.f;
   float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int i0 = g; i0 < n; i0 += groups * kJoinBatch) {
+  for (int i0 = g; i0 < n && on; i0 += groups * kJoinBatch) {
     float2 a[kJoinBatch];
     float4 y[kJoinBatch];
 #pragma unroll
     for (int b = 0; b < kJoinBatch; ++b) {
-      const int i = i0 + b * groups;
-      a[b] = i < n ? ml[i] : make_float2(-INFINITY, 0.f);
-      y[b] = i < n ? po[static_cast<int64_t>(i) * (dim / 4)] : make_float4(0.f, 0.f, 0.f, 0.f);
+      const int i = i0 + b * groups, slot = 2 * i + (i == 0 ? skip : 0);
+      a[b] = i < n ? ml[slot * heads] : make_float2(-INFINITY, 0.f);
+      y[b] = i < n ? po[slot * (heads * dim / 4)] : make_float4(0.f, 0.f, 0.f, 0.f);
     }
     float mm = m;
 #pragma unroll
@@ -639,33 +822,30 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constan
     m = mm;
   }
   if (groups > 1) {
-    if (c == 0) s_m[team] = m, s_l[team] = l;
-    s_x[team][c] = x;
+    s_m[threadIdx.x] = m, s_l[threadIdx.x] = l, s_x[threadIdx.x] = x;
     __syncthreads();
     if (g) return;
     float mm = m;
-    for (int i = 1; i < groups; ++i) mm = fmaxf(mm, s_m[team + i]);
+    for (int i = 1; i < groups; ++i) mm = fmaxf(mm, s_m[i * per + threadIdx.x]);
     const float f0 = m == -INFINITY ? 0.f : ex2(m - mm);
     l *= f0, x.x *= f0, x.y *= f0, x.z *= f0, x.w *= f0;
     for (int i = 1; i < groups; ++i) {
-      const float f = s_m[team + i] == -INFINITY ? 0.f : ex2(s_m[team + i] - mm);
-      const float4 y = s_x[team + i][c];
-      l += s_l[team + i] * f;
+      const float mi = s_m[i * per + threadIdx.x], f = mi == -INFINITY ? 0.f : ex2(mi - mm);
+      const float4 y = s_x[i * per + threadIdx.x];
+      l += s_l[i * per + threadIdx.x] * f;
       x.x += y.x * f, x.y += y.y * f, x.z += y.z * f, x.w += y.w * f;
     }
     m = mm;
   }
   if (!on) return;
+  const int64_t head = static_cast<int64_t>(row) * p.q_heads + unit / p.head_tiles * p.group + in_group;
   const float inv = l == 0.f ? 0.f : 1.f / l;
-  *reinterpret_cast<uint2*>(p.out + head * dim + at * 4) = make_uint2(pack_bf16(x.x * inv, x.y * inv), pack_bf16(x.z * inv, x.w * inv));
-  if (at == 0) p.lse[head] = l == 0.f ? -INFINITY : (m - lift + log2f(l)) * 0.69314718055994531f;
+  const int d = i4 * 4 - h * dim;
+  *reinterpret_cast<uint2*>(p.out + head * dim + d) = make_uint2(pack_bf16(x.x * inv, x.y * inv), pack_bf16(x.z * inv, x.w * inv));
+  if (d == 0) p.lse[head] = lse_of(m, l, quant);
 }
 
 // ------------------------------------------------------------------ host side
-struct Plan {
-  int head_tiles, splits, min_tiles;
-};
-
 static int sms() {
   int dev = 0;
   cudaGetDevice(&dev);
@@ -674,23 +854,42 @@ static int sms() {
 
 static int tile_heads(int group) { return group > 8 ? 16 : 8; }
 
-static Plan plan(int rows, int q_heads, int kv_heads, int dim, bool quant, int64_t tiles) {
-  Plan r;
-  const int group = q_heads / kv_heads, heads = tile_heads(group);
+// How a call is laid out, from its sizes and the table's width (`tiles` of 16 tokens a row at most): the quickest by a model
+// of the time in microseconds, in which the longest row fills the table and the rows are 0.7 of it on average.
+//   A CTA reads about 56 KB a microsecond (35 KB of e4m3), the machine 6.2 MB (4.5 MB). A launch with its first copies and
+//   last sums takes 4.5 (one CTA a unit) or 7.5 (a cluster a unit); one CTA a unit leaves the machine idle at the end,
+//   5%; the stream takes 12 (the count of the rows, and the join's launch).
+// Measured at 1 / 4 / 32 / 128 units (one row, 2 x 2, 8 x 4, 16 x 8) of up to 1,000 tokens: one CTA a unit 19.8 / 19.8 /
+// 12.3 / 15.5 us, clusters 10.0 / 10.1 / 8.5 / -, stream 10.4 / 13.5 / 13.8 / 22.4; of up to 8,000: 129 / 129 / 74 / 83,
+// 22.6 / 22.7 / 26 / -, 13.0 / 16.8 / 23.7 / 67 (256-value heads for the first two, else 128; bf16).
+struct Plan {
+  int head_tiles, splits, ctas;  // splits: CTAs of a cluster, 0: stream over `ctas`
+};
+static Plan plan(int rows, int q_heads, int kv_heads, int dim, int page_size, int per_row, bool quant, int64_t window) {
+  Plan r{};
+  int64_t tiles = static_cast<int64_t>(per_row) * (page_size / kTile);
+  if (window > 0 && window / kTile + 2 < tiles) tiles = window / kTile + 2;  // the tiles that a window touches
+  const int group = q_heads / kv_heads, heads = tile_heads(group), ctas = 2 * sms();
   r.head_tiles = (group + heads - 1) / heads;
-  const int64_t units = static_cast<int64_t>(rows) * kv_heads * r.head_tiles;
-  r.min_tiles = kWarps;
-  int64_t s = (static_cast<int64_t>(sms()) * 4 + units - 1) / units;
-  const int64_t most = (tiles + r.min_tiles - 1) / r.min_tiles;
-  if (s > most) s = most;
-  if (s > 65535) s = 65535;
-  r.splits = static_cast<int>(s < 1 ? 1 : s);
+  const double units = static_cast<double>(rows) * kv_heads * r.head_tiles, unit = static_cast<double>(tiles) * dim * (quant ? 32 : 64);
+  const double all = 0.7 * units * unit / (quant ? 4.5e6 : 6.2e6);
+  double best = 12 + all;
+  r.ctas = ctas;
+  for (int s = 1; s <= kMaxCluster && (s == 1 || units * s <= sms()); s *= 2) {
+    const double one = unit / s / (quant ? 35e3 : 56e3), t = s == 1 ? 4.5 + (one > 1.05 * all ? one : 1.05 * all) : 7.5 + (one > all ? one : all);
+    if (t < best) best = t, r.splits = s;
+  }
   return r;
+}
+static size_t part_bytes(const Plan& r, int rows, int q_heads, int kv_heads, int dim) {
+  if (r.splits) return 0;
+  const size_t heads = tile_heads(q_heads / kv_heads);
+  return 2 * static_cast<size_t>(r.ctas) * heads * (dim * sizeof(float) + sizeof(float2)) + (static_cast<size_t>(rows) + 1) * sizeof(int64_t);
 }
 
 template <typename... A>
-static cudaError_t start(void (*kernel)(A...), dim3 grid, int threads, int shared, void* stream, A... args) {
-  cudaLaunchAttribute attr[1];
+static cudaError_t start(void (*kernel)(A...), dim3 grid, int threads, int shared, int cluster, void* stream, A... args) {
+  cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = pdl_enabled() ? 1 : 0;
   cudaLaunchConfig_t cfg{};
@@ -700,6 +899,12 @@ static cudaError_t start(void (*kernel)(A...), dim3 grid, int threads, int share
   cfg.stream = static_cast<cudaStream_t>(stream);
   cfg.attrs = attr;
   cfg.numAttrs = 1;
+  if (cluster > 1) {
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = cluster;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    cfg.numAttrs = 2;
+  }
   return cudaLaunchKernelEx(&cfg, kernel, args...);
 }
 
@@ -717,11 +922,12 @@ static int attend(const Params& p, dim3 grid, void* stream) {
   cudaGetDevice(&dev);
   const uint64_t bit = uint64_t(1) << (dev & 63);
   if (!(allowed.load(std::memory_order_relaxed) & bit)) {
-    const cudaError_t err = cudaFuncSetAttribute(attend_kernel<kDim, kQuant, kNT, kU>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kShared);
+    cudaError_t err = cudaFuncSetAttribute(attend_kernel<kDim, kQuant, kNT, kU>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kShared);
+    if (err == cudaSuccess) err = cudaFuncSetAttribute(attend_kernel<kDim, kQuant, kNT, kU>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
     if (err != cudaSuccess) return set_error(std::string("paged_attention: ") + cudaGetErrorString(err)), DM3_ECUDA;
     allowed.fetch_or(bit, std::memory_order_relaxed);
   }
-  const cudaError_t err = start(attend_kernel<kDim, kQuant, kNT, kU>, grid, kWarps * 32, C::kShared, stream, p, maps[0], maps[1]);
+  const cudaError_t err = start(attend_kernel<kDim, kQuant, kNT, kU>, grid, kWarps * 32, C::kShared, p.splits, stream, p, maps[0], maps[1]);
   if (err != cudaSuccess) return set_error(std::string("paged_attention launch: ") + cudaGetErrorString(err)), DM3_ECUDA;
   return DM3_OK;
 }
@@ -730,7 +936,7 @@ template <int kDim, bool kQuant>
 static int attend(const Params& p, dim3 grid, void* stream) {
   // token tiles a step: 8 KB of keys, one unit of the ring (6 KB for 384-byte rows)
   constexpr int kRow = kDim * (kQuant ? 1 : 2), kU = kRow <= 64 ? 8 : kRow <= 128 ? 4 : kRow <= 256 ? 2 : 1;
-  return tile_heads(p.group) == 16 ? attend<kDim, kQuant, 2, kU>(p, grid, stream) : attend<kDim, kQuant, 1, kU>(p, grid, stream);
+  return tile_heads(p.group) == 16 ? attend<kDim, kQuant, 2, (kU > 2 ? 3 : kU)>(p, grid, stream) : attend<kDim, kQuant, 1, kU>(p, grid, stream);
 }
 
 }  // namespace attn
@@ -740,11 +946,10 @@ int dm3::wait_limit_attention(uint64_t ns) { return static_cast<int>(set_wait_li
 
 // ------------------------------------------------------------------ C ABI
 extern "C" size_t dm3_paged_attention_workspace_bytes(int rows, int q_heads, int kv_heads, int dim, int page_size,
-                                                      int per_row) {
-  if (rows < 1 || q_heads < 1 || kv_heads < 1 || q_heads < kv_heads || dim < 1 || page_size < 16 || per_row < 0) return 0;
-  const int64_t tiles = static_cast<int64_t>(per_row) * (page_size / dm3::attn::kTile);
-  const int splits = dm3::attn::plan(rows, q_heads, kv_heads, dim, false, tiles).splits;
-  return splits == 1 ? 0 : static_cast<size_t>(rows) * q_heads * splits * (dim * sizeof(float) + sizeof(float2));
+                                                      int per_row, int quantised, int64_t window) {
+  if (rows < 1 || kv_heads < 1 || q_heads < kv_heads || dim < 1 || page_size < dm3::attn::kTile || per_row < 0) return 0;
+  return dm3::attn::part_bytes(dm3::attn::plan(rows, q_heads, kv_heads, dim, page_size, per_row, quantised != 0, window), rows, q_heads,
+                               kv_heads, dim);
 }
 
 extern "C" int dm3_paged_attention(const void* q, int64_t q_rs, int64_t q_hs, int q_heads, const void* k_cache,
@@ -767,21 +972,20 @@ extern "C" int dm3_paged_attention(const void* q, int64_t q_rs, int64_t q_hs, in
   if (!q || !lengths || !out || !lse) return set_error("paged_attention: null pointer"), DM3_EINVAL;
   if (reinterpret_cast<uintptr_t>(q) % 16 || q_rs % 8 || q_hs % 8 || reinterpret_cast<uintptr_t>(out) % 16)
     return set_error("paged_attention: rows must start on 16 bytes"), DM3_EINVAL;
-  int64_t tiles = static_cast<int64_t>(per_row) * (page_size / attn::kTile);
-  if (window > 0 && window / attn::kTile + 2 < tiles) tiles = window / attn::kTile + 2;  // the tiles that a window touches
-  const attn::Plan plan = attn::plan(rows, q_heads, kv_heads, dim, k_exp != nullptr, tiles);
+  const attn::Plan plan = attn::plan(rows, q_heads, kv_heads, dim, page_size, per_row, k_exp != nullptr, window);
   p.q = static_cast<const __nv_bfloat16*>(q), p.q_rs = q_rs, p.q_hs = q_hs, p.q_heads = q_heads, p.kv_heads = kv_heads;
-  p.group = q_heads / kv_heads, p.head_tiles = plan.head_tiles, p.splits = plan.splits, p.min_tiles = plan.min_tiles;
+  p.group = q_heads / kv_heads, p.head_tiles = plan.head_tiles, p.splits = plan.splits;
   p.lengths = lengths, p.scale_log2 = scale * 1.44269504088896341f, p.window = window;
   p.out = static_cast<__nv_bfloat16*>(out), p.lse = lse;
-  const int64_t parts = static_cast<int64_t>(rows) * q_heads * plan.splits;
-  if (plan.splits > 1) {
-    if (workspace_bytes < parts * (dim * sizeof(float) + sizeof(float2))) return set_error("workspace too small"), DM3_ENOSPACE;
+  const int heads = attn::tile_heads(p.group);
+  if (!plan.splits) {
+    if (workspace_bytes < attn::part_bytes(plan, rows, q_heads, kv_heads, dim)) return set_error("workspace too small"), DM3_ENOSPACE;
     if (!workspace || reinterpret_cast<uintptr_t>(workspace) % 256) return set_error("workspace must be 256-byte aligned"), DM3_EINVAL;
     p.part_o = static_cast<float*>(workspace);
-    p.part_ml = reinterpret_cast<float2*>(p.part_o + parts * dim);
+    p.part_ml = reinterpret_cast<float2*>(p.part_o + 2 * static_cast<int64_t>(plan.ctas) * heads * dim);
+    p.row_at = reinterpret_cast<int64_t*>(p.part_ml + 2 * static_cast<int64_t>(plan.ctas) * heads);
   }
-  const dim3 grid(plan.splits, kv_heads * plan.head_tiles, rows);
+  const dim3 grid = plan.splits ? dim3(plan.splits, kv_heads * plan.head_tiles, rows) : dim3(plan.ctas);
   int rc;
   switch (dim) {
     case 64: rc = k_exp ? attn::attend<64, true>(p, grid, stream) : attn::attend<64, false>(p, grid, stream); break;
@@ -790,13 +994,14 @@ extern "C" int dm3_paged_attention(const void* q, int64_t q_rs, int64_t q_hs, in
     default: rc = k_exp ? attn::attend<256, true>(p, grid, stream) : attn::attend<256, false>(p, grid, stream); break;
   }
   if (rc) return rc;
-  if (plan.splits > 1) {
-    const int groups = plan.splits <= 4 ? 1 : plan.splits <= 24 ? 4 : 16;  // teams that share a head's splits
-    const int64_t pieces = static_cast<int64_t>(rows) * q_heads * (dim / 64);
-    const cudaError_t err = attn::start(attn::join_kernel, dim3(static_cast<unsigned>((pieces * groups + 15) / 16)), attn::kJoinThreads, 0,
-                                        stream, p, dim, groups, k_exp ? attn::kLift : 0.f);
+  if (!plan.splits) {
+    // threads that share a unit's parts: few where there are many units, which have two or three parts each
+    const int64_t units = static_cast<int64_t>(rows) * kv_heads * plan.head_tiles;
+    const int groups = units * 4 >= plan.ctas ? 2 : 16;
+    const dim3 joins(static_cast<unsigned>(units), (heads * (dim / 4) * groups + attn::kJoinThreads - 1) / attn::kJoinThreads);
+    const cudaError_t err = attn::start(attn::join_kernel, joins, attn::kJoinThreads, 0, 1, stream, p, dim, plan.ctas, heads, groups, k_exp != nullptr);
     if (err != cudaSuccess) return set_error(std::string("paged_attention launch: ") + cudaGetErrorString(err)), DM3_ECUDA;
   }
-  note_launches(plan.splits > 1 ? 2 : 1);
+  note_launches(plan.splits ? 1 : 2);
   return DM3_OK;
 }

@@ -752,7 +752,8 @@ def _paged_attention(q: Tensor, k_cache: Tensor, v_cache: Tensor, k_exp: Optiona
     out = torch.empty((rows, q_heads, dim), dtype=BF16, device=q.device)
     lse = torch.empty((rows, q_heads), dtype=torch.float32, device=q.device)
     # scratch from the caller's allocator: calls on other streams and in other graphs have their own
-    nbytes = _lib.load().dm3_paged_attention_workspace_bytes(rows, q_heads, heads, dim, size, tab[3])
+    nbytes = _lib.load().dm3_paged_attention_workspace_bytes(rows, q_heads, heads, dim, size, tab[3], k_exp is not None,
+                                                              window)
     ws = torch.empty((nbytes,), dtype=torch.uint8, device=q.device) if nbytes else None
     _launch(dev, "dm3_paged_attention", q.data_ptr(), q.stride(0), q.stride(1), q_heads, *held, pages, size, heads, dim, *tab,
             lengths.data_ptr(), dim ** -0.5 if scale is None else scale, window, out.data_ptr(), lse.data_ptr(),

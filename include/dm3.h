@@ -415,7 +415,8 @@ int dm3_kv_read(const void* k_cache, const void* v_cache, int64_t page_stride, c
                 void* k_out, void* v_out, uint32_t* status, void* stream);
 
 /* Workspace bytes of dm3_paged_attention (its contents need no initial value). */
-size_t dm3_paged_attention_workspace_bytes(int rows, int q_heads, int kv_heads, int dim, int page_size, int per_row);
+size_t dm3_paged_attention_workspace_bytes(int rows, int q_heads, int kv_heads, int dim, int page_size, int per_row,
+                                           int quantised, int64_t window);
 
 /*
  * One new token's attention for every row: out[r, h] = sum_t p_t v_t with p = softmax(scale * q[r, h] . k_t)
@@ -423,7 +424,7 @@ size_t dm3_paged_attention_workspace_bytes(int rows, int q_heads, int kv_heads, 
  * h / (q_heads / kv_heads); lse[r, h] = log sum exp. A row that sees nothing gives zeros and -inf.
  *   q    bf16 [rows, q_heads, dim], row stride q_rs and head stride q_hs (16-byte aligned rows)
  *   out  bf16 [rows, q_heads, dim]; lse fp32 [rows, q_heads]
- *   workspace  dm3_paged_attention_workspace_bytes, 256-byte aligned, not shared by calls that may overlap
+ *   workspace  dm3_paged_attention_workspace_bytes (may be 0), 256-byte aligned, not shared by calls that may overlap
  */
 int dm3_paged_attention(const void* q, int64_t q_rs, int64_t q_hs, int q_heads, const void* k_cache, const void* v_cache,
                         int64_t page_stride, const int8_t* k_exp, const int8_t* v_exp, int64_t exp_stride, int pages,

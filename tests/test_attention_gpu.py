@@ -49,6 +49,23 @@ def test_long_row(dm3, quant):
     check_attention(*_run(dm3, d, q), d, q)
 
 
+def _spread(rows, longest, empty, seed):
+    g = torch.Generator().manual_seed(seed)
+    n = torch.randint(1, longest + 1, (rows,), generator=g)
+    n[torch.rand(rows, generator=g) < empty] = 0
+    return n.tolist()
+
+
+@pytest.mark.parametrize("rows,longest,empty,capacity", [(300, 90, 0.3, 9000), (129, 400, 0.0, 9000), (128, 33, 0.9, 9000), (1, 3000, 0.0, 200000),
+                                                         (3, 2500, 0.4, 200000), (700, 5, 0.5, 9000), (40, 700, 0.0, 700)])
+@pytest.mark.parametrize("kv_heads,group,dim,quant,window", [(2, 4, 128, False, 0), (1, 12, 64, True, 0), (3, 20, 64, False, 50), (1, 9, 256, True, 0)])
+def test_many_and_ragged_rows(dm3, rows, longest, empty, capacity, kv_heads, group, dim, quant, window):
+    """Rows of all lengths in one sequence cut into equal shares: cuts inside rows, at their ends, and over many of them."""
+    d = paged(_spread(rows, longest, empty, rows + dim), kv_heads, dim, 16, quant, rows, capacity=capacity)
+    q = _q(rows, kv_heads * group, dim, rows)
+    check_attention(*_run(dm3, d, q, None, window), d, q, None, window)
+
+
 def test_nothing_to_see(dm3):
     d = paged([0, 0, 0], 2, 64, 16, False, 1)
     q = _q(3, 4, 64, 1)
@@ -58,6 +75,9 @@ def test_nothing_to_see(dm3):
     dev = to_cuda(d)
     out, lse = dm3.ops.paged_attention(e, *held(dev), dev["table"][:0], dev["lengths"][:0], dev["status"])
     assert out.shape == (0, 4, 64) and lse.shape == (0, 4)
+    wide = paged([0, 0, 0], 2, 64, 16, False, 1, capacity=100000)
+    out, lse = _run(dm3, wide, q)
+    assert (out == 0).all() and (lse == -math.inf).all()
     out, lse = dm3.ops.paged_attention(q.cuda(), *held(dev), dev["table"][:, :0], dev["lengths"], dev["status"])
     assert (out == 0).all() and (lse == -math.inf).all() and int(dev["status"]) == 0
 
@@ -111,6 +131,17 @@ def test_bad_pages_and_lengths(dm3):
             out, lse = dm3.ops.paged_attention(q.cuda(), *held(dev), dev["table"], dev["lengths"], dev["status"])
             assert int(dev["status"]) == 4
             check_attention(out, lse, d, q)
+        for capacity in (112, 100000):
+            d = paged([0, 100, 40], 2, 64, 16, quant, 4, capacity=capacity)
+            dev = to_cuda(d)
+            dev["table"] = dev["table"].clone()
+            full = dev["table"].shape[1] * 16
+            dev["table"][0] = dev["table"][1, 0]  # a row with pages to the end, and a length behind them
+            dev["lengths"][0] = full + 1
+            out, lse = dm3.ops.paged_attention(q[:1].expand(3, -1, -1).cuda(), *held(dev), dev["table"], dev["lengths"], dev["status"])
+            assert int(dev["status"]) == 4
+            d["table"], d["lengths"] = dev["table"].cpu(), torch.tensor([full, 100, 40])
+            check_attention(out, lse, d, q[:1].expand(3, -1, -1))
         d = paged([100, 112], 2, 64, 16, quant, 4)
         d["lengths"][1] = 1 << 41
         dev = to_cuda(d)
