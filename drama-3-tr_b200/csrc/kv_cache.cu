@@ -493,19 +493,19 @@ static bool aligned(const Heads& h) {
   return reinterpret_cast<uintptr_t>(h.p) % 16 == 0 && h.ts % 8 == 0 && h.hs % 8 == 0;
 }
 
-// Tokens of a CTA: eight a CTA of each SM's eight at most, so that a token's angles and places cost little beside its
-// rows, but no fewer CTAs than that. And CTAs that share a block's rows when there are few tokens.
+// Tokens of a CTA: up to eight, so that their angles and places cost little beside their rows, but as few as fill the
+// last wave of four CTAs an SM. And CTAs that share a block's rows when there are few tokens.
 struct Blocks {
   int tokens, shares;
 };
 static Blocks blocks(int64_t T, int rot, int64_t rounds_a_token) {
   int dev = 0;
   cudaGetDevice(&dev);
-  const int64_t ctas = 8 * sm_count(dev);
+  const int64_t wave = 4 * sm_count(dev), waves = (T + wave * kBlockTokens - 1) / (wave * kBlockTokens);
   Blocks b;
-  b.tokens = static_cast<int>(T / ctas < 1 ? 1 : T / ctas < kBlockTokens ? T / ctas : kBlockTokens);
+  b.tokens = static_cast<int>((T + wave * waves - 1) / (wave * waves));
   while (b.tokens * (rot / 2) > kAngles) --b.tokens;
-  const int64_t want = (ctas / 4 + T - 1) / T;
+  const int64_t want = (wave / 2 + T - 1) / T;
   b.shares = static_cast<int>(b.tokens > 1 ? 1 : want < rounds_a_token ? want : rounds_a_token);
   return b;
 }
