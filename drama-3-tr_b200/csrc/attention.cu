@@ -5,31 +5,34 @@
 //
 // One pass with a running maximum M and sum l; a row that sees nothing gives zeros and lse = -inf.
 //
-// Bound: the bytes of the cache's rows, each used by the group of query heads that shares them
-// (2 * group flops a byte and less), so the kernel is laid out to keep loads in flight, not for the tensor
-// peak: the products run as warp-level m16n8k16 tiles whose operands come from global memory straight into
-// registers, without shared memory, barriers between warps or a shuffle of the data. With tokens as the
-// tile's 16 rows and the query heads as its 8 columns,
-//   S^T = K Q^T:  a lane's 16-byte load of a key row holds the k-columns of 2 (bf16) or 4 (e4m3) tiles
-//                 once the same permutation of dim is applied to Q;
-//   O^T = V^T P^T: a lane loads 16 bytes of 4 tokens' value rows and interleaves pairs of tokens with byte
-//                 permutes; P^T comes from S^T's accumulators by an 8x8 transpose (movmatrix).
-// A group of up to 8 heads wastes nothing, where heads as rows would waste half of the tile and of the registers.
-// Every warp walks its own 16-token tiles, the next keys loading while the softmax and the values' product
-// run; the warps of a CTA join in shared memory at the end.
+// Bound: the bytes of the cache's rows, each used by the group of query heads that shares them (2 * group flops a byte
+// and less), so the kernel is laid out to keep copies in flight and to spend few instructions a row, not for the
+// tensor peak: the products are warp-level m16n8k16 tiles with tokens as the 16 rows and query heads as the 8 columns
+// (heads as rows would waste half of the tile and of the registers for groups of up to 8):
+//   S^T = K Q^T:  a lane's 16 bytes of a key row hold the k-columns of 2 (bf16) or 4 (e4m3) tiles once the same
+//                 permutation of dim is applied to Q;
+//   O^T = V^T P^T: a lane takes 16 bytes of 4 tokens' value rows and interleaves pairs of tokens with byte permutes; P^T
+//                 comes from S^T's accumulators by an 8x8 transpose (movmatrix).
+// Every warp walks 16-token tiles of its own: TMA brings a step's keys and values, swizzled, into a ring of shared memory
+// that belongs to the warp, so warps never wait for one another until the join at the end. (Loads straight into
+// registers kept too little in flight, 82% of the copy bandwidth against 93% over 64 ragged rows of a bf16 cache;
+// cp.async in their place doubled the traffic through L1 and was slower still. FP8 tensor instructions for the keys' product,
+// with the queries as two e4m3 parts, took a quarter longer than converting the keys to fp16.)
 //
-// Rows are split over CTAs by the lengths that the device reads, so one captured graph serves all lengths, in one of two
-// ways (plan() says when); neither uses atomics, and the order of every sum is fixed by the lengths alone.
-//   * Clusters: `splits` CTAs of a cluster share a row's tiles and join over distributed shared memory: one launch,
-//     for short rows.
+// A unit is a row and up to 16 of the query heads that share a cache head. Units are split over CTAs by the lengths that the
+// device reads, so one captured graph serves all lengths, in one of two ways (plan() says when); neither uses atomics,
+// and the order of every sum is fixed by the lengths and sizes alone.
+//   * Clusters: the `splits` CTAs of a cluster (1 to 8) share a unit's tiles and join over distributed shared memory: one
+//     launch, for short rows.
 //   * Stream: the tiles of all rows and heads are one sequence, cut into equal shares for two CTAs an SM whatever the
-//     rows' lengths; a CTA leaves (M, l, O) in fp32 of a row that it shares, and a second kernel joins them.
+//     rows' lengths; a CTA leaves (M, l, O) in fp32 of a unit that it shares, and a second kernel joins them.
 //
 // An e4m3 row is code * 2^e. For keys 2^e joins the logit's scale. For values it joins the weight's exponent:
 // w_t = 2^(s_t + e_t - M) with M the running maximum of s_t + e_t, so weights are in fp16's range whatever the rows'
 // sizes, and l sums w_t * 2^-e_t. Codes are exact in fp16; queries are scaled by a power of two to
-// [2^14, 2^15), where fp16 holds a bf16 row to 2^-40 of its largest value; a weight is rounded once to 11 bits.
-// With a bf16 cache a weight goes to the tensor cores as a bf16 pair (high and low part, 16 bits).
+// [2^14, 2^15), where fp16 holds a bf16 row to 2^-40 of its largest value; a weight is rounded once to 11 bits (2^-12 of
+// it at most, 1/16 of what rounding the output to bf16 costs). With a bf16 cache a weight goes to the tensor cores
+// as a bf16 pair, high and low part: 16 bits.
 #include <atomic>
 #include <cmath>
 #include <cstdint>
@@ -52,6 +55,8 @@ constexpr int kTile = 16;  // tokens of one tile; pages hold whole tiles
 // The maximum is raised only when a logit exceeds it by more than kSlack (log2): weights reach 2^kSlack. fp16
 // weights carry 2^kLift besides, so that they stay normal down to 2^-(14 + kLift).
 constexpr float kSlack = 8.f, kLift = 6.f;
+// With e4m3 rows l is held times 2^-kSpan: 2^-e_t reaches 2^110 there, and a sum of many has to stay finite.
+constexpr int kSpan = 7;
 
 struct Params {
   const __nv_bfloat16* q;  // [rows][q_heads][dim]
@@ -134,6 +139,11 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
   return r;
 }
+__device__ __forceinline__ float ex2_all(float x) {  // results below 2^-126 kept
+  float r;
+  asm("ex2.approx.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
 __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
   const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&h);
@@ -179,9 +189,15 @@ __device__ __forceinline__ int token_of(int lr) {
   return kBox == 128 ? ((lr ^ lr >> 2) & 1) << 2 | (lr & 2) | lr >> 2 : lr;
 }
 
-__device__ __forceinline__ float lse_of(float m, float l, bool quant) {  // natural log of the sum, from log2 units
-  return l == 0.f ? -INFINITY : (m - (quant ? kLift : 0.f) + log2f(l)) * 0.69314718055994531f;
+// l * 2^d, d <= 0, where 2^d alone may vanish: the maxima that l refers to can lie 2^229 apart (see the exponents above).
+__device__ __forceinline__ float scale_sum(float l, float d) {
+  const float h = ex2(0.5f * d);
+  return l * h * h;
 }
+__device__ __forceinline__ float lse_of(float m, float l, bool quant) {  // natural log of the sum, from log2 units
+  return l == 0.f ? -INFINITY : (m + (quant ? kSpan - kLift : 0.f) + log2f(l)) * 0.69314718055994531f;
+}
+__device__ __forceinline__ float inverse(float l, bool quant) { return l == 0.f ? 0.f : (quant ? 1.f / (1 << kSpan) : 1.f) / l; }
 
 __device__ __forceinline__ bool elect_one() {  // true in one lane of the warp
   uint32_t r;
@@ -293,8 +309,8 @@ __global__ void __launch_bounds__(kWarps * 32, 2)
   int64_t row, begin, end;
   int unit;
   Span sp;
-  int64_t left = 0;             // stream: tiles of this CTA's share from the segment on
-  int part = 0;                 // stream: segments done
+  int64_t left = 0;  // stream: tiles of this CTA's share from the segment on
+  int part = 0;      // stream: segments done
   if (p.splits) {
     row = blockIdx.z, unit = blockIdx.y;
     sp = row_span(p, row);
@@ -319,6 +335,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2)
   uint8_t* const ring = smem + warp * C::kRing * C::kUnit;
   int slot = 0;  // of the ring's next unit, and its barrier's parity
   uint32_t parity = 0;
+  bool lost = false;  // a wait ran out
   const int tok = token_of<C::kBox>(lr), sw = C::kBox == 128 ? tok : tok >> 1;  // the lane's token of a key tile, its swizzle
   int vtok[2];                                                                    // its tokens of a value tile (and + 8)
 #pragma unroll
@@ -326,456 +343,476 @@ __global__ void __launch_bounds__(kWarps * 32, 2)
   const int per_page = p.c.page_size / kTile;
 
   for (;;) {
-  const int kvh = unit / p.head_tiles, h0 = unit % p.head_tiles * C::kHeads;  // h0: first head of the group
-  const int64_t qrow = row * p.q_heads + kvh * p.group + h0;                   // output row of head h0
-  // A warp's steps: kU tiles each, tiles going to the warps in turn. Lane i of a block of 32 tiles knows where the
-  // block's tile i lies, and asks for it.
-  constexpr int kBlock = 32 / kU;  // steps a block
-  const int mine = static_cast<int>((end - begin - warp + kWarps - 1) / kWarps);  // tiles of this warp
-  int steps = mine > 0 ? (mine + kU - 1) / kU : 0;
-  int page, y, range;  // y: first row of the tile in its page
-  auto find = [&](int step0) {
-    const int64_t t = begin + (static_cast<int64_t>(step0) * kU + lane) * kWarps + warp;
-    int tile = 0;
-    page = 0, range = 0;
-    if (t < end && lane < kBlock * kU) {
-      const int64_t g = sp.tile0 + t, nth = div(g, per_page), t0 = g * kTile;
-      tile = static_cast<int>(g - nth * per_page);
-      page = p.c.table[row * p.c.table_stride + nth];
-      if (page < 0 || page >= p.c.pages)
-        kv::set_status(p.c.status, STATUS_BAD_PAGE);
-      else
-        range = (sp.first > t0 ? static_cast<int>(sp.first - t0) : 0) | (sp.n - t0 < kTile ? static_cast<int>(sp.n - t0) : kTile) << 8;
-    }
-    y = kvh * p.c.page_size + tile * kTile;
-  };
-  find(0);
-
-  auto ask = [&](bool keys, int step, int to_slot) {
-    if (step >= steps) return;
-    if (keys && step % kBlock == 0 && step > 0) find(step);
-    int pg[kU], yy[kU], rg[kU];
-#pragma unroll
-    for (int u = 0; u < kU; ++u) {
-      const int from = step % kBlock * kU + u;
-      pg[u] = __shfl_sync(0xffffffffu, page, from), yy[u] = __shfl_sync(0xffffffffu, y, from), rg[u] = __shfl_sync(0xffffffffu, range, from);
-    }
-    if (elect_one()) {
-      int tiles = 0;
-#pragma unroll
-      for (int u = 0; u < kU; ++u) {
-        s_range[to_slot][u] = rg[u];
-        tiles += rg[u] != 0;
+    const int kvh = unit / p.head_tiles, h0 = unit % p.head_tiles * C::kHeads;  // h0: first head of the group
+    const int64_t qrow = row * p.q_heads + kvh * p.group + h0;                   // output row of head h0
+    // A warp's steps: kU tiles each, tiles going to the warps in turn. Lane i of a block of 32 tiles knows where the
+    // block's tile i lies, and asks for it.
+    constexpr int kBlock = 32 / kU;  // steps a block
+    const int mine = static_cast<int>((end - begin - warp + kWarps - 1) / kWarps);  // tiles of this warp
+    int steps = mine > 0 ? (mine + kU - 1) / kU : 0;
+    int page, y, range;  // y: first row of the tile in its page
+    auto find = [&](int step0) {
+      const int64_t t = begin + (static_cast<int64_t>(step0) * kU + lane) * kWarps + warp;
+      int tile = 0;
+      page = 0, range = 0;
+      if (t < end && lane < kBlock * kU) {
+        const int64_t g = sp.tile0 + t, nth = div(g, per_page), t0 = g * kTile;
+        tile = static_cast<int>(g - nth * per_page);
+        page = p.c.table[row * p.c.table_stride + nth];
+        if (page < 0 || page >= p.c.pages)
+          kv::set_status(p.c.status, STATUS_BAD_PAGE);
+        else
+          range = (sp.first > t0 ? static_cast<int>(sp.first - t0) : 0) | (sp.n - t0 < kTile ? static_cast<int>(sp.n - t0) : kTile) << 8;
       }
-      mbar_arrive_expect_tx(&full[to_slot], tiles * (C::kTileBytes + (kQuant && keys ? 32 : 0)));
+      y = kvh * p.c.page_size + tile * kTile;
+    };
+    find(0);
+
+    auto ask = [&](bool keys, int step, int to_slot) {
+      if (step >= steps) return;
+      if (keys && step % kBlock == 0 && step > 0) find(step);
+      int pg[kU], yy[kU], rg[kU];
 #pragma unroll
       for (int u = 0; u < kU; ++u) {
-        if (rg[u] == 0) continue;  // nothing there: no copy, the place keeps what it held, to be masked
-        uint8_t* const to = ring + to_slot * C::kUnit + u * C::kTileBytes;
+        const int from = step % kBlock * kU + u;
+        pg[u] = __shfl_sync(0xffffffffu, page, from), yy[u] = __shfl_sync(0xffffffffu, y, from), rg[u] = __shfl_sync(0xffffffffu, range, from);
+      }
+      if (elect_one()) {
+        int tiles = 0;
 #pragma unroll
-        for (int b = 0; b < C::kBoxes; ++b)
-          tc::tma_load_3d(to + b * kTile * C::kBox, keys ? &kmap : &vmap, b * C::kBox, yy[u], pg[u], &full[to_slot]);
-        if (kQuant && keys) {
-          const int64_t x = pg[u] * p.c.exp_stride + yy[u];
-          bulk_g2s(s_exp[to_slot][u], p.c.k_exp + x, 16, &full[to_slot]);
-          bulk_g2s(s_exp[to_slot][u] + 16, p.c.v_exp + x, 16, &full[to_slot]);
+        for (int u = 0; u < kU; ++u) {
+          s_range[to_slot][u] = rg[u];
+          tiles += rg[u] != 0;
+        }
+        mbar_arrive_expect_tx(&full[to_slot], tiles * (C::kTileBytes + (kQuant && keys ? 32 : 0)));
+#pragma unroll
+        for (int u = 0; u < kU; ++u) {
+          if (rg[u] == 0) continue;  // nothing there: no copy, the place keeps what it held, to be masked
+          uint8_t* const to = ring + to_slot * C::kUnit + u * C::kTileBytes;
+#pragma unroll
+          for (int b = 0; b < C::kBoxes; ++b)
+            tc::tma_load_3d(to + b * kTile * C::kBox, keys ? &kmap : &vmap, b * C::kBox, yy[u], pg[u], &full[to_slot]);
+          if (kQuant && keys) {
+            const int64_t x = pg[u] * p.c.exp_stride + yy[u];
+            bulk_g2s(s_exp[to_slot][u], p.c.k_exp + x, 16, &full[to_slot]);
+            bulk_g2s(s_exp[to_slot][u] + 16, p.c.v_exp + x, 16, &full[to_slot]);
+          }
         }
       }
-    }
-    __syncwarp();
-  };
+      __syncwarp();
+    };
 #pragma unroll
-  for (int i = 0; i < C::kRing; ++i) ask(!(i & 1), i / 2, slot + i < C::kRing ? slot + i : slot + i - C::kRing);
+    for (int i = 0; i < C::kRing; ++i) ask(!(i & 1), i / 2, slot + i < C::kRing ? slot + i : slot + i - C::kRing);
 
-  // Stream: the unit behind this one, its length on its way while this one is worked on (the share ends before the rows do)
-  int64_t next_row = row;
-  int next_unit = unit + 1;
-  Span next_sp = sp;
-  if (left > end - begin && next_unit == units) {
-    next_unit = 0;
-    do {
-      if (++next_row >= p.c.rows) return;
-      next_sp = row_span(p, next_row);
-    } while (next_sp.tiles == 0);
-  }
-
-  // Queries as B operands, in the permutation of dim that 16-byte key copies give; warp nt prepares tile nt.
-  if (warp < kNT) {
-    const int h = h0 + warp * 8 + lr;
-    const __nv_bfloat16* src = p.q + row * p.q_rs + static_cast<int64_t>(kvh * p.group + h) * p.q_hs;
-    uint4 w[kDim / 32];
-#pragma unroll
-    for (int j = 0; j < kDim / 32; ++j) {
-      const int d = kQuant ? j / 2 * 64 + lc * 16 + j % 2 * 8 : j * 32 + lc * 8;
-      w[j] = h < p.group ? *reinterpret_cast<const uint4*>(src + d) : make_uint4(0, 0, 0, 0);
+    // Stream: the unit behind this one, its length on its way while this one is worked on (the share ends before the rows do)
+    int64_t next_row = row;
+    int next_unit = unit + 1;
+    Span next_sp = sp;
+    if (left > end - begin && next_unit == units) {
+      next_unit = 0;
+      while (++next_row < p.c.rows && (next_sp = row_span(p, next_row)).tiles == 0) {}
+      if (next_row >= p.c.rows) left = end - begin;  // never, unless lengths change under the kernel
     }
-    float qs = p.scale_log2;  // logit scale of head h
-    if (kQuant) {
-      uint32_t top = 0;  // the largest magnitude's bits
-      auto mag = [](uint32_t x) { return max(x << 16 & 0x7fffffffu, x & 0x7fff0000u); };
-#pragma unroll
-      for (int j = 0; j < kDim / 32; ++j) top = max(top, max(max(mag(w[j].x), mag(w[j].y)), max(mag(w[j].z), mag(w[j].w))));
-      top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-      top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-      const int e = min(max(static_cast<int>(top >> 23) - 127, -112), 126) - 14;  // 2^-e puts the largest in [2^14, 2^15)
-      const float up = exp2i(-e);
-      auto half = [up](uint32_t x) { return pack_half(__uint_as_float(x << 16) * up, __uint_as_float(x & 0xffff0000u) * up); };
-#pragma unroll
-      for (int j = 0; j < kDim / 32; ++j) w[j] = make_uint4(half(w[j].x), half(w[j].y), half(w[j].z), half(w[j].w));
-      qs *= exp2i(e);
-    }
-#pragma unroll
-    for (int j = 0; j < kDim / 32; ++j) s_q[(warp * (kDim / 32) + j) * 32 + lane] = w[j];
-    if (lc == 0) s_qs[warp * 8 + lr] = qs;
-  }
-  __syncthreads();
 
-  float o[kNT][kDim / 16][4];
-  // Of the lane's two heads a tile: the maximum m (the same in all lanes of a head), what is subtracted (m, or 0
-  // before any logit was seen, less the lift), and a lane's part of l.
-  float m[kNT][2], sub[kNT][2], l[kNT][2], qs[kNT][2];
+    // Queries as B operands, in the permutation of dim that 16-byte key copies give; warp nt prepares tile nt.
+    if (warp < kNT) {
+      const int h = h0 + warp * 8 + lr;
+      const __nv_bfloat16* src = p.q + row * p.q_rs + static_cast<int64_t>(kvh * p.group + h) * p.q_hs;
+      uint4 w[kDim / 32];
 #pragma unroll
-  for (int nt = 0; nt < kNT; ++nt) {
+      for (int j = 0; j < kDim / 32; ++j) {
+        const int d = kQuant ? j / 2 * 64 + lc * 16 + j % 2 * 8 : j * 32 + lc * 8;
+        w[j] = h < p.group ? *reinterpret_cast<const uint4*>(src + d) : make_uint4(0, 0, 0, 0);
+      }
+      float qs = p.scale_log2;  // logit scale of head h
+      if (kQuant) {
+        uint32_t top = 0;  // the largest magnitude's bits
+        auto mag = [](uint32_t x) { return max(x << 16 & 0x7fffffffu, x & 0x7fff0000u); };
 #pragma unroll
-    for (int i = 0; i < kDim / 16; ++i)
+        for (int j = 0; j < kDim / 32; ++j) top = max(top, max(max(mag(w[j].x), mag(w[j].y)), max(mag(w[j].z), mag(w[j].w))));
+        top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        const int e = min(max(static_cast<int>(top >> 23) - 127, -112), 126) - 14;  // 2^-e puts the largest in [2^14, 2^15)
+        const float up = exp2i(-e);
+        auto half = [up](uint32_t x) { return pack_half(__uint_as_float(x << 16) * up, __uint_as_float(x & 0xffff0000u) * up); };
 #pragma unroll
-      for (int j = 0; j < 4; ++j) o[nt][i][j] = 0.f;
+        for (int j = 0; j < kDim / 32; ++j) w[j] = make_uint4(half(w[j].x), half(w[j].y), half(w[j].z), half(w[j].w));
+        qs *= exp2i(e);
+      }
 #pragma unroll
-    for (int h = 0; h < 2; ++h) m[nt][h] = -INFINITY, sub[nt][h] = 0.f, l[nt][h] = 0.f, qs[nt][h] = s_qs[nt * 8 + 2 * lc + h];
-  }
-
-  // The unit in the current slot has landed; when the wait ran out, no more are asked for.
-  auto landed = [&](int step) {
-    if (__any_sync(0xffffffffu, !mbar_wait(&full[slot], parity))) {
-      if (lane == 0) kv::set_status(p.c.status, STATUS_TIMEOUT);
-      steps = min(steps, step + (C::kRing + 1) / 2);
+      for (int j = 0; j < kDim / 32; ++j) s_q[(warp * (kDim / 32) + j) * 32 + lane] = w[j];
+      if (lc == 0) s_qs[warp * 8 + lr] = qs;
     }
-  };
-  auto next_slot = [&] {
-    if (++slot == C::kRing) slot = 0, parity ^= 1;
-  };
-  for (int step = 0; step < steps; ++step) {
-    landed(step);
-    const uint8_t* unit = ring + slot * C::kUnit;
-    // a product takes the sum of the one before 25 cycles later: two sums side by side where a step has but one tile
-    constexpr int kChains = kU * kNT == 1 ? 2 : 1;
-    float s[kU][kNT][4], part[kChains][kU][kNT][4];
+    __syncthreads();
+
+    float o[kNT][kDim / 16][4];
+    // Of the lane's two heads a tile: the maximum m (the same in all lanes of a head), what is subtracted (m, or 0
+    // before any logit was seen, less the lift), and a lane's part of l.
+    float m[kNT][2], sub[kNT][2], l[kNT][2], qs[kNT][2];
 #pragma unroll
-    for (int i = 0; i < kChains; ++i)
+    for (int nt = 0; nt < kNT; ++nt) {
+#pragma unroll
+      for (int i = 0; i < kDim / 16; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) o[nt][i][j] = 0.f;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) m[nt][h] = -INFINITY, sub[nt][h] = 0.f, l[nt][h] = 0.f, qs[nt][h] = s_qs[nt * 8 + 2 * lc + h];
+    }
+
+    int ev0 = 0;        // the exponent of the first value row seen
+    bool wide = false;  // a later one is more than 44 away
+
+    // The unit in the current slot has landed; when the wait ran out, no more are asked for.
+    auto landed = [&](int step) {
+      if (__any_sync(0xffffffffu, !mbar_wait(&full[slot], parity))) {
+        if (lane == 0) kv::set_status(p.c.status, STATUS_TIMEOUT);
+        steps = min(steps, step + (C::kRing + 1) / 2);
+        lost = true;
+      }
+    };
+    auto next_slot = [&] {
+      if (++slot == C::kRing) slot = 0, parity ^= 1;
+    };
+    for (int step = 0; step < steps; ++step) {
+      landed(step);
+      const uint8_t* unit = ring + slot * C::kUnit;
+      // a product takes the sum of the one before 25 cycles later: two sums side by side where a step has but one tile
+      constexpr int kChains = kU * kNT == 1 ? 2 : 1;
+      float s[kU][kNT][4], part[kChains][kU][kNT][4];
+#pragma unroll
+      for (int i = 0; i < kChains; ++i)
+#pragma unroll
+        for (int u = 0; u < kU; ++u)
+#pragma unroll
+          for (int nt = 0; nt < kNT; ++nt)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) part[i][u][nt][j] = 0.f;
+      auto key = [&](int u, int half, int j) {
+        constexpr int kIn = C::kBox / 64;  // passes a box
+        return *reinterpret_cast<const uint4*>(unit + u * C::kTileBytes + (j / kIn * kTile + tok + half * 8) * C::kBox +
+                                               (((j % kIn) * 4 + lc) ^ (C::kBox == 128 ? sw : sw & 3)) * 16);
+      };
+#pragma unroll
+      for (int j = 0; j < C::kKP; ++j) {
+        if (!kQuant) {
+          uint4 w[kNT];
+#pragma unroll
+          for (int nt = 0; nt < kNT; ++nt) w[nt] = s_q[(nt * (kDim / 32) + j) * 32 + lane];
+#pragma unroll
+          for (int u = 0; u < kU; ++u) {
+            const uint4 a = key(u, 0, j), b = key(u, 1, j);
+#pragma unroll
+            for (int nt = 0; nt < kNT; ++nt) {
+              mma<false>(part[0][u][nt], a.x, b.x, a.y, b.y, w[nt].x, w[nt].y);
+              mma<false>(part[kChains - 1][u][nt], a.z, b.z, a.w, b.w, w[nt].z, w[nt].w);
+            }
+          }
+        } else {
+          uint4 w[kNT][2];
+#pragma unroll
+          for (int nt = 0; nt < kNT; ++nt)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) w[nt][i] = s_q[(nt * (kDim / 32) + 2 * j + i) * 32 + lane];
+#pragma unroll
+          for (int u = 0; u < kU; ++u) {
+            const uint4 x = key(u, 0, j), y = key(u, 1, j);
+            const uint32_t a[4] = {x.x, x.y, x.z, x.w}, b[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const uint32_t x0 = half_pair(a[i]), x1 = half_pair(b[i]), x2 = half_pair_hi(a[i]), x3 = half_pair_hi(b[i]);
+#pragma unroll
+              for (int nt = 0; nt < kNT; ++nt)
+                mma<true>(part[i % kChains][u][nt], x0, x1, x2, x3, i & 1 ? w[nt][i / 2].z : w[nt][i / 2].x,
+                          i & 1 ? w[nt][i / 2].w : w[nt][i / 2].y);
+            }
+          }
+        }
+      }
 #pragma unroll
       for (int u = 0; u < kU; ++u)
 #pragma unroll
         for (int nt = 0; nt < kNT; ++nt)
 #pragma unroll
-          for (int j = 0; j < 4; ++j) part[i][u][nt][j] = 0.f;
-    auto key = [&](int u, int half, int j) {
-      constexpr int kIn = C::kBox / 64;  // passes a box
-      return *reinterpret_cast<const uint4*>(unit + u * C::kTileBytes + (j / kIn * kTile + tok + half * 8) * C::kBox +
-                                             (((j % kIn) * 4 + lc) ^ (C::kBox == 128 ? sw : sw & 3)) * 16);
-    };
+          for (int j = 0; j < 4; ++j) {
+            s[u][nt][j] = part[0][u][nt][j];
 #pragma unroll
-    for (int j = 0; j < C::kKP; ++j) {
-      if (!kQuant) {
-        uint4 w[kNT];
-#pragma unroll
-        for (int nt = 0; nt < kNT; ++nt) w[nt] = s_q[(nt * (kDim / 32) + j) * 32 + lane];
-#pragma unroll
-        for (int u = 0; u < kU; ++u) {
-          const uint4 a = key(u, 0, j), b = key(u, 1, j);
-#pragma unroll
-          for (int nt = 0; nt < kNT; ++nt) {
-            mma<false>(part[0][u][nt], a.x, b.x, a.y, b.y, w[nt].x, w[nt].y);
-            mma<false>(part[kChains - 1][u][nt], a.z, b.z, a.w, b.w, w[nt].z, w[nt].w);
+            for (int i = 1; i < kChains; ++i) s[u][nt][j] += part[i][u][nt][j];
           }
+      // logits in log2 units (with the value rows' exponents), -inf where nothing is seen
+      float back[kU][2];  // 2^-(exponent + kSpan)
+      if (kQuant && step == 0) ev0 = static_cast<int8_t>(s_exp[slot][0][16 + (s_range[slot][0] & 255)]);
+#pragma unroll
+      for (int u = 0; u < kU; ++u) {
+        float kf[2], vf[2];
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          const int8_t* x = reinterpret_cast<const int8_t*>(&s_exp[slot][u][r * 8 + tok]);
+          kf[r] = kQuant ? exp2i(x[0]) : 1.f;
+          vf[r] = kQuant ? __uint_as_float(0x4b400000u + x[16]) - 12582912.f : 0.f;  // the exponent as a float, off the conversion pipe
+          back[u][r] = kQuant ? exp2i(-min(max(static_cast<int>(x[16]), -119), 119) - kSpan) : 1.f;  // finite in places not seen, too
+          if (kQuant) wide |= static_cast<uint32_t>(x[16] - ev0 + 44) > 88u;
         }
-      } else {
-        uint4 w[kNT][2];
-#pragma unroll
-        for (int nt = 0; nt < kNT; ++nt)
-#pragma unroll
-          for (int i = 0; i < 2; ++i) w[nt][i] = s_q[(nt * (kDim / 32) + 2 * j + i) * 32 + lane];
-#pragma unroll
-        for (int u = 0; u < kU; ++u) {
-          const uint4 x = key(u, 0, j), y = key(u, 1, j);
-          const uint32_t a[4] = {x.x, x.y, x.z, x.w}, b[4] = {y.x, y.y, y.z, y.w};
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const uint32_t x0 = half_pair(a[i]), x1 = half_pair(b[i]), x2 = half_pair_hi(a[i]), x3 = half_pair_hi(b[i]);
-#pragma unroll
-            for (int nt = 0; nt < kNT; ++nt)
-              mma<true>(part[i % kChains][u][nt], x0, x1, x2, x3, i & 1 ? w[nt][i / 2].z : w[nt][i / 2].x,
-                        i & 1 ? w[nt][i / 2].w : w[nt][i / 2].y);
-          }
-        }
-      }
-    }
-#pragma unroll
-    for (int u = 0; u < kU; ++u)
-#pragma unroll
-      for (int nt = 0; nt < kNT; ++nt)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          s[u][nt][j] = part[0][u][nt][j];
-#pragma unroll
-          for (int i = 1; i < kChains; ++i) s[u][nt][j] += part[i][u][nt][j];
-        }
-    // logits in log2 units (with the value rows' exponents), -inf where nothing is seen
-    float back[kU][2];
-#pragma unroll
-    for (int u = 0; u < kU; ++u) {
-      float kf[2], vf[2];
-#pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        const int8_t* x = reinterpret_cast<const int8_t*>(&s_exp[slot][u][r * 8 + tok]);
-        kf[r] = kQuant ? exp2i(x[0]) : 1.f;
-        vf[r] = kQuant ? __uint_as_float(0x4b400000u + x[16]) - 12582912.f : 0.f;  // the exponent as a float, off the conversion pipe
-        back[u][r] = kQuant ? exp2i(-max(static_cast<int>(x[16]), -126)) : 1.f;  // finite in places not seen, too
-      }
-      const int seen = s_range[slot][u];
-#pragma unroll
-      for (int nt = 0; nt < kNT; ++nt)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          float z = s[u][nt][j] * qs[nt][j & 1];
-          if (kQuant) z = z * kf[j >> 1] + vf[j >> 1];
-          s[u][nt][j] = z;
-        }
-      if (seen != kTile << 8)
+        const int seen = s_range[slot][u];
 #pragma unroll
         for (int nt = 0; nt < kNT; ++nt)
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            const int r = tok + (j >> 1) * 8;
-            if (r < (seen & 255) || r >= seen >> 8) s[u][nt][j] = -INFINITY;
+            float z = s[u][nt][j] * qs[nt][j & 1];
+            if (kQuant) z = z * kf[j >> 1] + vf[j >> 1];
+            s[u][nt][j] = z;
           }
-    }
-    __syncwarp();  // the unit is read
-    ask(!(C::kRing & 1), step + C::kRing / 2, slot);
-    next_slot();
-
-    bool above = false;
+        if (seen != kTile << 8)
 #pragma unroll
-    for (int nt = 0; nt < kNT; ++nt)
+          for (int nt = 0; nt < kNT; ++nt)
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        float x = fmaxf(s[0][nt][h], s[0][nt][2 + h]);
-#pragma unroll
-        for (int u = 1; u < kU; ++u) x = fmaxf(x, fmaxf(s[u][nt][h], s[u][nt][2 + h]));
-        above |= x > m[nt][h] + kSlack;
+            for (int j = 0; j < 4; ++j) {
+              const int r = tok + (j >> 1) * 8;
+              if (r < (seen & 255) || r >= seen >> 8) s[u][nt][j] = -INFINITY;
+            }
       }
-    if (__any_sync(0xffffffffu, above)) {
+      __syncwarp();  // the unit is read
+      ask(!(C::kRing & 1), step + C::kRing / 2, slot);
+      next_slot();
+
+      // Weights of rows whose exponents lie far apart can vanish where their share of l does not: from then on l takes its
+      // terms from the logits themselves.
+      if (kQuant) wide = __any_sync(0xffffffffu, wide);
+      bool above = false;
 #pragma unroll
       for (int nt = 0; nt < kNT; ++nt)
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          float x = m[nt][h];
+          float x = fmaxf(s[0][nt][h], s[0][nt][2 + h]);
 #pragma unroll
-          for (int u = 0; u < kU; ++u) x = fmaxf(x, fmaxf(s[u][nt][h], s[u][nt][2 + h]));
-#pragma unroll
-          for (int w = 4; w < 32; w *= 2) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, w));
-          const float f = m[nt][h] == -INFINITY ? 0.f : ex2(m[nt][h] - x);
-          m[nt][h] = x;
-          sub[nt][h] = (x == -INFINITY ? 0.f : x) - (kQuant ? kLift : 0.f);
-          l[nt][h] *= f;
-#pragma unroll
-          for (int i = 0; i < kDim / 16; ++i) o[nt][i][h] *= f, o[nt][i][2 + h] *= f;
+          for (int u = 1; u < kU; ++u) x = fmaxf(x, fmaxf(s[u][nt][h], s[u][nt][2 + h]));
+          above |= x > m[nt][h] + kSlack;
         }
-    }
-    // weights, as the second product's B operands
-    uint32_t ph[kU][kNT][2], pl[kU][kNT][2];
+      if (__any_sync(0xffffffffu, above)) {
 #pragma unroll
-    for (int u = 0; u < kU; ++u)
+        for (int nt = 0; nt < kNT; ++nt)
 #pragma unroll
-      for (int nt = 0; nt < kNT; ++nt) {
-        float w[4];
+          for (int h = 0; h < 2; ++h) {
+            float x = m[nt][h];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          w[j] = ex2(s[u][nt][j] - sub[nt][j & 1]);
-          l[nt][j & 1] += kQuant ? w[j] * back[u][j >> 1] : w[j];
-        }
+            for (int u = 0; u < kU; ++u) x = fmaxf(x, fmaxf(s[u][nt][h], s[u][nt][2 + h]));
 #pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          if (kQuant) {
-            ph[u][nt][r] = transpose8(pack_half(w[2 * r], w[2 * r + 1]));
-          } else {
-            const uint32_t h = pack_bf16(w[2 * r], w[2 * r + 1]);
-            ph[u][nt][r] = transpose8(h);
-            pl[u][nt][r] = transpose8(pack_bf16(w[2 * r] - __uint_as_float(h << 16), w[2 * r + 1] - __uint_as_float(h & 0xffff0000u)));
+            for (int w = 4; w < 32; w *= 2) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, w));
+            const float m_was = m[nt][h], f = m_was == -INFINITY ? 0.f : ex2(m_was - x);
+            m[nt][h] = x;
+            sub[nt][h] = (x == -INFINITY ? 0.f : x) - (kQuant ? kLift : 0.f);
+            l[nt][h] = m_was == -INFINITY ? 0.f : scale_sum(l[nt][h], m_was - x);
+#pragma unroll
+            for (int i = 0; i < kDim / 16; ++i) o[nt][i][h] *= f, o[nt][i][2 + h] *= f;
           }
-        }
       }
-
-    landed(step);
-    unit = ring + slot * C::kUnit;
+      if (kQuant && wide) {
 #pragma unroll
-    for (int u = 0; u < kU; ++u) {
-      const int seen = s_range[slot][u];
+        for (int u = 0; u < kU; ++u)
 #pragma unroll
-      for (int j = 0; j < C::kVP; ++j) {
-        uint32_t v[4][C::kVW];
+          for (int r = 0; r < 2; ++r) {
+            const float shift = static_cast<float>(static_cast<int>(__float_as_uint(back[u][r]) >> 23) - 127);
+            back[u][r] = 0.f;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int t = vtok[i & 1], key = C::kBox == 128 ? t : t >> 1 & 3;
-          const uint8_t* src = unit + u * C::kTileBytes + (j * kTile + t + (i >> 1) * 8) * C::kBox;
-          if constexpr (C::kVB == 16) {
-            const uint4 w = *reinterpret_cast<const uint4*>(src + (lr ^ key) * 16);
-            v[i][0] = w.x, v[i][1] = w.y, v[i][2] = w.z, v[i][3] = w.w;
-          } else {
-            const uint2 w = *reinterpret_cast<const uint2*>(src + (lr * 8 ^ key * 16));
-            v[i][0] = w.x, v[i][1] = w.y;
+            for (int nt = 0; nt < kNT; ++nt)
+#pragma unroll
+              for (int h = 0; h < 2; ++h) l[nt][h] += ex2_all(s[u][nt][2 * r + h] - sub[nt][h] + shift);
+          }
+      }
+      // weights, as the second product's B operands
+      uint32_t ph[kU][kNT][2], pl[kU][kNT][2];
+#pragma unroll
+      for (int u = 0; u < kU; ++u)
+#pragma unroll
+        for (int nt = 0; nt < kNT; ++nt) {
+          float w[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            w[j] = ex2(s[u][nt][j] - sub[nt][j & 1]);
+            l[nt][j & 1] += kQuant ? w[j] * back[u][j >> 1] : w[j];
+          }
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            if (kQuant) {
+              ph[u][nt][r] = transpose8(pack_half(w[2 * r], w[2 * r + 1]));
+            } else {
+              const uint32_t h = pack_bf16(w[2 * r], w[2 * r + 1]);
+              ph[u][nt][r] = transpose8(h);
+              pl[u][nt][r] = transpose8(pack_bf16(w[2 * r] - __uint_as_float(h << 16), w[2 * r + 1] - __uint_as_float(h & 0xffff0000u)));
+            }
           }
         }
-        // what lies in places not seen may be anything, and no weight of zero makes a NaN harmless
-        if (seen != kTile << 8)
+
+      landed(step);
+      unit = ring + slot * C::kUnit;
+#pragma unroll
+      for (int u = 0; u < kU; ++u) {
+        const int seen = s_range[slot][u];
+#pragma unroll
+        for (int j = 0; j < C::kVP; ++j) {
+          uint32_t v[4][C::kVW];
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            const int r = vtok[i & 1] + (i >> 1) * 8;
-            if (r < (seen & 255) || r >= seen >> 8)
-#pragma unroll
-              for (int w = 0; w < C::kVW; ++w) v[i][w] = 0;
-          }
-#pragma unroll
-        for (int w = 0; w < C::kVW; ++w) {
-          const uint32_t t0 = v[0][w], t1 = v[1][w], t8 = v[2][w], t9 = v[3][w];
-          if (!kQuant) {
-            const int tile = j * 4 + w;
-            const uint32_t a0 = __byte_perm(t0, t1, 0x5410), a1 = __byte_perm(t0, t1, 0x7632);
-            const uint32_t a2 = __byte_perm(t8, t9, 0x5410), a3 = __byte_perm(t8, t9, 0x7632);
-#pragma unroll
-            for (int nt = 0; nt < kNT; ++nt) {
-              mma<false>(o[nt][tile], a0, a1, a2, a3, ph[u][nt][0], ph[u][nt][1]);
-              mma<false>(o[nt][tile], a0, a1, a2, a3, pl[u][nt][0], pl[u][nt][1]);
+            const int t = vtok[i & 1], key = C::kBox == 128 ? t : t >> 1 & 3;
+            const uint8_t* src = unit + u * C::kTileBytes + (j * kTile + t + (i >> 1) * 8) * C::kBox;
+            if constexpr (C::kVB == 16) {
+              const uint4 w = *reinterpret_cast<const uint4*>(src + (lr ^ key) * 16);
+              v[i][0] = w.x, v[i][1] = w.y, v[i][2] = w.z, v[i][3] = w.w;
+            } else {
+              const uint2 w = *reinterpret_cast<const uint2*>(src + (lr * 8 ^ key * 16));
+              v[i][0] = w.x, v[i][1] = w.y;
             }
-          } else {
-            const int tile = (j * C::kVW + w) * 2;
-            const uint32_t x0 = __byte_perm(t0, t1, 0x5140), x1 = __byte_perm(t0, t1, 0x7362);
-            const uint32_t y0 = __byte_perm(t8, t9, 0x5140), y1 = __byte_perm(t8, t9, 0x7362);
-            const uint32_t a0 = half_pair(x0), a1 = half_pair_hi(x0), a2 = half_pair(y0), a3 = half_pair_hi(y0);
-            const uint32_t b0 = half_pair(x1), b1 = half_pair_hi(x1), b2 = half_pair(y1), b3 = half_pair_hi(y1);
+          }
+          // what lies in places not seen may be anything, and no weight of zero makes a NaN harmless
+          if (seen != kTile << 8)
 #pragma unroll
-            for (int nt = 0; nt < kNT; ++nt) {
-              mma<true>(o[nt][tile], a0, a1, a2, a3, ph[u][nt][0], ph[u][nt][1]);
-              mma<true>(o[nt][tile + 1], b0, b1, b2, b3, ph[u][nt][0], ph[u][nt][1]);
+            for (int i = 0; i < 4; ++i) {
+              const int r = vtok[i & 1] + (i >> 1) * 8;
+              if (r < (seen & 255) || r >= seen >> 8)
+#pragma unroll
+                for (int w = 0; w < C::kVW; ++w) v[i][w] = 0;
+            }
+#pragma unroll
+          for (int w = 0; w < C::kVW; ++w) {
+            const uint32_t t0 = v[0][w], t1 = v[1][w], t8 = v[2][w], t9 = v[3][w];
+            if (!kQuant) {
+              const int tile = j * 4 + w;
+              const uint32_t a0 = __byte_perm(t0, t1, 0x5410), a1 = __byte_perm(t0, t1, 0x7632);
+              const uint32_t a2 = __byte_perm(t8, t9, 0x5410), a3 = __byte_perm(t8, t9, 0x7632);
+#pragma unroll
+              for (int nt = 0; nt < kNT; ++nt) {
+                mma<false>(o[nt][tile], a0, a1, a2, a3, ph[u][nt][0], ph[u][nt][1]);
+                mma<false>(o[nt][tile], a0, a1, a2, a3, pl[u][nt][0], pl[u][nt][1]);
+              }
+            } else {
+              const int tile = (j * C::kVW + w) * 2;
+              const uint32_t x0 = __byte_perm(t0, t1, 0x5140), x1 = __byte_perm(t0, t1, 0x7362);
+              const uint32_t y0 = __byte_perm(t8, t9, 0x5140), y1 = __byte_perm(t8, t9, 0x7362);
+              const uint32_t a0 = half_pair(x0), a1 = half_pair_hi(x0), a2 = half_pair(y0), a3 = half_pair_hi(y0);
+              const uint32_t b0 = half_pair(x1), b1 = half_pair_hi(x1), b2 = half_pair(y1), b3 = half_pair_hi(y1);
+#pragma unroll
+              for (int nt = 0; nt < kNT; ++nt) {
+                mma<true>(o[nt][tile], a0, a1, a2, a3, ph[u][nt][0], ph[u][nt][1]);
+                mma<true>(o[nt][tile + 1], b0, b1, b2, b3, ph[u][nt][0], ph[u][nt][1]);
+              }
             }
           }
         }
       }
+      __syncwarp();  // the unit is read
+      ask(C::kRing & 1, step + (C::kRing + 1) / 2, slot);
+      next_slot();
     }
-    __syncwarp();  // the unit is read
-    ask(C::kRing & 1, step + (C::kRing + 1) / 2, slot);
-    next_slot();
-  }
 
-  // join the warps; the ring's place is free once every warp is here (it has waited for all that it asked for)
-  float(*s_o)[kNT * 4][C::kPitch] = reinterpret_cast<float(*)[kNT * 4][C::kPitch]>(smem);
+    // join the warps; the ring's place is free once every warp is here (it has waited for all that it asked for)
+    float(*s_o)[kNT * 4][C::kPitch] = reinterpret_cast<float(*)[kNT * 4][C::kPitch]>(smem);
 #pragma unroll
-  for (int nt = 0; nt < kNT; ++nt)
+    for (int nt = 0; nt < kNT; ++nt)
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
+      for (int h = 0; h < 2; ++h) {
 #pragma unroll
-      for (int w = 4; w < 32; w *= 2) l[nt][h] += __shfl_xor_sync(0xffffffffu, l[nt][h], w);
-      if (lr == 0) s_m[warp][nt * 8 + 2 * lc + h] = m[nt][h], s_l[warp][nt * 8 + 2 * lc + h] = l[nt][h];
-    }
-  __syncthreads();
-  const bool whole = p.splits ? p.splits == 1 : begin == 0 && end == sp.tiles;
-  const int64_t to = 2 * static_cast<int64_t>(blockIdx.x) + (part ? 1 : 0);  // stream: where a shared row's part goes
-  if (threadIdx.x < C::kHeads) {  // each warp's factor into s_m, the joined sum and maximum into s_l[0], s_l[1]
-    const int h = threadIdx.x;
-    float mm = -INFINITY, ll = 0.f;
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) mm = fmaxf(mm, s_m[w][h]);
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
-      const float f = s_m[w][h] == -INFINITY ? 0.f : ex2(s_m[w][h] - mm);
-      ll += s_l[w][h] * f;
-      s_m[w][h] = f;
-    }
-    s_l[0][h] = ll, s_l[1][h] = mm;
-    s_qs[h] = whole ? (ll == 0.f ? 0.f : 1.f / ll) : 1.f;
-    if (whole) {
-      if (h0 + h < p.group) p.lse[qrow + h] = lse_of(mm, ll, kQuant);
-    } else if (!p.splits) {
-      p.part_ml[to * C::kHeads + h] = make_float2(mm, ll);
-    }
-  }
-  // (value d of both heads of a pair) at d with its low bits turned by lr, so that neither these writes (lanes kE
-  // values apart) nor the reads (neighbours) meet on a bank
-#pragma unroll
-  for (int nt = 0; nt < kNT; ++nt)
-#pragma unroll
-    for (int i = 0; i < kDim / 16; ++i)
-#pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        const int d = i / (C::kE / 2) * 8 * C::kE + lr * C::kE + i % (C::kE / 2) * 2 + r;
-        *reinterpret_cast<float2*>(&s_o[warp][nt * 4 + lc][(d ^ (lr & 3)) * 2]) = make_float2(o[nt][i][2 * r], o[nt][i][2 * r + 1]);
+        for (int w = 4; w < 32; w *= 2) l[nt][h] += __shfl_xor_sync(0xffffffffu, l[nt][h], w);
+        if (lr == 0) s_m[warp][nt * 8 + 2 * lc + h] = m[nt][h], s_l[warp][nt * 8 + 2 * lc + h] = l[nt][h];
       }
-  __syncthreads();
-  auto place = [&](int d) { return (d ^ (d / C::kE & 3)) * 2; };
-  auto put = [&](int h, int d, float x, float y) {
-    if (h0 + h < p.group) p.out[(qrow + h) * kDim + d] = __float2bfloat16_rn(x);
-    if (h0 + h + 1 < p.group) p.out[(qrow + h + 1) * kDim + d] = __float2bfloat16_rn(y);
-  };
-  for (int i = threadIdx.x; i < C::kHeads / 2 * kDim; i += blockDim.x) {
-    const int hp = i / kDim, d = i % kDim, h = 2 * hp;
-    float x = 0.f, y = 0.f;
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
-      const float2 v = *reinterpret_cast<const float2*>(&s_o[w][hp][place(d)]);
-      const float2 f = *reinterpret_cast<const float2*>(&s_m[w][h]);
-      x += v.x * f.x, y += v.y * f.y;
-    }
-    x *= s_qs[h], y *= s_qs[h + 1];
-    if (whole) {
-      put(h, d, x, y);
-    } else if (p.splits) {
-      *reinterpret_cast<float2*>(&s_o[0][hp][place(d)]) = make_float2(x, y);  // read by this thread alone so far
-    } else {
-      float* dst = p.part_o + (to * C::kHeads + h) * kDim + d;
-      dst[0] = x, dst[kDim] = y;
-    }
-  }
-  if (p.splits) {
-    if (p.splits == 1) return;
-    // every CTA of the cluster joins its part of the values
-    const int rank = blockIdx.x;
-    float(*const s_f)[C::kHeads] = s_m + 2 * kWarps + 1;  // [splits]
-    cluster_sync();
-    if (threadIdx.x < C::kHeads) {
+    __syncthreads();
+    const bool whole = p.splits ? p.splits == 1 : begin == 0 && end == sp.tiles;
+    const int64_t to = 2 * static_cast<int64_t>(blockIdx.x) + (part ? 1 : 0);  // stream: where a shared row's part goes
+    if (threadIdx.x < C::kHeads) {  // each warp's factor into s_m, the joined sum and maximum into s_l[0], s_l[1]
       const int h = threadIdx.x;
       float mm = -INFINITY, ll = 0.f;
-      for (int r = 0; r < p.splits; ++r) {
-        s_f[r][h] = ld_cluster(&s_l[1][h], r);
-        mm = fmaxf(mm, s_f[r][h]);
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) mm = fmaxf(mm, s_m[w][h]);
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) {
+        const float f = s_m[w][h] == -INFINITY ? 0.f : ex2(s_m[w][h] - mm);
+        ll += s_m[w][h] == -INFINITY ? 0.f : scale_sum(s_l[w][h], s_m[w][h] - mm);
+        s_m[w][h] = f;
       }
-      for (int r = 0; r < p.splits; ++r) {
-        const float f = s_f[r][h] == -INFINITY ? 0.f : ex2(s_f[r][h] - mm);
-        ll += ld_cluster(&s_l[0][h], r) * f;
-        s_f[r][h] = f;
+      s_l[0][h] = ll, s_l[1][h] = mm;
+      s_qs[h] = whole ? inverse(ll, kQuant) : 1.f;
+      if (whole) {
+        if (h0 + h < p.group) p.lse[qrow + h] = lse_of(mm, ll, kQuant);
+      } else if (!p.splits) {
+        p.part_ml[to * C::kHeads + h] = make_float2(mm, ll);
       }
-      s_qs[h] = ll == 0.f ? 0.f : 1.f / ll;
-      if (rank == 0 && h0 + h < p.group) p.lse[qrow + h] = lse_of(mm, ll, kQuant);
     }
+    // (value d of both heads of a pair) at d with its low bits turned by lr, so that neither these writes (lanes kE
+    // values apart) nor the reads (neighbours) meet on a bank
+#pragma unroll
+    for (int nt = 0; nt < kNT; ++nt)
+#pragma unroll
+      for (int i = 0; i < kDim / 16; ++i)
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          const int d = i / (C::kE / 2) * 8 * C::kE + lr * C::kE + i % (C::kE / 2) * 2 + r;
+          *reinterpret_cast<float2*>(&s_o[warp][nt * 4 + lc][(d ^ (lr & 3)) * 2]) = make_float2(o[nt][i][2 * r], o[nt][i][2 * r + 1]);
+        }
     __syncthreads();
-    for (int i = rank * blockDim.x + threadIdx.x; i < C::kHeads / 2 * kDim; i += p.splits * blockDim.x) {
+    auto place = [&](int d) { return (d ^ (d / C::kE & 3)) * 2; };
+    auto put = [&](int h, int d, float x, float y) {
+      if (h0 + h < p.group) p.out[(qrow + h) * kDim + d] = __float2bfloat16_rn(x);
+      if (h0 + h + 1 < p.group) p.out[(qrow + h + 1) * kDim + d] = __float2bfloat16_rn(y);
+    };
+    for (int i = threadIdx.x; i < C::kHeads / 2 * kDim; i += blockDim.x) {
       const int hp = i / kDim, d = i % kDim, h = 2 * hp;
       float x = 0.f, y = 0.f;
-#pragma unroll 4
-      for (int r = 0; r < p.splits; ++r) {
-        const float2 v = ld_cluster2(&s_o[0][hp][place(d)], r);
-        x += v.x * s_f[r][h], y += v.y * s_f[r][h + 1];
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) {
+        const float2 v = *reinterpret_cast<const float2*>(&s_o[w][hp][place(d)]);
+        const float2 f = *reinterpret_cast<const float2*>(&s_m[w][h]);
+        x += v.x * f.x, y += v.y * f.y;
       }
-      put(h, d, x * s_qs[h], y * s_qs[h + 1]);
+      x *= s_qs[h], y *= s_qs[h + 1];
+      if (whole) {
+        put(h, d, x, y);
+      } else if (p.splits) {
+        *reinterpret_cast<float2*>(&s_o[0][hp][place(d)]) = make_float2(x, y);  // read by this thread alone so far
+      } else {
+        float* dst = p.part_o + (to * C::kHeads + h) * kDim + d;
+        dst[0] = x, dst[kDim] = y;
+      }
     }
-    cluster_sync();  // no CTA leaves while another reads its shared memory
-    return;
-  }
-  left -= end - begin;
-  if (left <= 0) return;
-  ++part;
-  row = next_row, unit = next_unit, sp = next_sp;
-  begin = 0, end = min(left, sp.tiles);
-  tc::fence_proxy_async_smem();  // the join's reads and writes of the ring come before the next copies into it
-  __syncthreads();
+    if (p.splits) {
+      if (p.splits == 1) return;
+      // every CTA of the cluster joins its part of the values
+      const int rank = blockIdx.x;
+      float(*const s_f)[C::kHeads] = s_m + 2 * kWarps + 1;  // [splits]
+      cluster_sync();
+      if (threadIdx.x < C::kHeads) {
+        const int h = threadIdx.x;
+        float mm = -INFINITY, ll = 0.f;
+        for (int r = 0; r < p.splits; ++r) {
+          s_f[r][h] = ld_cluster(&s_l[1][h], r);
+          mm = fmaxf(mm, s_f[r][h]);
+        }
+        for (int r = 0; r < p.splits; ++r) {
+          const float f = s_f[r][h] == -INFINITY ? 0.f : ex2(s_f[r][h] - mm);
+          ll += s_f[r][h] == -INFINITY ? 0.f : scale_sum(ld_cluster(&s_l[0][h], r), s_f[r][h] - mm);
+          s_f[r][h] = f;
+        }
+        s_qs[h] = inverse(ll, kQuant);
+        if (rank == 0 && h0 + h < p.group) p.lse[qrow + h] = lse_of(mm, ll, kQuant);
+      }
+      __syncthreads();
+      for (int i = rank * blockDim.x + threadIdx.x; i < C::kHeads / 2 * kDim; i += p.splits * blockDim.x) {
+        const int hp = i / kDim, d = i % kDim, h = 2 * hp;
+        float x = 0.f, y = 0.f;
+#pragma unroll 4
+        for (int r = 0; r < p.splits; ++r) {
+          const float2 v = ld_cluster2(&s_o[0][hp][place(d)], r);
+          x += v.x * s_f[r][h], y += v.y * s_f[r][h + 1];
+        }
+        put(h, d, x * s_qs[h], y * s_qs[h + 1]);
+      }
+      cluster_sync();  // no CTA leaves while another reads its shared memory
+      return;
+    }
+    left -= end - begin;
+    if (left <= 0) return;
+    ++part;
+    row = next_row, unit = next_unit, sp = next_sp;
+    begin = 0, end = min(left, sp.tiles);
+    tc::fence_proxy_async_smem();  // the join's reads and writes of the ring come before the next copies into it
+    if (__syncthreads_or(lost)) return;
   }
 }
 
@@ -812,11 +849,12 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constan
 #pragma unroll
     for (int b = 0; b < kJoinBatch; ++b) mm = fmaxf(mm, a[b].x);
     const float back = m == -INFINITY ? 0.f : ex2(m - mm);
-    l *= back, x.x *= back, x.y *= back, x.z *= back, x.w *= back;
+    l = m == -INFINITY ? 0.f : scale_sum(l, m - mm);
+    x.x *= back, x.y *= back, x.z *= back, x.w *= back;
 #pragma unroll
     for (int b = 0; b < kJoinBatch; ++b) {
       const float f = a[b].x == -INFINITY ? 0.f : ex2(a[b].x - mm);
-      l += a[b].y * f;
+      l += a[b].x == -INFINITY ? 0.f : scale_sum(a[b].y, a[b].x - mm);
       x.x += y[b].x * f, x.y += y[b].y * f, x.z += y[b].z * f, x.w += y[b].w * f;
     }
     m = mm;
@@ -828,18 +866,19 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constan
     float mm = m;
     for (int i = 1; i < groups; ++i) mm = fmaxf(mm, s_m[i * per + threadIdx.x]);
     const float f0 = m == -INFINITY ? 0.f : ex2(m - mm);
-    l *= f0, x.x *= f0, x.y *= f0, x.z *= f0, x.w *= f0;
+    l = m == -INFINITY ? 0.f : scale_sum(l, m - mm);
+    x.x *= f0, x.y *= f0, x.z *= f0, x.w *= f0;
     for (int i = 1; i < groups; ++i) {
       const float mi = s_m[i * per + threadIdx.x], f = mi == -INFINITY ? 0.f : ex2(mi - mm);
       const float4 y = s_x[i * per + threadIdx.x];
-      l += s_l[i * per + threadIdx.x] * f;
+      l += mi == -INFINITY ? 0.f : scale_sum(s_l[i * per + threadIdx.x], mi - mm);
       x.x += y.x * f, x.y += y.y * f, x.z += y.z * f, x.w += y.w * f;
     }
     m = mm;
   }
   if (!on) return;
   const int64_t head = static_cast<int64_t>(row) * p.q_heads + unit / p.head_tiles * p.group + in_group;
-  const float inv = l == 0.f ? 0.f : 1.f / l;
+  const float inv = inverse(l, quant);
   const int d = i4 * 4 - h * dim;
   *reinterpret_cast<uint2*>(p.out + head * dim + d) = make_uint2(pack_bf16(x.x * inv, x.y * inv), pack_bf16(x.z * inv, x.w * inv));
   if (d == 0) p.lse[head] = lse_of(m, l, quant);
@@ -967,6 +1006,7 @@ extern "C" int dm3_paged_attention(const void* q, int64_t q_rs, int64_t q_hs, in
   if (q_heads < kv_heads || q_heads % kv_heads || q_heads > 65535)
     return set_error("paged_attention: the query heads must be a multiple of the cache's heads"), DM3_EINVAL;
   if (rows > 65535) return set_error("paged_attention: at most 65535 rows"), DM3_EINVAL;
+  if (static_cast<int64_t>(rows) * q_heads > INT32_MAX) return set_error("paged_attention: too many rows and heads"), DM3_EINVAL;
   if (window < 0 || !std::isfinite(scale)) return set_error("paged_attention: bad window or scale"), DM3_EINVAL;
   if (rows == 0) return DM3_OK;
   if (!q || !lengths || !out || !lse) return set_error("paged_attention: null pointer"), DM3_EINVAL;

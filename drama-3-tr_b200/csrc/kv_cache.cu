@@ -520,6 +520,8 @@ bool kv_cache_ok(const kv::Cache& c, int kv_heads, int dim) {
   if (!c.k_exp != !c.v_exp) return set_error("cache: one of the exponent tables is missing"), false;
   if (c.rows < 0 || c.per_row < 0 || (c.rows > 0 && c.per_row > 0 && !c.table) || c.table_stride < c.per_row)
     return set_error("bad page table"), false;
+  if (static_cast<int64_t>(c.per_row) * c.page_size > INT32_MAX || static_cast<int64_t>(kv_heads) * c.page_size > INT32_MAX)
+    return set_error("cache: a row's table, or a page, of 2^31 tokens and more"), false;
   const int64_t row = static_cast<int64_t>(kv_heads) * c.page_size;
   const int unit = c.k_exp ? 16 : 8;  // elements in 16 bytes
   if (c.page_stride < row * dim || c.page_stride % unit || (c.k_exp && (c.exp_stride < row || c.exp_stride % 16)))

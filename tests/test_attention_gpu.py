@@ -120,6 +120,21 @@ def test_queries_of_extreme_size(dm3):
             check_attention(*_run(dm3, d, q, 1.0 / size), d, q, 1.0 / size)
 
 
+def test_value_rows_of_extreme_size(dm3):
+    """Quantised value rows whose exponents lie at either end, alone and mixed, short and long: weights and sums stay in range."""
+    for lengths in ([700, 20000], [33, 64, 1]):
+        d = paged(lengths, 1, 64, 16, True, 8)
+        q = _q(len(lengths), 4, 64, 2, 2.0)
+        e = d["v_exp"].clone()
+        for low, high in ((-110, -110), (119, 119), (-110, 119)):
+            d["v_exp"] = torch.where(torch.rand(e.shape, generator=torch.Generator().manual_seed(1)) < 0.9, low, high).to(torch.int8)
+            out, lse = _run(dm3, d, q)
+            scale = 2.0 ** -max(low, high)  # the check's absolute floor is far from these values
+            d["v_exp"] = (d["v_exp"].int() - max(low, high)).clamp(min=-128).to(torch.int8)
+            # 448 * 2^119 is the largest value a cache holds; a sum of weights of one cannot exceed it
+            check_attention(out.double() * scale, lse, d, q)
+
+
 def test_bad_pages_and_lengths(dm3):
     """Tokens of a page outside the cache are left out and reported, a length behind the table is cut and reported."""
     for quant in (False, True):

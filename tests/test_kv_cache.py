@@ -129,7 +129,10 @@ ODD = ctypes.c_void_p(264)  # not on 16 bytes
 BAD_CACHE = [dict(dim=96), dict(dim=0), dict(kv_heads=0), dict(page_size=8), dict(page_size=40), dict(pages=0), dict(k_cache=None), dict(v_cache=None),
              dict(k_cache=ODD), dict(v_cache=ODD), dict(status=None), dict(k_exp=P), dict(v_exp=P), dict(page_stride=2 * 16 * 64 - 8),
              dict(page_stride=2 * 16 * 64 + 4), dict(k_exp=P, v_exp=P, exp_stride=31, page_stride=2 * 16 * 64), dict(table=None),
-             dict(table_stride=3), dict(table_rows=-1), dict(per_row=-1)]
+             dict(table_stride=3), dict(table_rows=-1), dict(per_row=-1),
+             dict(page_size=1 << 28, page_stride=1 << 36, exp_stride=1 << 36, per_row=8, table_stride=8),
+             dict(page_size=1 << 28, page_stride=1 << 40, kv_heads=8), dict(k_exp=P, v_exp=P, exp_stride=40),
+             dict(k_exp=ctypes.c_void_p(264), v_exp=P, exp_stride=32)]
 BAD = {
     "dm3_rope": [dict(T=-1), dict(heads=0), dict(dim=0), dict(rot=0), dict(rot=7), dict(rot=66), dict(rot=2048, dim=4096), dict(x=None),
                  dict(positions=None), dict(inv_freq=None), dict(y=None), dict(heads=1 << 20)],
