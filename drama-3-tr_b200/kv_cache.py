@@ -71,7 +71,8 @@ class KVCache:
     k, v [layers, pages, kv_heads, page_size, head_dim] bf16, or float8_e4m3fn with one power-of-two exponent a
     token and head in k_exp, v_exp (int8 [layers, pages, kv_heads, page_size]): half the memory and traffic.
     table int32 [rows, pages_per_row] on the device, -1 where a row has no page. status: one device word that
-    collects tokens which the kernels skipped because their page or place does not exist (`check`)."""
+    collects tokens which the kernels skipped because their page or place does not exist (4), and waits that
+    ran out (1); `check` reads it."""
 
     def __init__(self, layers: int, rows: int, tokens_per_row: int, kv_heads: int, head_dim: int, page_size: int = 64,
                  pages: Optional[int] = None, quantised: bool = False, device="cuda"):

@@ -1,6 +1,7 @@
 /*
  * drama3-b200 C ABI: the drop-in boundary for the Drama-3 per-frame MoE feed-forward and the
- * block-FP8 GEMV, built for NVIDIA B200 (sm_100a).
+ * block-FP8 GEMV, and the attention side of a frame (rotary positions, paged key-value cache,
+ * one-token attention), built for NVIDIA B200 (sm_100a).
  *
  * Every entry point takes raw device pointers, explicit sizes and strides, and a cudaStream_t
  * passed as `void*` (0 = legacy default stream). Nothing here allocates device memory except
@@ -384,10 +385,12 @@ int dm3_rope(const void* x, int T, int heads, int dim, int64_t ts, int64_t hs, c
  *                     bf16 when k_exp and v_exp are null, else e4m3 codes
  *   k_exp, v_exp      int8 [pages][kv_heads][page_size], pages exp_stride apart: a row stands for
  *                     code * 2^exp, exp = the smallest with amax <= 448 * 2^exp, in [-110, 119]
+ *                     (16-byte aligned, exp_stride a multiple of 16)
  *   table             int32 [table_rows][per_row] page ids, rows table_stride apart: token t of row r lies
  *                     in page table[r][t / page_size]
- *   status            one device word; STATUS_BAD_PAGE (4) is or-ed in when a page id, row, position or
- *                     length outside the cache or table was met (such tokens are skipped, never accessed)
+ *   status            one device word; bit 4 is or-ed in when a page id, row, position or length outside
+ *                     the cache or table was met (such tokens are skipped, never accessed), bit 1 when a bounded
+ *                     wait of dm3_paged_attention ran out (its output is then not valid)
  * dim 64, 128, 192 or 256; page_size a multiple of 16.
  */
 

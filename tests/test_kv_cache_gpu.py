@@ -123,6 +123,66 @@ def test_kv_write(dm3, dim, kv_heads, q_heads, size, rot, quant, interleaved):
     assert int(dev["status"]) == 0
 
 
+@pytest.mark.parametrize("tokens", [700, 4800, 9001])
+@pytest.mark.parametrize("quant", [False, True])
+def test_many_tokens(dm3, tokens, quant):
+    """Enough tokens for blocks of several a CTA, the last one cut short: every one where it belongs."""
+    dim, size = 64, 16
+    g = torch.Generator().manual_seed(tokens)
+    c = dm3.KVCache(1, 3, tokens, 1, dim, page_size=size, quantised=quant)
+    c.reserve(1, tokens)
+    x = torch.randn(tokens, 5, dim, generator=g).to(BF)
+    q, k, v = x.split([3, 1, 1], 1)
+    xd = x.cuda()
+    pos = torch.randperm(tokens, generator=g)
+    rope = dm3.Rope(32, 1e5, True)
+    out = c.write(0, xd[:, 3:4], xd[:, 4:], pos.cuda(), torch.ones(tokens, dtype=torch.int64).cuda(), xd[:, :3], rope)
+    inv = rope.inv_freq.cpu()
+    _near(out, q, kv_oracle.rope(q, pos, inv, True), 32)
+    _near(rope(xd, pos.cuda()), x, kv_oracle.rope(x, pos, inv, True), 32)
+    rk, rv = c.read(0, torch.tensor([0, tokens, 0]).cuda(), tokens)
+    kr = kv_oracle.rope(k, pos, inv, True)[:, 0]
+    if quant:
+        assert torch.equal(rk[1, 0].double().cpu()[pos], kv_oracle.quantise(kr.to(BF))[0])
+        assert torch.equal(rv[1, 0].double().cpu()[pos], kv_oracle.quantise(v[:, 0])[0])
+    else:
+        _near(rk[1].transpose(0, 1)[pos.cuda()], k, kr[:, None], 32)
+        assert torch.equal(rv[1, 0].cpu()[pos], v[:, 0])
+    assert (rk[0] == 0).all() and (rk[2] == 0).all() and c.check() == 0
+
+
+def test_traced_calls_are_the_same(dm3):
+    """Under torch.compile the ops are traced as operators, with the same results and the same writes."""
+    g = torch.Generator().manual_seed(3)
+    x = torch.randn(2, 8, 64, generator=g).to(BF).cuda()
+    rope = dm3.Rope(64, device="cuda")
+    pos = torch.tensor([17, 4]).cuda()
+
+    def frame(cache, x, pos):
+        q = cache.write(0, x[:, :2], x[:, 2:4], pos, None, x[:, 4:], rope)
+        out, lse = cache.attend(0, q, pos + 1)
+        k, v = cache.read(0, pos + 1, 20)
+        return rope(q, pos), out, lse, k, v
+
+    got = []
+    for traced in (False, True):
+        cache = dm3.KVCache(1, 2, 32, 2, 64, page_size=16, quantised=True)
+        for r in range(2):
+            cache.reserve(r, 32)
+        fn = torch.compile(frame, backend="aot_eager", dynamic=False, fullgraph=True) if traced else frame
+        got.append([*fn(cache, x, pos), cache.k.view(torch.uint8).clone(), cache.v_exp.clone()])
+    for a, b in zip(*got):
+        assert torch.equal(a, b)
+
+
+def test_gradients_are_refused(dm3):
+    """No operator here has a gradient: one that is asked for is an error, not a silent zero."""
+    x = torch.randn(2, 1, 64, dtype=BF, device="cuda", requires_grad=True)
+    y = dm3.Rope(64)(x, torch.arange(2).cuda())
+    with pytest.raises(RuntimeError):
+        y.sum().backward()
+
+
 def test_kv_write_extremes(dm3):
     """Rows of zeros, one huge value, the largest and smallest bf16, subnormals, infinities and NaN; ties."""
     dim = 64
