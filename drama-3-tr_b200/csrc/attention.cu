@@ -67,6 +67,7 @@ struct Params {
   float scale_log2;  // scale * log2(e)
   int64_t window;
   int splits;          // CTAs of a cluster; 0: stream
+  bool longest_first;  // one CTA a unit: blockIdx.z counts the rows by their tiles
   __nv_bfloat16* out;  // [rows][q_heads][dim]
   float* lse;          // [rows][q_heads]
   // stream: the first tile of each row in the sequence and their number ([rows + 1], a tile counted once a head unit),
@@ -180,6 +181,7 @@ struct Shape {
   static constexpr int kRingBytes = kWarps * kRing * kUnit;
   static constexpr int kShared = 1024 + kRingBytes + kQBytes + kWarps * kRing * kSide + kStats;
   static_assert(kRing >= 2 && kWarps * kNT * 4 * kPitch * 4 <= kRingBytes, "the ring holds two units and the join");
+  static_assert(kStats >= 129 * 4, "room for row_by_length");
 };
 // The token that lane group lr's rows of a tile hold (and + 8): with it, the eight lanes of every 16-byte shared
 // memory access, of keys (two lane groups, four chunks) as of values (two chunks, four tokens), fall on
@@ -222,6 +224,26 @@ __device__ __forceinline__ float2 ld_cluster2(const float* p, int rank) {
   float2 v;
   asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(in_cta(p, rank)) : "memory");
   return v;
+}
+
+// The row with the nth most tiles, of 128 rows at most (the nth one where all are short). All threads call it; scratch: 129
+// words, 16-byte aligned.
+__device__ __forceinline__ int64_t row_by_length(const Params& p, int nth, int* scratch) {
+  constexpr int kShort = 24;
+  const int t = threadIdx.x, tiles = t < p.c.rows ? static_cast<int>(min(row_span(p, t).tiles, int64_t(1) << 23)) : 0;
+  const int mine = t < p.c.rows ? tiles * (kWarps * 32) + kWarps * 32 - 1 - t : -1;  // tiles, then the lower row: no two alike
+  scratch[t] = mine;
+  if (!__syncthreads_or(tiles > kShort)) return nth;
+  int before = 0;
+  for (int j = 0; j < p.c.rows; j += 4) {
+    const int4 x = *reinterpret_cast<const int4*>(scratch + j);
+    before += (x.x > mine) + (x.y > mine) + (x.z > mine) + (x.w > mine);
+  }
+  if (t < p.c.rows && before == nth) scratch[kWarps * 32] = t;
+  __syncthreads();
+  const int64_t row = scratch[kWarps * 32];
+  __syncthreads();  // the scratch is free
+  return row;
 }
 
 // Stream: counts the rows' tiles and finds where this CTA's share of the sequence begins; CTA 0 leaves the rows' places for
@@ -312,7 +334,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2)
   int64_t left = 0;  // stream: tiles of this CTA's share from the segment on
   int part = 0;      // stream: segments done
   if (p.splits) {
-    row = blockIdx.z, unit = blockIdx.y;
+    row = p.longest_first ? row_by_length(p, blockIdx.z, reinterpret_cast<int*>(s_m)) : blockIdx.z, unit = blockIdx.y;
     sp = row_span(p, row);
     const int64_t chunk = max((sp.tiles + p.splits - 1) / p.splits, static_cast<int64_t>(kWarps));
     begin = min(blockIdx.x * chunk, sp.tiles);
@@ -635,9 +657,11 @@ __global__ void __launch_bounds__(kWarps * 32, 2)
             if (kQuant) {
               ph[u][nt][r] = transpose8(pack_half(w[2 * r], w[2 * r + 1]));
             } else {
-              const uint32_t h = pack_bf16(w[2 * r], w[2 * r + 1]);
-              ph[u][nt][r] = transpose8(h);
-              pl[u][nt][r] = transpose8(pack_bf16(w[2 * r] - __uint_as_float(h << 16), w[2 * r + 1] - __uint_as_float(h & 0xffff0000u)));
+              // high part cut, so the low part has its sign and, kept from zero, an infinite value stays infinite
+              const uint32_t x = __float_as_uint(w[2 * r]), y = __float_as_uint(w[2 * r + 1]);
+              ph[u][nt][r] = transpose8(__byte_perm(x, y, 0x7632));
+              pl[u][nt][r] = transpose8(pack_bf16(fmaxf(w[2 * r] - __uint_as_float(x & 0xffff0000u), 0x1p-120f),
+                                                  fmaxf(w[2 * r + 1] - __uint_as_float(y & 0xffff0000u), 0x1p-120f)));
             }
           }
         }
@@ -896,13 +920,16 @@ static int tile_heads(int group) { return group > 8 ? 16 : 8; }
 // How a call is laid out, from its sizes and the table's width (`tiles` of 16 tokens a row at most): the quickest by a model
 // of the time in microseconds, in which the longest row fills the table and the rows are 0.7 of it on average.
 //   A CTA reads about 56 KB a microsecond (35 KB of e4m3), the machine 6.2 MB (4.5 MB). A launch with its first copies and
-//   last sums takes 4.5 (one CTA a unit) or 7.5 (a cluster a unit); one CTA a unit leaves the machine idle at the end,
-//   5%; the stream takes 12 (the count of the rows, and the join's launch).
+//   last sums takes 4.5 (one CTA a unit) or 7.5 (a cluster a unit). One CTA a unit leaves the machine idle at the end, 5%,
+//   unless the units are more than run at once and the longest start first, which takes 1.5 (row_by_length). The
+//   stream takes 12 (the count of the rows, and the join's launch).
 // Measured at 1 / 4 / 32 / 128 units (one row, 2 x 2, 8 x 4, 16 x 8) of up to 1,000 tokens: one CTA a unit 19.8 / 19.8 /
 // 12.3 / 15.5 us, clusters 10.0 / 10.1 / 8.5 / -, stream 10.4 / 13.5 / 13.8 / 22.4; of up to 8,000: 129 / 129 / 74 / 83,
-// 22.6 / 22.7 / 26 / -, 13.0 / 16.8 / 23.7 / 67 (256-value heads for the first two, else 128; bf16).
+// 22.6 / 22.7 / 26 / -, 13.0 / 16.8 / 23.7 / 67 (256-value heads for the first two, else 128; bf16). 512 units (64 x 8) of up
+// to 8,192: one CTA a unit 193, longest first 169, stream 185; of up to 2,000 50.3 and 44.7; of up to 600 21.5 and 22.1.
 struct Plan {
   int head_tiles, splits, ctas;  // splits: CTAs of a cluster, 0: stream over `ctas`
+  bool longest_first;            // more CTAs than run at once: the long rows' start first
 };
 static Plan plan(int rows, int q_heads, int kv_heads, int dim, int page_size, int per_row, bool quant, int64_t window) {
   Plan r{};
@@ -912,12 +939,15 @@ static Plan plan(int rows, int q_heads, int kv_heads, int dim, int page_size, in
   r.head_tiles = (group + heads - 1) / heads;
   const double units = static_cast<double>(rows) * kv_heads * r.head_tiles, unit = static_cast<double>(tiles) * dim * (quant ? 32 : 64);
   const double all = 0.7 * units * unit / (quant ? 4.5e6 : 6.2e6);
+  const bool sorted = units > ctas && tiles >= 48 && rows > 1 && rows <= kWarps * 32;
   double best = 12 + all;
   r.ctas = ctas;
   for (int s = 1; s <= kMaxCluster && (s == 1 || units * s <= sms()); s *= 2) {
-    const double one = unit / s / (quant ? 35e3 : 56e3), t = s == 1 ? 4.5 + (one > 1.05 * all ? one : 1.05 * all) : 7.5 + (one > all ? one : all);
+    const double one = unit / s / (quant ? 35e3 : 56e3), end = s == 1 && !sorted ? 1.05 * all : all;
+    const double t = (s > 1 ? 7.5 : sorted ? 6 : 4.5) + (one > end ? one : end);
     if (t < best) best = t, r.splits = s;
   }
+  r.longest_first = r.splits == 1 && sorted;
   return r;
 }
 static size_t part_bytes(const Plan& r, int rows, int q_heads, int kv_heads, int dim) {
@@ -1014,7 +1044,7 @@ extern "C" int dm3_paged_attention(const void* q, int64_t q_rs, int64_t q_hs, in
     return set_error("paged_attention: rows must start on 16 bytes"), DM3_EINVAL;
   const attn::Plan plan = attn::plan(rows, q_heads, kv_heads, dim, page_size, per_row, k_exp != nullptr, window);
   p.q = static_cast<const __nv_bfloat16*>(q), p.q_rs = q_rs, p.q_hs = q_hs, p.q_heads = q_heads, p.kv_heads = kv_heads;
-  p.group = q_heads / kv_heads, p.head_tiles = plan.head_tiles, p.splits = plan.splits;
+  p.group = q_heads / kv_heads, p.head_tiles = plan.head_tiles, p.splits = plan.splits, p.longest_first = plan.longest_first;
   p.lengths = lengths, p.scale_log2 = scale * 1.44269504088896341f, p.window = window;
   p.out = static_cast<__nv_bfloat16*>(out), p.lse = lse;
   const int heads = attn::tile_heads(p.group);

@@ -12,8 +12,6 @@ enum : uint32_t {
 
 namespace kv {
 
-constexpr int kMaxDim = 256;
-
 struct Cache {
   void *k, *v;            // [pages][kv_heads][page_size][dim] bf16, or e4m3 codes
   int8_t *k_exp, *v_exp;  // [pages][kv_heads][page_size] exponents of an e4m3 cache, else null

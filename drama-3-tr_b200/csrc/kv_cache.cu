@@ -518,7 +518,8 @@ bool kv_cache_ok(const kv::Cache& c, int kv_heads, int dim) {
   if (c.page_size < 16 || c.page_size % 16) return set_error("page_size must be a multiple of 16"), false;
   if (c.pages < 1 || !c.k || !c.v || !c.status) return set_error("cache: null pointer or no pages"), false;
   if (!c.k_exp != !c.v_exp) return set_error("cache: one of the exponent tables is missing"), false;
-  if (c.rows < 0 || c.per_row < 0 || (c.rows > 0 && c.per_row > 0 && !c.table) || c.table_stride < c.per_row)
+  if (c.rows < 0 || c.per_row < 0 || (c.rows > 0 && c.per_row > 0 && !c.table) || c.table_stride < 0 ||
+      (c.table_stride < c.per_row && c.table_stride != 0))
     return set_error("bad page table"), false;
   if (static_cast<int64_t>(c.per_row) * c.page_size > INT32_MAX || static_cast<int64_t>(kv_heads) * c.page_size > INT32_MAX)
     return set_error("cache: a row's table, or a page, of 2^31 tokens and more"), false;

@@ -617,7 +617,7 @@ def _cache_args(k_cache: Tensor, v_cache: Tensor, k_exp: Optional[Tensor], v_exp
     if status.dtype != torch.int32 or status.numel() != 1:
         raise RuntimeError("status must be one int32")
     return ((k_cache.data_ptr(), v_cache.data_ptr(), strides[0], k_at, v_at, exp_stride), (pages, size), (heads, dim),
-            (table.data_ptr(), step if step > per_row else per_row, rows, per_row))
+            (table.data_ptr(), step if rows > 1 else per_row, rows, per_row))
 
 
 def _rope(x: Tensor, positions: Tensor, inv_freq: Tensor, interleaved: bool = False, factor: float = 1.0) -> Tensor:

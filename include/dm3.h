@@ -386,7 +386,7 @@ int dm3_rope(const void* x, int T, int heads, int dim, int64_t ts, int64_t hs, c
  *   k_exp, v_exp      int8 [pages][kv_heads][page_size], pages exp_stride apart: a row stands for
  *                     code * 2^exp, exp = the smallest with amax <= 448 * 2^exp, in [-110, 119]
  *                     (16-byte aligned, exp_stride a multiple of 16)
- *   table             int32 [table_rows][per_row] page ids, rows table_stride apart: token t of row r lies
+ *   table             int32 [table_rows][per_row] page ids, rows table_stride apart (0: all rows share one): token t of row r lies
  *                     in page table[r][t / page_size]
  *   status            one device word; bit 4 is or-ed in when a page id, row, position or length outside
  *                     the cache or table was met (such tokens are skipped, never accessed), bit 1 when a bounded

@@ -1,11 +1,14 @@
 """dm3::paged_attention against the 64-bit oracle, alone and in a decode loop with the cache."""
 
 import math
+import subprocess
+import sys
 
 import pytest
 import torch
 
 from oracle import kv_oracle
+from tests.conftest import ROOT
 from tests.kv_helpers import check_attention, held, paged, to_cuda
 
 pytestmark = pytest.mark.gpu
@@ -64,6 +67,17 @@ def test_many_and_ragged_rows(dm3, rows, longest, empty, capacity, kv_heads, gro
     d = paged(_spread(rows, longest, empty, rows + dim), kv_heads, dim, 16, quant, rows, capacity=capacity)
     q = _q(rows, kv_heads * group, dim, rows)
     check_attention(*_run(dm3, d, q, None, window), d, q, None, window)
+
+
+@pytest.mark.parametrize("rows,longest", [(128, 900), (100, 900), (101, 200)])
+@pytest.mark.parametrize("quant", [False, True])
+def test_longest_rows_first(dm3, rows, longest, quant):
+    """More units than run at once, in a table of 1,000 tokens a row: rows of equal lengths, of none, and in any order."""
+    n = _spread(rows, longest, 0.1, rows)
+    n[3:40] = [n[3]] * 37
+    d = paged(n, 3, 64, 16, quant, rows, capacity=1000)
+    q = _q(rows, 6, 64, rows)
+    check_attention(*_run(dm3, d, q), d, q)
 
 
 def test_nothing_to_see(dm3):
@@ -287,6 +301,69 @@ def test_frames_together(dm3, quant):
                     assert abs(float(lse[r, h] - s.logsumexp(-1))) <= off + 1e-4
     assert cache.check() == 0
     assert torch.equal(cache.table[0, :5].cpu() >= 0, torch.ones(5, dtype=torch.bool))
+
+
+def test_one_table_for_all_rows(dm3):
+    """A table of one row expanded over all of them (stride 0): rows that read the same tokens."""
+    d = paged([90], 2, 64, 16, False, 3)
+    dev = to_cuda(d)
+    q = _q(3, 4, 64, 1)
+    n = torch.tensor([90, 40, 0])
+    out, lse = dm3.ops.paged_attention(q.cuda(), *held(dev), dev["table"].expand(3, -1), n.cuda(), dev["status"])
+    d["table"], d["lengths"] = d["table"].expand(3, -1).contiguous(), n
+    check_attention(out, lse, d, q)
+    k, _ = dm3.ops.kv_read(*held(dev), dev["table"].expand(3, -1), n.cuda(), 90, dev["status"])
+    assert torch.equal(k[1, :, :40], k[0, :, :40]) and int(dev["status"]) == 0
+
+
+@pytest.mark.parametrize("quant", [False, True])
+def test_nan_and_infinity_that_are_seen(dm3, quant):
+    """A NaN key makes its row NaN, a NaN value its column; an infinite value (bf16) its column infinite. Rows beside them
+    are as they were."""
+    d = paged([100, 100, 100, 100], 1, 64, 16, quant, 3)
+    q = _q(4, 4, 64, 1, 0.1)
+    at = lambda r, t: (int(d["table"][r, t // 16]), 0, t % 16)  # noqa: E731
+    if quant:
+        d["k"].view(torch.uint8)[at(1, 50)][5] = 0x7F
+        d["v"].view(torch.uint8)[at(2, 50)][5] = 0x7F
+    else:
+        d["k"][at(1, 50)][5] = math.nan
+        d["v"][at(2, 50)][5] = math.nan
+        d["v"][at(3, 50)][5] = math.inf
+    dev = to_cuda(d)
+    out, lse = dm3.ops.paged_attention(q.cuda(), *held(dev), dev["table"], dev["lengths"], dev["status"])
+    ref, rlse, _, _ = kv_oracle.attention(q, *held(d), d["table"], d["lengths"])
+    out, lse = out.double().cpu(), lse.double().cpu()
+    assert out[1].isnan().all() and lse[1].isnan().all()
+    assert torch.equal(out.isnan(), ref.isnan()) and torch.equal(out == math.inf, ref == math.inf)
+    ok = ref.isfinite()
+    assert (out - ref)[ok].abs().max() <= ref[ok].abs().max() * 2.0**-7
+    assert (lse - rlse)[rlse.isfinite()].abs().max() < 1e-4
+
+
+def test_captured_without_a_first_call(dm3):
+    """The first call of a process's kernels may be a captured one."""
+    code = """
+import torch, sys
+sys.path.insert(0, ".")
+import drama3_b200 as dm3
+c = dm3.KVCache(1, 2, 64, 1, 192, page_size=16, quantised=True)
+[c.reserve(r, 64) for r in range(2)]
+x = torch.randn(2, 1, 192, device="cuda").bfloat16()
+pos, rope = torch.tensor([0, 0], device="cuda"), dm3.Rope(64)
+torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    q = c.write(0, x, x, pos, None, x, rope)
+    out, lse = c.attend(0, q, pos + 1)
+    k, v = c.read(0, pos + 1, 4)
+g.replay()
+torch.cuda.synchronize()
+assert torch.equal(out, v[:, :, 0]) and c.check() == 0
+print("fine")
+"""
+    got = subprocess.run([sys.executable, "-c", code], cwd=ROOT, capture_output=True, text=True, timeout=120)
+    assert got.stdout.strip() == "fine", got.stderr[-2000:]
 
 
 def test_two_graphs_and_two_streams(dm3):
