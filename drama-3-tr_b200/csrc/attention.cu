@@ -15,7 +15,7 @@
 //                 comes from S^T's accumulators by an 8x8 transpose (movmatrix).
 // Every warp walks 16-token tiles of its own: TMA brings a step's keys and values, swizzled, into a ring of shared memory
 // that belongs to the warp, so warps never wait for one another until the join at the end. (Loads straight into
-// registers kept too little in flight, 82% of the copy bandwidth against 93% over 64 ragged rows of a bf16 cache;
+// registers kept too little in flight, 82% of the copy bandwidth where this has all of it, 64 ragged rows of a bf16 cache;
 // cp.async in their place doubled the traffic through L1 and was slower still. FP8 tensor instructions for the keys' product,
 // with the queries as two e4m3 parts, took a quarter longer than converting the keys to fp16.)
 //
@@ -251,6 +251,27 @@ __device__ __forceinline__ int64_t row_by_length(const Params& p, int nth, int* 
 __device__ __forceinline__ bool find_share(const Params& p, int units, int64_t* scratch, int64_t& row, int& unit, int64_t& begin,
                                            int64_t& left) {
   constexpr int kThreads = kWarps * 32;
+  if (p.c.rows <= 32) {  // every warp by itself, a lane a row
+    const int lane = threadIdx.x & 31;
+    const int64_t mine = lane < p.c.rows ? row_span(p, lane).tiles : 0;
+    int64_t upto = mine;
+#pragma unroll
+    for (int w = 1; w < 32; w *= 2) {
+      const int64_t x = __shfl_up_sync(0xffffffffu, upto, w);
+      if (lane >= w) upto += x;
+    }
+    const int64_t total = __shfl_sync(0xffffffffu, upto, 31);
+    if (blockIdx.x == 0 && threadIdx.x <= p.c.rows) p.row_at[threadIdx.x] = threadIdx.x < p.c.rows ? upto - mine : total;
+    const int64_t share = share_of(total, p.c.rows, units, gridDim.x), from = blockIdx.x * share;
+    if (from >= total * units) return false;
+    left = min(share, total * units - from);
+    const int hit = __ffs(__ballot_sync(0xffffffffu, mine > 0 && from < upto * units)) - 1;  // the first row that ends behind it
+    const int64_t tiles = __shfl_sync(0xffffffffu, mine, hit), in = from - (__shfl_sync(0xffffffffu, upto, hit) - tiles) * units;
+    row = hit;
+    unit = static_cast<int>(div(in, tiles));
+    begin = in - unit * tiles;
+    return true;
+  }
   int64_t *const s_sum = scratch, *const s_hit = scratch + kWarps;  // s_hit: the row found, its place, its tiles
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, rows = p.c.rows;
   int64_t total = 0, mine = 0, upto = 0;  // this thread's row of a block of 128: its tiles, and the sum up to it
@@ -298,6 +319,20 @@ __device__ __forceinline__ bool find_share(const Params& p, int units, int64_t* 
   return true;
 }
 
+// Stream, once a CTA's share is done: CTAs take the rows in turn to write what one without tokens gives, and to report
+// lengths behind the table.
+template <int kDim>
+__device__ __forceinline__ void tend_rows(const Params& p) {
+  for (int64_t row = blockIdx.x; row < p.c.rows; row += gridDim.x) {
+    const Span sp = row_span(p, row);
+    if (sp.cut && threadIdx.x == 0) kv::set_status(p.c.status, STATUS_BAD_PAGE);
+    if (sp.tiles) continue;
+    const int64_t at = row * p.q_heads;
+    for (int i = threadIdx.x; i < p.q_heads * kDim; i += blockDim.x) p.out[at * kDim + i] = __float2bfloat16_rn(0.f);
+    for (int i = threadIdx.x; i < p.q_heads; i += blockDim.x) p.lse[at + i] = -INFINITY;
+  }
+}
+
 template <int kDim, bool kQuant, int kNT, int kU>
 __global__ void __launch_bounds__(kWarps * 32, 2)
     attend_kernel(const __grid_constant__ Params p, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap) {
@@ -325,7 +360,6 @@ __global__ void __launch_bounds__(kWarps * 32, 2)
 
   griddep_launch();
   griddep_wait();
-  fence_proxy_async();  // the cache's rows may have been written just before; the copies read them
   const int units = p.kv_heads * p.head_tiles;  // of a row
   // The segment at hand: tiles [begin, end) of a row and unit, counted from the row's first tile seen.
   int64_t row, begin, end;
@@ -341,16 +375,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2)
     end = min(begin + chunk, sp.tiles);
     if (sp.cut && threadIdx.x == 0) kv::set_status(p.c.status, STATUS_BAD_PAGE);
   } else {
-    // CTAs take the rows in turn to write what one without tokens gives, and to report lengths behind the table
-    for (row = blockIdx.x; row < p.c.rows; row += gridDim.x) {
-      sp = row_span(p, row);
-      if (sp.cut && threadIdx.x == 0) kv::set_status(p.c.status, STATUS_BAD_PAGE);
-      if (sp.tiles) continue;
-      const int64_t at = row * p.q_heads;
-      for (int i = threadIdx.x; i < p.q_heads * kDim; i += blockDim.x) p.out[at * kDim + i] = __float2bfloat16_rn(0.f);
-      for (int i = threadIdx.x; i < p.q_heads; i += blockDim.x) p.lse[at + i] = -INFINITY;
-    }
-    if (!find_share(p, units, reinterpret_cast<int64_t*>(s_m), row, unit, begin, left)) return;
+    if (!find_share(p, units, reinterpret_cast<int64_t*>(s_m), row, unit, begin, left)) return tend_rows<kDim>(p);
     sp = row_span(p, row);
     end = min(begin + left, sp.tiles);
   }
@@ -831,12 +856,12 @@ __global__ void __launch_bounds__(kWarps * 32, 2)
       return;
     }
     left -= end - begin;
-    if (left <= 0) return;
+    if (left <= 0) return tend_rows<kDim>(p);
     ++part;
     row = next_row, unit = next_unit, sp = next_sp;
     begin = 0, end = min(left, sp.tiles);
     tc::fence_proxy_async_smem();  // the join's reads and writes of the ring come before the next copies into it
-    if (__syncthreads_or(lost)) return;
+    if (__syncthreads_or(lost)) return tend_rows<kDim>(p);
   }
 }
 
