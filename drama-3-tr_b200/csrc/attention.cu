@@ -30,8 +30,8 @@
 // An e4m3 row is code * 2^e. For keys 2^e joins the logit's scale. For values it joins the weight's exponent:
 // w_t = 2^(s_t + e_t - M) with M the running maximum of s_t + e_t, so weights are in fp16's range whatever the rows'
 // sizes, and l sums w_t * 2^-e_t. Codes are exact in fp16; queries are scaled by a power of two to
-// [2^14, 2^15), where fp16 holds a bf16 row to 2^-40 of its largest value; a weight is rounded once to 11 bits (2^-12 of
-// it at most, 1/16 of what rounding the output to bf16 costs). With a bf16 cache a weight goes to the tensor cores
+// [2^14, 2^15), where fp16 holds a bf16 row to 2^-40 of its largest value; a weight is rounded once to 11 bits (2^-11 of
+// it at most, 1/8 of what rounding the output to bf16 costs). With a bf16 cache a weight goes to the tensor cores
 // as a bf16 pair, high and low part: 16 bits.
 #include <atomic>
 #include <cmath>

@@ -528,6 +528,9 @@ def _(logits, lse, token, eos_id, semantic_begin, score):
 # mutated arguments). So `rope`, `kv_write`, `kv_read` and `paged_attention` call their kernels directly where nothing
 # has to see the call as an operator, and go through torch.ops.dm3.* under tracing, for tensor subclasses (fake
 # tensors among them) and where autograd would have to be told that there is no gradient.
+_INT_MAX = 2**31 - 1  # the C entries take counts as int
+
+
 def _plain(*ts: Optional[Tensor]) -> bool:
     if torch.compiler.is_compiling():
         return False
@@ -573,8 +576,8 @@ def _heads(t: Tensor, name: str) -> Tensor:
 
 
 def _int64(t: Tensor, n: int, name: str) -> Tensor:
-    if t.dtype != torch.int64 or t.shape != (n,):
-        raise RuntimeError(f"{name} must be int64 [{n}]")
+    if t.dtype != torch.int64 or t.shape != (n,) or n > _INT_MAX:
+        raise RuntimeError(f"{name} must be int64 [{n}], at most {_INT_MAX} of them")
     return t.contiguous()
 
 
@@ -612,6 +615,8 @@ def _cache_args(k_cache: Tensor, v_cache: Tensor, k_exp: Optional[Tensor], v_exp
         raise RuntimeError("the page table must be int32 [rows, pages a row] with unit column stride")
     rows, per_row = table.shape
     step, col = table.stride()
+    if max(pages, rows, per_row) > _INT_MAX:
+        raise RuntimeError(f"pages and the page table's sides must be at most {_INT_MAX}")
     if per_row > 1 and col != 1:
         raise RuntimeError("the page table must be int32 [rows, pages a row] with unit column stride")
     if status.dtype != torch.int32 or status.numel() != 1:
@@ -627,6 +632,8 @@ def _rope(x: Tensor, positions: Tensor, inv_freq: Tensor, interleaved: bool = Fa
     if x.stride(2) != 1:
         x = x.contiguous()
     T, heads, dim = x.shape
+    if heads * dim > 1 << 24:
+        raise RuntimeError("rope: bad head count or head size")
     positions, inv_freq = _int64(positions, T, "positions"), _angles(inv_freq)
     y = torch.empty((T, heads, dim), dtype=BF16, device=x.device)
     _launch(dev, "dm3_rope", x.data_ptr(), T, heads, dim, x.stride(0), x.stride(1), positions.data_ptr(),

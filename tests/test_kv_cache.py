@@ -114,6 +114,25 @@ def test_ops_refuse_cpu_tensors(dm3):
         c.write(0, torch.zeros(1, 1, 64, dtype=BF), torch.zeros(1, 1, 64, dtype=BF), n)
 
 
+def test_ops_refuse_counts_beyond_32_bits(dm3, monkeypatch):
+    """Counts that a C int would cut short; the tensors are expanded views of one element or row."""
+    ops, many = dm3.ops, 2**32 + 1
+    monkeypatch.setattr(ops, "_same_device", lambda *a: 0)
+    monkeypatch.setattr(ops, "_launch", lambda *a: pytest.fail("launched"))
+    inv, zero = torch.ones(32, dtype=torch.float64), torch.zeros(1, dtype=torch.int64)
+    k, c = torch.zeros(1, 1, 64, dtype=BF), torch.zeros(1, 1, 16, 64, dtype=BF)
+    t, s = torch.zeros(1, 1, dtype=torch.int32), torch.zeros(1, dtype=torch.int32)
+    for bad in (
+        lambda: ops.rope(k.expand(many, 1, 64), zero.expand(many), inv),
+        lambda: ops.rope(k.expand(1, many, 64), zero, inv),
+        lambda: ops.kv_write(k.expand(many, 1, 64), k.expand(many, 1, 64), zero.expand(many), t, c, c, None, None, s),
+        lambda: ops.kv_read(c, c, None, None, t.expand(many, 1), zero.expand(many), 0, s),
+        lambda: ops.paged_attention(k, c.expand(many, 1, 16, 64), c.expand(many, 1, 16, 64), None, None, t, zero, s),
+    ):
+        with pytest.raises(RuntimeError, match="at most|bad head"):
+            bad()
+
+
 # What each C entry is called with, by name; a refusal test changes one of them.
 _CACHE = dict(k_cache=P, v_cache=P, page_stride=2 * 16 * 64, k_exp=None, v_exp=None, exp_stride=0, pages=5, page_size=16)
 _TABLE = dict(table=P, table_stride=4, table_rows=3, per_row=4)
