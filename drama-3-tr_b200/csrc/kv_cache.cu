@@ -110,28 +110,56 @@ __device__ __forceinline__ Where where(int i, int rot) {
   return turned && !kInter ? Where{i, i + rot / 16, true} : Where{2 * i, 2 * i + 1, turned};
 }
 
-// The angles of a CTA's tokens: pair 8i + 2k + e of token t at [t][k][i][e], so neighbouring threads read
-// neighbouring 16 bytes.
+// The angles of a CTA's tokens: cosines and sines of pairs 8i + 2k, 8i + 2k + 1 of token t as (c, c, s, s) at [t][k][i],
+// so neighbouring threads read neighbouring 16 bytes.
 template <bool kLow>
 __device__ __forceinline__ void fill_angles(float2* high, float2* low, int tokens, const int64_t* positions,
                                             const double* inv_freq, int rot, double factor) {
   const int half = rot / 2, units = rot / 16;
   for (int x = threadIdx.x; x < tokens * half; x += blockDim.x) {
-    const int t = x / half, f = x - t * half, at = t * half + (((f & 7) >> 1) * units + (f >> 3)) * 2 + (f & 1);
+    const int t = x / half, f = x - t * half, at = t * rot + (((f & 7) >> 1) * units + (f >> 3)) * 4 + (f & 1);
     float2 h, l;
     angle<kLow>(positions[t], inv_freq[f], factor, h, l);
-    high[at] = h;
-    if (kLow) low[at] = l;
+    reinterpret_cast<float*>(high)[at] = h.x, reinterpret_cast<float*>(high)[at + 2] = h.y;
+    if (kLow) reinterpret_cast<float*>(low)[at] = l.x, reinterpret_cast<float*>(low)[at + 2] = l.y;
   }
 }
 
-// a cos - b sin to about 2^-46 of |a| + |b|: products and the sum with their rounding errors carried along
-__device__ __forceinline__ float exact_turn(float a, float b, float ch, float cl, float sh, float sl) {
-  const float p = __fmul_rn(a, ch), q = __fmul_rn(-b, sh);  // _rn: not to be contracted
-  const float pe = fmaf(a, ch, -p), qe = fmaf(-b, sh, -q);
-  const float d = __fadd_rn(p, q), z = __fsub_rn(d, p);
-  const float de = __fadd_rn(__fsub_rn(p, __fsub_rn(d, z)), __fsub_rn(q, z));
-  return __fadd_rn(d, __fadd_rn(__fadd_rn(de, __fadd_rn(pe, qe)), fmaf(a, cl, -b * sl)));
+// Two 32-bit values an instruction, each rounded as its scalar form.
+struct Two {
+  uint64_t v;
+};
+__device__ __forceinline__ Two two(float a, float b) {
+  return {static_cast<uint64_t>(__float_as_uint(a)) | static_cast<uint64_t>(__float_as_uint(b)) << 32};
+}
+__device__ __forceinline__ float first(Two a) { return __uint_as_float(static_cast<uint32_t>(a.v)); }
+__device__ __forceinline__ float second(Two a) { return __uint_as_float(static_cast<uint32_t>(a.v >> 32)); }
+__device__ __forceinline__ Two operator-(Two a) { return two(-first(a), -second(a)); }
+__device__ __forceinline__ Two mul(Two a, Two b) {
+  Two r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ Two add(Two a, Two b) {
+  Two r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ Two fma(Two a, Two b, Two c) {
+  Two r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return r;
+}
+__device__ __forceinline__ Two sub(Two a, Two b) { return fma(b, two(-1.f, -1.f), a); }
+
+// a c + b s to about 2^-46 of |a| + |b|: products and the sum with their rounding errors carried along. nc, ns: -c, -s;
+// cl, sl: the low parts of c and s.
+__device__ __forceinline__ Two exact_turn(Two a, Two b, Two c, Two nc, Two cl, Two s, Two ns, Two sl) {
+  const Two p = mul(a, c), q = mul(b, s);
+  const Two error = add(fma(a, nc, p), fma(b, ns, q));  // of both products, negated
+  const Two d = add(p, q), z = sub(d, p);
+  const Two de = add(sub(p, sub(d, z)), sub(q, z));
+  return add(d, add(sub(de, error), fma(a, cl, mul(b, sl))));
 }
 
 // Turns the 16 values of unit i in place. angles: of the token.
@@ -141,24 +169,23 @@ __device__ __forceinline__ void turn(Chunk& x, Chunk& y, int i, const float2* hi
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
     const float4 h = *reinterpret_cast<const float4*>(high + (k * units + i) * 2);
-    float4 l = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (kExact) l = *reinterpret_cast<const float4*>(low + (k * units + i) * 2);
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      const float ch = e ? h.z : h.x, sh = e ? h.w : h.y, cl = e ? l.z : l.x, sl = e ? l.w : l.y;
-      auto pair = [&](float& a, float& b) {
-        const float a0 = a, b0 = b;
-        a = kExact ? exact_turn(a0, b0, ch, cl, sh, sl) : a0 * ch - b0 * sh;
-        b = kExact ? exact_turn(b0, -a0, ch, cl, sh, sl) : b0 * ch + a0 * sh;
-      };
-      const int j = 2 * k + e;
-      if (!kInter)
-        pair(x.v[j], y.v[j]);
-      else if (k < 2)
-        pair(x.v[2 * j], x.v[2 * j + 1]);
-      else
-        pair(y.v[2 * j - 8], y.v[2 * j - 7]);
+    const Two c = two(h.x, h.y), s = two(h.z, h.w), ns = -s;
+    Chunk& z = k < 2 ? x : y;
+    const int j = kInter ? 4 * (k % 2) : 2 * k;
+    float &a0 = kInter ? z.v[j] : x.v[j], &b0 = kInter ? z.v[j + 1] : y.v[j];
+    float &a1 = kInter ? z.v[j + 2] : x.v[j + 1], &b1 = kInter ? z.v[j + 3] : y.v[j + 1];
+    const Two a = two(a0, a1), b = two(b0, b1);
+    Two ra, rb;
+    if (kExact) {
+      const float4 l = *reinterpret_cast<const float4*>(low + (k * units + i) * 2);
+      const Two cl = two(l.x, l.y), sl = two(l.z, l.w), nc = -c;
+      ra = exact_turn(a, b, c, nc, cl, ns, s, -sl);
+      rb = exact_turn(b, a, c, nc, cl, s, ns, sl);
+    } else {
+      ra = fma(a, c, mul(b, ns));
+      rb = fma(b, c, mul(a, s));
     }
+    a0 = first(ra), a1 = second(ra), b0 = first(rb), b1 = second(rb);
   }
 }
 
@@ -275,11 +302,18 @@ __device__ __forceinline__ int row_exponent(float amax) {
   return min(max(e, -110), 119);
 }
 
-// As rope_kernel, over the rows of q, k and v, two rows a thread at a time. A row belongs to kSeg neighbouring lanes, so the amax of a quantised
-// row is a few shuffles. A quantised key is turned to 2^-46: it is the code of the exactly turned key, whichever call
-// wrote it (in 32 bits about one value in 10^6 would fall on the other side of a code's border).
-template <int kSeg, bool kQuant, bool kInter>
-__global__ void __launch_bounds__(kThreads, 4) write_kernel(const __grid_constant__ WriteParams p, const Div rows_of) {
+// As rope_kernel, over the rows of q, then those of k, then those of v; each of the three starts with a warp, so a warp
+// is at one of them at a time. A row belongs to kSeg neighbouring lanes, so the amax of a quantised row is a few
+// shuffles. A quantised key is turned to 2^-46: it is the code of the exactly turned key, whichever call wrote it (in
+// 32 bits about one value in 10^6 would fall on the other side of a code's border).
+//
+// Loads in flight: the next row's while a thread is at one, in four CTAs an SM; or (kMany) two rows' at a time in five.
+// With a bf16 cache the second is faster for many tokens and slower for few (about 100,000 tokens with 32 + 4 + 4 heads of
+// 64: 216 against 235 us; 256 tokens with 16 + 2 + 2 of 256: 3.7 against 3.0). An e4m3 cache is bound by its
+// instructions, and the first is faster (31,733 tokens with 32 + 8 + 8 of 128: 140 us, 152 with two rows at a time).
+template <int kSeg, bool kQuant, bool kInter, bool kMany>
+__global__ void __launch_bounds__(kThreads, kMany ? 5 : 4) write_kernel(const __grid_constant__ WriteParams p, const Div by_q,
+                                                                       const Div by_k) {
   __shared__ __align__(16) float2 high[kAngles], low[kQuant ? kAngles : 1];
   __shared__ int64_t s_at[kBlockTokens], s_exp[kBlockTokens];  // place of a token's row of head 0; -1: not cached
   __shared__ bool s_pad[kBlockTokens];
@@ -287,37 +321,48 @@ __global__ void __launch_bounds__(kThreads, 4) write_kernel(const __grid_constan
   griddep_wait();
   const int64_t t0 = static_cast<int64_t>(blockIdx.x) * p.block;
   const int tokens = p.T - t0 < p.block ? static_cast<int>(p.T - t0) : p.block;
-  constexpr int kSegs = kThreads / kSeg, kBatch = 2;
-  const int i = threadIdx.x % kSeg, n = p.q.n + 2 * p.k.n, total = tokens * n;
+  constexpr int kSegs = kThreads / kSeg, kWarp = 32 / kSeg;
+  const int i = threadIdx.x % kSeg;
+  const int q_rows = (tokens * p.q.n + kWarp - 1) & -kWarp, k_rows = (tokens * p.k.n + kWarp - 1) & -kWarp;
+  const int total = q_rows + 2 * k_rows;
   const Where w = where<kInter>(i, p.rot);
   const bool mine = i < p.dim / 16;
-  uint4 ra[kBatch], rb[kBatch];
-  int t[kBatch], head[kBatch], side[kBatch];  // side 0: query, 1: key, 2: value, -1: none
-  auto load = [&](int base) {
-#pragma unroll
-    for (int b = 0; b < kBatch; ++b) {
-      const int r = base + b * kSegs + threadIdx.x / kSeg;
-      side[b] = -1;
-      ra[b] = rb[b] = make_uint4(0, 0, 0, 0);
-      if (r < total && mine) {
-        t[b] = rows_of(r);
-        int h = r - t[b] * n;
-        side[b] = 0;
-        if (h >= p.q.n) h -= p.q.n, side[b] = 1;
-        if (side[b] == 1 && h >= p.k.n) h -= p.k.n, side[b] = 2;
-        head[b] = h;
-        const Heads& in = side[b] == 0 ? p.q : side[b] == 1 ? p.k : p.v;
-        const __nv_bfloat16* row = in.p + (t0 + t[b]) * in.ts + h * in.hs;
-        ra[b] = __ldcs(reinterpret_cast<const uint4*>(row + w.a * 8));
-        rb[b] = __ldcs(reinterpret_cast<const uint4*>(row + w.b * 8));
-      }
+  struct Row {
+    uint4 a, b;
+    int side, t, head;  // side 0: query, 1: key, 2: value; head -1: no row
+  };
+  auto load = [&](Row& x, int base) {
+    int r = base + threadIdx.x / kSeg;
+    x.side = r < q_rows ? 0 : r < q_rows + k_rows ? 1 : 2;
+    x.head = -1;
+    x.a = x.b = make_uint4(0, 0, 0, 0);
+    auto from = [&](const Heads& in, const Div& by) {
+      x.t = by(r);
+      if (x.t >= tokens || !mine) return;
+      x.head = r - x.t * in.n;
+      const __nv_bfloat16* row = in.p + t0 * in.ts + static_cast<uint32_t>(x.t) * in.ts + static_cast<uint32_t>(x.head) * in.hs;
+      x.a = __ldcs(reinterpret_cast<const uint4*>(row + w.a * 8));
+      x.b = __ldcs(reinterpret_cast<const uint4*>(row + w.b * 8));
+    };
+    if (x.side == 0) {
+      from(p.q, by_q);
+    } else if (x.side == 1) {
+      r -= q_rows;
+      from(p.k, by_k);
+    } else {
+      r -= q_rows + k_rows;
+      from(p.v, by_k);
     }
   };
-  load(blockIdx.y * kSegs * kBatch);  // on its way while the angles and places are found
+  constexpr int kBatch = kMany ? 2 : 1;
+  Row now[kBatch];
+#pragma unroll
+  for (int b = 0; b < kBatch; ++b) load(now[b], (blockIdx.y * kBatch + b) * kSegs);  // while angles and places are found
   // a place is found by the last threads, while the first ones are at the angles
+  bool padding = false;
   if (const int t = kThreads - 1 - threadIdx.x; t < tokens) {
     const int64_t pos = p.positions[t0 + t], r = p.rows ? p.rows[t0 + t] : t0 + t;
-    const bool padding = pos < 0 || r < 0;
+    padding = pos < 0 || r < 0;
     int64_t at = -1, x = 0;
     if (!padding) {
       const int64_t nth = pos / p.c.page_size, in = pos - nth * p.c.page_size;
@@ -330,63 +375,78 @@ __global__ void __launch_bounds__(kThreads, 4) write_kernel(const __grid_constan
     s_at[t] = at, s_exp[t] = x, s_pad[t] = padding;
   }
   if (p.rot) fill_angles<kQuant>(high, low, tokens, p.positions + t0, p.inv_freq, p.rot, p.factor);
-  __syncthreads();
-  // all lanes of a warp make the same number of rounds: the shuffles need them
-  for (int base = blockIdx.y * kSegs * kBatch; base < total;) {
-#pragma unroll
-    for (int b = 0; b < kBatch; ++b) {
-      Chunk x = unpack(ra[b]), y = unpack(rb[b]);
-      if (w.turned && (side[b] == 0 || side[b] == 1)) {
-        const int at = t[b] * (p.rot / 2);
-        if (kQuant && side[b] == 1)
-          turn<kQuant, kInter>(x, y, i, high + at, low + at, p.rot);
-        else
-          turn<false, kInter>(x, y, i, high + at, nullptr, p.rot);
-      }
-      const uint4 px = pack(x), py = pack(y);
-      if (side[b] == 0) {
-        __nv_bfloat16* dst = p.y + ((t0 + t[b]) * p.q.n + head[b]) * p.dim;
-        const uint4 zero = make_uint4(0, 0, 0, 0);
-        *reinterpret_cast<uint4*>(dst + w.a * 8) = s_pad[t[b]] ? zero : px;
-        *reinterpret_cast<uint4*>(dst + w.b * 8) = s_pad[t[b]] ? zero : py;
-      }
-      const int64_t place = side[b] > 0 ? s_at[t[b]] : -1;
-      if (!kQuant) {
-        if (place >= 0) {
-          __nv_bfloat16* dst = static_cast<__nv_bfloat16*>(side[b] == 1 ? p.c.k : p.c.v) + place +
-                               static_cast<int64_t>(head[b]) * p.c.page_size * p.dim;
-          *reinterpret_cast<uint4*>(dst + w.a * 8) = px;
-          *reinterpret_cast<uint4*>(dst + w.b * 8) = py;
-        }
-        continue;
-      }
-      if (!__any_sync(0xffffffffu, side[b] > 0)) continue;
-      uint32_t top = max_magnitude(px, py);
-#pragma unroll
-      for (int o = kSeg / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-      x = unpack(px), y = unpack(py);  // the key as a bf16 cache would hold it
-      if (__any_sync(0xffffffffu, top >= 0x7f80u)) {  // infinities and NaN: not counted, and NaN in the cache
-        float amax = 0.f;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          amax = fmaxf(amax, fmaxf(isfinite(x.v[j]) ? fabsf(x.v[j]) : 0.f, isfinite(y.v[j]) ? fabsf(y.v[j]) : 0.f));
-          if (!isfinite(x.v[j])) x.v[j] = NAN;
-          if (!isfinite(y.v[j])) y.v[j] = NAN;
-        }
-#pragma unroll
-        for (int o = kSeg / 2; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-        top = __float_as_uint(amax) >> 16;
-      }
-      if (place >= 0) {
-        const int e = row_exponent(__uint_as_float(top << 16));
-        uint8_t* dst = static_cast<uint8_t*>(side[b] == 1 ? p.c.k : p.c.v) + place + static_cast<int64_t>(head[b]) * p.c.page_size * p.dim;
-        *reinterpret_cast<uint2*>(dst + w.a * 8) = encode(x, exp2i(-e));
-        *reinterpret_cast<uint2*>(dst + w.b * 8) = encode(y, exp2i(-e));
-        if (i == 0) (side[b] == 1 ? p.c.k_exp : p.c.v_exp)[s_exp[t[b]] + static_cast<int64_t>(head[b]) * p.c.page_size] = static_cast<int8_t>(e);
-      }
+  const bool padded = __syncthreads_or(padding);
+  __nv_bfloat16* const queries = p.y + t0 * p.q.n * p.dim;
+  // a row in the cache, once its values are final
+  auto keep = [&](const Row& x, void* cache, int8_t* exps) {
+    const int64_t place = x.head < 0 ? -1 : s_at[x.t];
+    if (!kQuant) {
+      if (place < 0) return;
+      __nv_bfloat16* dst = static_cast<__nv_bfloat16*>(cache) + place + static_cast<int64_t>(x.head * p.c.page_size) * p.dim;
+      *reinterpret_cast<uint4*>(dst + w.a * 8) = x.a;
+      *reinterpret_cast<uint4*>(dst + w.b * 8) = x.b;
+      return;
     }
-    base += gridDim.y * kSegs * kBatch;
-    if (base < total) load(base);
+    uint32_t top = max_magnitude(x.a, x.b);
+#pragma unroll
+    for (int o = kSeg / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+    Chunk a = unpack(x.a), b = unpack(x.b);  // a key as a bf16 cache would hold it
+    if (__any_sync(0xffffffffu, top >= 0x7f80u)) {  // infinities and NaN: not counted, and NaN in the cache
+      float amax = 0.f;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        amax = fmaxf(amax, fmaxf(isfinite(a.v[j]) ? fabsf(a.v[j]) : 0.f, isfinite(b.v[j]) ? fabsf(b.v[j]) : 0.f));
+        if (!isfinite(a.v[j])) a.v[j] = NAN;
+        if (!isfinite(b.v[j])) b.v[j] = NAN;
+      }
+#pragma unroll
+      for (int o = kSeg / 2; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+      top = __float_as_uint(amax) >> 16;
+    }
+    if (place < 0) return;
+    const int e = row_exponent(__uint_as_float(top << 16)), row = x.head * p.c.page_size;
+    uint8_t* dst = static_cast<uint8_t*>(cache) + place + static_cast<int64_t>(row) * p.dim;
+    *reinterpret_cast<uint2*>(dst + w.a * 8) = encode(a, exp2i(-e));
+    *reinterpret_cast<uint2*>(dst + w.b * 8) = encode(b, exp2i(-e));
+    if (i == 0) exps[s_exp[x.t] + row] = static_cast<int8_t>(e);
+  };
+  auto finish = [&](Row& x) {
+    if (x.side < 2 && w.turned && x.head >= 0) {
+      Chunk a = unpack(x.a), b = unpack(x.b);
+      const int at = x.t * (p.rot / 2);
+      if (kQuant && x.side == 1)
+        turn<kQuant, kInter>(a, b, i, high + at, low + at, p.rot);
+      else
+        turn<false, kInter>(a, b, i, high + at, nullptr, p.rot);
+      x.a = pack(a), x.b = pack(b);
+    }
+    if (x.side == 0) {
+      if (x.head < 0) return;
+      if (padded && s_pad[x.t]) x.a = x.b = make_uint4(0, 0, 0, 0);
+      __nv_bfloat16* dst = queries + (x.t * p.q.n + x.head) * p.dim;
+      *reinterpret_cast<uint4*>(dst + w.a * 8) = x.a;
+      *reinterpret_cast<uint4*>(dst + w.b * 8) = x.b;
+    } else if (x.side == 1) {
+      keep(x, p.c.k, p.c.k_exp);
+    } else {
+      keep(x, p.c.v, p.c.v_exp);
+    }
+  };
+  for (int base = blockIdx.y * kBatch * kSegs; base < total;) {
+    base += gridDim.y * kBatch * kSegs;
+    if constexpr (kMany) {
+#pragma unroll
+      for (int b = 0; b < kBatch; ++b) finish(now[b]);
+      if (base < total) {
+#pragma unroll
+        for (int b = 0; b < kBatch; ++b) load(now[b], base + b * kSegs);
+      }
+    } else {
+      Row next;
+      load(next, base);
+      finish(now[0]);
+      now[0] = next;
+    }
   }
 }
 
@@ -589,16 +649,21 @@ extern "C" int dm3_kv_write(const void* q, int q_heads, int64_t q_ts, int64_t q_
   p.y = static_cast<__nv_bfloat16*>(q_out);
   p.T = T, p.dim = dim, p.rows = rows, p.positions = positions;
   p.inv_freq = inv_freq, p.rot = rot, p.factor = factor;
-  const int seg = dim == 64 ? 4 : dim == 128 ? 8 : 16, round = 2 * kThreads / seg, n = q_heads + 2 * kv_heads;
+  const int seg = dim == 64 ? 4 : dim == 128 ? 8 : 16, n = q_heads + 2 * kv_heads;
   if (n > 65535 / kBlockTokens) return set_error("kv_write: too many heads"), DM3_EINVAL;
-  const Blocks b = blocks(T, rot, (n + round - 1) / round, 4);
+  int dev = 0;
+  cudaGetDevice(&dev);
+  const bool many = !k_exp && T > 5 * kBlockTokens * sm_count(dev);  // more than one wave of full blocks
+  const int round = (many ? 2 : 1) * kThreads / seg;
+  const Blocks b = blocks(T, rot, (n + round - 1) / round, many ? 5 : 4);
   p.block = b.tokens;
   const dim3 grid((T + b.tokens - 1) / b.tokens, b.shares);
-  auto go = [&](auto kernel) { return launch(kernel, grid, kThreads, stream, "kv_write", p, Div(n)); };
+  auto go = [&](auto kernel) { return launch(kernel, grid, kThreads, stream, "kv_write", p, Div(q_heads), Div(kv_heads)); };
   auto pick = [&](auto lanes) {
     constexpr int kSeg = decltype(lanes)::value;
-    if (k_exp) return interleaved ? go(write_kernel<kSeg, true, true>) : go(write_kernel<kSeg, true, false>);
-    return interleaved ? go(write_kernel<kSeg, false, true>) : go(write_kernel<kSeg, false, false>);
+    if (k_exp) return interleaved ? go(write_kernel<kSeg, true, true, false>) : go(write_kernel<kSeg, true, false, false>);
+    if (many) return interleaved ? go(write_kernel<kSeg, false, true, true>) : go(write_kernel<kSeg, false, false, true>);
+    return interleaved ? go(write_kernel<kSeg, false, true, false>) : go(write_kernel<kSeg, false, false, false>);
   };
   return seg == 4   ? pick(std::integral_constant<int, 4>{})
          : seg == 8 ? pick(std::integral_constant<int, 8>{})

@@ -151,6 +151,35 @@ def test_many_tokens(dm3, tokens, quant):
     assert (rk[0] == 0).all() and (rk[2] == 0).all() and c.check() == 0
 
 
+@pytest.mark.parametrize("dim,kv_heads,q_heads,rot", [(64, 1, 3, 64), (128, 2, 5, 96), (192, 1, 2, 48), (256, 1, 0, 256)])
+@pytest.mark.parametrize("quant", [False, True])
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_one_call_and_many(dm3, dim, kv_heads, q_heads, rot, quant, interleaved):
+    """Tokens of one long call, padding among them, get the bits that they get in short calls."""
+    tokens, step = 6113, 1201
+    g = torch.Generator().manual_seed(dim)
+    rows, pos = torch.randint(0, 2, (tokens,), generator=g), torch.randperm(tokens, generator=g)
+    rows[torch.randperm(tokens, generator=g)[:57]] = -1
+    x = torch.randn(tokens, q_heads + 2 * kv_heads, dim, generator=g).to(BF).cuda()
+    q, k, v = x.split([q_heads, kv_heads, kv_heads], 1)
+    rope, rows, pos = dm3.Rope(rot, 1e4, interleaved), rows.cuda(), pos.cuda()
+    one, many = (dm3.KVCache(1, 2, tokens, kv_heads, dim, quantised=quant) for _ in range(2))
+    for c in (one, many):
+        c.reserve(0, tokens), c.reserve(1, tokens)
+    full = torch.full((2,), tokens).cuda()
+    out = one.write(0, k, v, pos, rows, q if q_heads else None, rope)
+    parts = [many.write(0, k[a:a + step], v[a:a + step], pos[a:a + step], rows[a:a + step], q[a:a + step] if q_heads else None, rope)
+             for a in range(0, tokens, step)]
+    assert torch.equal(out, torch.cat(parts)) and one.check() == 0 and many.check() == 0
+    seen = torch.zeros(2, tokens, dtype=torch.bool, device="cuda")
+    seen[rows[rows >= 0], pos[rows >= 0]] = True
+    for a, b in zip(one.read(0, full, tokens), many.read(0, full, tokens)):
+        a, b = a.transpose(1, 2)[seen], b.transpose(1, 2)[seen]
+        assert a.isfinite().all() and torch.equal(a, b)
+    if q_heads:
+        assert (out[rows < 0] == 0).all()
+
+
 def test_traced_calls_are_the_same(dm3):
     """Under torch.compile the ops are traced as operators, with the same results and the same writes."""
     g = torch.Generator().manual_seed(3)
