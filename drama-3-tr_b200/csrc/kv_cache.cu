@@ -162,30 +162,32 @@ __device__ __forceinline__ Two exact_turn(Two a, Two b, Two c, Two nc, Two cl, T
   return add(d, add(sub(de, error), fma(a, cl, mul(b, sl))));
 }
 
-// Turns the 16 values of unit i in place. angles: of the token.
+// Turns the 16 values of unit i in place. high, low: the token's angles. The exact turn takes two values an instruction;
+// the plain one, a few instructions, is slower so (rope of 2,643 tokens with 22 heads: 10.7 against 9.8 us).
 template <bool kExact, bool kInter>
 __device__ __forceinline__ void turn(Chunk& x, Chunk& y, int i, const float2* high, const float2* low, int rot) {
   const int units = rot / 16;
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
     const float4 h = *reinterpret_cast<const float4*>(high + (k * units + i) * 2);
-    const Two c = two(h.x, h.y), s = two(h.z, h.w), ns = -s;
     Chunk& z = k < 2 ? x : y;
     const int j = kInter ? 4 * (k % 2) : 2 * k;
     float &a0 = kInter ? z.v[j] : x.v[j], &b0 = kInter ? z.v[j + 1] : y.v[j];
     float &a1 = kInter ? z.v[j + 2] : x.v[j + 1], &b1 = kInter ? z.v[j + 3] : y.v[j + 1];
-    const Two a = two(a0, a1), b = two(b0, b1);
-    Two ra, rb;
     if (kExact) {
       const float4 l = *reinterpret_cast<const float4*>(low + (k * units + i) * 2);
-      const Two cl = two(l.x, l.y), sl = two(l.z, l.w), nc = -c;
-      ra = exact_turn(a, b, c, nc, cl, ns, s, -sl);
-      rb = exact_turn(b, a, c, nc, cl, s, ns, sl);
+      const Two a = two(a0, a1), b = two(b0, b1), c = two(h.x, h.y), s = two(h.z, h.w), cl = two(l.x, l.y), sl = two(l.z, l.w);
+      const Two ra = exact_turn(a, b, c, -c, cl, -s, s, -sl), rb = exact_turn(b, a, c, -c, cl, s, -s, sl);
+      a0 = first(ra), a1 = second(ra), b0 = first(rb), b1 = second(rb);
     } else {
-      ra = fma(a, c, mul(b, ns));
-      rb = fma(b, c, mul(a, s));
+      auto plain = [](float& a, float& b, float c, float s) {
+        const float a0 = a;
+        a = a0 * c - b * s;
+        b = b * c + a0 * s;
+      };
+      plain(a0, b0, h.x, h.z);
+      plain(a1, b1, h.y, h.w);
     }
-    a0 = first(ra), a1 = second(ra), b0 = first(rb), b1 = second(rb);
   }
 }
 
@@ -308,9 +310,10 @@ __device__ __forceinline__ int row_exponent(float amax) {
 // 32 bits about one value in 10^6 would fall on the other side of a code's border).
 //
 // Loads in flight: the next row's while a thread is at one, in four CTAs an SM; or (kMany) two rows' at a time in five.
-// With a bf16 cache the second is faster for many tokens and slower for few (about 100,000 tokens with 32 + 4 + 4 heads of
-// 64: 216 against 235 us; 256 tokens with 16 + 2 + 2 of 256: 3.7 against 3.0). An e4m3 cache is bound by its
-// instructions, and the first is faster (31,733 tokens with 32 + 8 + 8 of 128: 140 us, 152 with two rows at a time).
+// With a bf16 cache the second is faster for many tokens and slower for few (written and read back: 100,000 tokens with
+// 32 + 4 + 4 heads of 64 213 against 235 us, 256 tokens with 16 + 2 + 2 of 256 3.7 against 3.1). An e4m3 cache is bound
+// by its instructions and gains nothing (31,733 tokens with 32 + 8 + 8 of 128: 182 against 180).
+// Alone, the first writes in 160 us (6.4 TB/s) and the last in 132 (5.4 TB/s).
 template <int kSeg, bool kQuant, bool kInter, bool kMany>
 __global__ void __launch_bounds__(kThreads, kMany ? 5 : 4) write_kernel(const __grid_constant__ WriteParams p, const Div by_q,
                                                                        const Div by_k) {
@@ -437,10 +440,8 @@ __global__ void __launch_bounds__(kThreads, kMany ? 5 : 4) write_kernel(const __
     if constexpr (kMany) {
 #pragma unroll
       for (int b = 0; b < kBatch; ++b) finish(now[b]);
-      if (base < total) {
 #pragma unroll
-        for (int b = 0; b < kBatch; ++b) load(now[b], base + b * kSegs);
-      }
+      for (int b = 0; b < kBatch; ++b) load(now[b], base + b * kSegs);
     } else {
       Row next;
       load(next, base);
