@@ -88,18 +88,24 @@ class KVCache:
             raise ValueError("pages must be at least 1")
         shape = (layers, pages, kv_heads, page_size, head_dim)
         dtype = torch.float8_e4m3fn if quantised else torch.bfloat16
-        self.k, self.v = torch.zeros(shape, dtype=dtype, device=device), torch.zeros(shape, dtype=dtype, device=device)
-        self.k_exp = torch.zeros(shape[:-1], dtype=torch.int8, device=device) if quantised else None
-        self.v_exp = torch.zeros(shape[:-1], dtype=torch.int8, device=device) if quantised else None
+        held = [torch.zeros(shape, dtype=dtype, device=device) for _ in range(2)]
+        exps = [torch.zeros(shape[:-1], dtype=torch.int8, device=device) if quantised else None for _ in range(2)]
+        self._buffers = (*held, *exps)
+        self._views = [tuple(None if b is None else b[i] for b in self._buffers) for i in range(layers)]
         self.table = torch.full((rows, self.pages_per_row), -1, dtype=torch.int32, device=device)
         self.status = torch.zeros(1, dtype=torch.int32, device=device)
         self._free = list(range(pages - 1, -1, -1))
         self._held = [[] for _ in range(rows)]
 
+    # the buffers are not replaced: `layer` hands out views that were made once (four of them cost 8 us a call)
+    k = property(lambda self: self._buffers[0])
+    v = property(lambda self: self._buffers[1])
+    k_exp = property(lambda self: self._buffers[2])
+    v_exp = property(lambda self: self._buffers[3])
+
     def layer(self, layer: int) -> Tuple[Tensor, Tensor, Optional[Tensor], Optional[Tensor]]:
         """(k, v, k_exp, v_exp) of one layer, as the ops take them."""
-        return (self.k[layer], self.v[layer], None if self.k_exp is None else self.k_exp[layer],
-                None if self.v_exp is None else self.v_exp[layer])
+        return self._views[layer]
 
     def reserve(self, row: int, tokens: int) -> None:
         """Gives a row pages for its first `tokens` tokens (those it has stay). Raises, changing nothing, when

@@ -2,6 +2,7 @@
 quantiser against torch's own e4m3 conversion, shapes under tracing, and every refusal of the C entries and
 the ops (arguments are checked before any device work)."""
 
+import copy
 import ctypes
 import math
 
@@ -82,6 +83,22 @@ def _meta_cache(quant, pages=5, heads=2, size=16, dim=64, device="meta"):
     k = torch.empty(pages, heads, size, dim, dtype=torch.float8_e4m3fn if quant else BF, device=device)
     e = torch.empty(pages, heads, size, dtype=torch.int8, device=device) if quant else None
     return k, torch.empty_like(k), e, None if e is None else torch.empty_like(e)
+
+
+@pytest.mark.parametrize("quantised", [False, True])
+def test_layers_are_views_of_the_buffers(dm3, quantised):
+    c = dm3.KVCache(3, 2, 40, 2, 64, page_size=16, quantised=quantised, device="cpu")
+    for cache in (c, copy.deepcopy(c)):
+        for i in range(-3, 3):
+            for view, buffer in zip(cache.layer(i), (cache.k, cache.v, cache.k_exp, cache.v_exp)):
+                if buffer is None:
+                    assert view is None and not quantised
+                else:
+                    assert view.data_ptr() == buffer[i].data_ptr() and view.shape == buffer.shape[1:] and view.stride() == buffer[i].stride()
+    with pytest.raises(IndexError):
+        c.layer(3)
+    with pytest.raises(AttributeError):
+        c.k = c.k.clone()
 
 
 def test_fake_impls_trace_on_meta(dm3):
