@@ -191,10 +191,11 @@ __device__ __forceinline__ int token_of(int lr) {
   return kBox == 128 ? ((lr ^ lr >> 2) & 1) << 2 | (lr & 2) | lr >> 2 : lr;
 }
 
-// l * 2^d, d <= 0, where 2^d alone may vanish: the maxima that l refers to can lie 2^229 apart (see the exponents above).
-__device__ __forceinline__ float scale_sum(float l, float d) {
-  const float h = ex2(0.5f * d);
-  return l * h * h;
+// l with its maximum raised from `from` to `to`: l * 2^(from - to), where the power alone may vanish, since maxima that l
+// refers to can lie 2^229 apart (see the exponents above). Before any logit l is 0, or NaN where all of them were.
+__device__ __forceinline__ float raise_sum(float l, float from, float to) {
+  const float h = ex2(0.5f * (from - to));
+  return from == -INFINITY ? l : l * h * h;
 }
 __device__ __forceinline__ float lse_of(float m, float l, bool quant) {  // natural log of the sum, from log2 units
   return l == 0.f ? -INFINITY : (m + (quant ? kSpan - kLift : 0.f) + log2f(l)) * 0.69314718055994531f;
@@ -647,7 +648,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2)
             const float m_was = m[nt][h], f = m_was == -INFINITY ? 0.f : ex2(m_was - x);
             m[nt][h] = x;
             sub[nt][h] = (x == -INFINITY ? 0.f : x) - (kQuant ? kLift : 0.f);
-            l[nt][h] = m_was == -INFINITY ? 0.f : scale_sum(l[nt][h], m_was - x);
+            l[nt][h] = raise_sum(l[nt][h], m_was, x);
 #pragma unroll
             for (int i = 0; i < kDim / 16; ++i) o[nt][i][h] *= f, o[nt][i][2 + h] *= f;
           }
@@ -773,7 +774,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2)
 #pragma unroll
       for (int w = 0; w < kWarps; ++w) {
         const float f = s_m[w][h] == -INFINITY ? 0.f : ex2(s_m[w][h] - mm);
-        ll += s_m[w][h] == -INFINITY ? 0.f : scale_sum(s_l[w][h], s_m[w][h] - mm);
+        ll += raise_sum(s_l[w][h], s_m[w][h], mm);
         s_m[w][h] = f;
       }
       s_l[0][h] = ll, s_l[1][h] = mm;
@@ -835,7 +836,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2)
         }
         for (int r = 0; r < p.splits; ++r) {
           const float f = s_f[r][h] == -INFINITY ? 0.f : ex2(s_f[r][h] - mm);
-          ll += s_f[r][h] == -INFINITY ? 0.f : scale_sum(ld_cluster(&s_l[0][h], r), s_f[r][h] - mm);
+          ll += raise_sum(ld_cluster(&s_l[0][h], r), s_f[r][h], mm);
           s_f[r][h] = f;
         }
         s_qs[h] = inverse(ll, kQuant);
@@ -898,12 +899,12 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constan
 #pragma unroll
     for (int b = 0; b < kJoinBatch; ++b) mm = fmaxf(mm, a[b].x);
     const float back = m == -INFINITY ? 0.f : ex2(m - mm);
-    l = m == -INFINITY ? 0.f : scale_sum(l, m - mm);
+    l = raise_sum(l, m, mm);
     x.x *= back, x.y *= back, x.z *= back, x.w *= back;
 #pragma unroll
     for (int b = 0; b < kJoinBatch; ++b) {
       const float f = a[b].x == -INFINITY ? 0.f : ex2(a[b].x - mm);
-      l += a[b].x == -INFINITY ? 0.f : scale_sum(a[b].y, a[b].x - mm);
+      l += raise_sum(a[b].y, a[b].x, mm);
       x.x += y[b].x * f, x.y += y[b].y * f, x.z += y[b].z * f, x.w += y[b].w * f;
     }
     m = mm;
@@ -915,12 +916,12 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constan
     float mm = m;
     for (int i = 1; i < groups; ++i) mm = fmaxf(mm, s_m[i * per + threadIdx.x]);
     const float f0 = m == -INFINITY ? 0.f : ex2(m - mm);
-    l = m == -INFINITY ? 0.f : scale_sum(l, m - mm);
+    l = raise_sum(l, m, mm);
     x.x *= f0, x.y *= f0, x.z *= f0, x.w *= f0;
     for (int i = 1; i < groups; ++i) {
       const float mi = s_m[i * per + threadIdx.x], f = mi == -INFINITY ? 0.f : ex2(mi - mm);
       const float4 y = s_x[i * per + threadIdx.x];
-      l += mi == -INFINITY ? 0.f : scale_sum(s_l[i * per + threadIdx.x], mi - mm);
+      l += raise_sum(s_l[i * per + threadIdx.x], mi, mm);
       x.x += y.x * f, x.y += y.y * f, x.z += y.z * f, x.w += y.w * f;
     }
     m = mm;

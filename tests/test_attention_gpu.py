@@ -341,6 +341,30 @@ def test_nan_and_infinity_that_are_seen(dm3, quant):
     assert (lse - rlse)[rlse.isfinite()].abs().max() < 1e-4
 
 
+@pytest.mark.parametrize("lengths", [[1, 3], [900, 1, 700], [20000, 5, 40], [33] * 40])
+@pytest.mark.parametrize("quant", [False, True])
+def test_rows_of_nan(dm3, lengths, quant):
+    """Rows all of whose logits are NaN, by the query of one head or by every key: NaN in out and lse, not "nothing seen"."""
+    d = paged(lengths, 1, 64, 16, quant, 3)
+    q = _q(len(lengths), 4, 64, 1, 0.1)
+    q[0, 2, 7] = math.nan
+    n = lengths[1]
+    for t in range(n):
+        at = (int(d["table"][1, t // 16]), 0, t % 16)
+        if quant:
+            d["k"].view(torch.uint8)[at][t % 64] = 0x7F
+        else:
+            d["k"][at][t % 64] = math.nan
+    dev = to_cuda(d)
+    out, lse = dm3.ops.paged_attention(q.cuda(), *held(dev), dev["table"], dev["lengths"], dev["status"])
+    ref, rlse, _, _ = kv_oracle.attention(q, *held(d), d["table"], d["lengths"])
+    out, lse = out.double().cpu(), lse.double().cpu()
+    assert ref[1].isnan().all() and rlse[1].isnan().all() and ref[0, 2].isnan().all() and int(ref.isnan().sum()) == 5 * 64
+    assert torch.equal(out.isnan(), ref.isnan()) and torch.equal(lse.isnan(), rlse.isnan())
+    ok = rlse.isfinite()
+    assert (out - ref)[ok].abs().max() <= ref[ok].abs().max() * 2.0**-7 and (lse - rlse)[ok].abs().max() < 1e-4
+
+
 def test_captured_without_a_first_call(dm3):
     """The first call of a process's kernels may be a captured one."""
     code = """
