@@ -194,8 +194,8 @@ __device__ __forceinline__ int token_of(int lr) {
 // l with its maximum raised from `from` to `to`: l * 2^(from - to), where the power alone may vanish, since maxima that l
 // refers to can lie 2^229 apart (see the exponents above). Before any logit l is 0, or NaN where all of them were.
 __device__ __forceinline__ float raise_sum(float l, float from, float to) {
-  const float h = ex2(0.5f * (from - to));
-  return from == -INFINITY ? l : l * h * h;
+  const float h = from == -INFINITY ? 1.f : ex2(0.5f * (from - to));
+  return l * h * h;
 }
 __device__ __forceinline__ float lse_of(float m, float l, bool quant) {  // natural log of the sum, from log2 units
   return l == 0.f ? -INFINITY : (m + (quant ? kSpan - kLift : 0.f) + log2f(l)) * 0.69314718055994531f;
