@@ -529,6 +529,7 @@ def _(logits, lse, token, eos_id, semantic_begin, score):
 # has to see the call as an operator, and go through torch.ops.dm3.* under tracing, for tensor subclasses (fake
 # tensors among them) and where autograd would have to be told that there is no gradient.
 _INT_MAX = 2**31 - 1  # the C entries take counts as int
+_DENSE = torch.contiguous_format
 
 
 def _plain(*ts: Optional[Tensor]) -> bool:
@@ -635,7 +636,7 @@ def _rope(x: Tensor, positions: Tensor, inv_freq: Tensor, interleaved: bool = Fa
     if heads * dim > 1 << 24:
         raise RuntimeError("rope: bad head count or head size")
     positions, inv_freq = _int64(positions, T, "positions"), _angles(inv_freq)
-    y = torch.empty((T, heads, dim), dtype=BF16, device=x.device)
+    y = torch.empty_like(x, memory_format=_DENSE)
     _launch(dev, "dm3_rope", x.data_ptr(), T, heads, dim, x.stride(0), x.stride(1), positions.data_ptr(),
             inv_freq.data_ptr(), 2 * inv_freq.shape[0], 1 if interleaved else 0, factor, y.data_ptr())
     return y
@@ -677,10 +678,10 @@ def _kv_write(k: Tensor, v: Tensor, positions: Tensor, table: Tensor, k_cache: T
         q_heads = q.shape[1]
         if q.shape != (T, q_heads, dim):
             raise RuntimeError(f"q must be [{T}, heads, {dim}]")
-        out = torch.empty((T, q_heads, dim), dtype=BF16, device=k.device)
+        out = torch.empty_like(q, memory_format=_DENSE)
         q_at, (q_ts, q_hs, _) = q.data_ptr(), q.stride()
     else:
-        out = torch.empty((0,), dtype=BF16, device=k.device)
+        out = k.new_empty((0,))
     if inv_freq is not None:
         inv_freq = _angles(inv_freq)
         inv_at, rot = inv_freq.data_ptr(), 2 * inv_freq.shape[0]
@@ -722,7 +723,7 @@ def _kv_read(k_cache: Tensor, v_cache: Tensor, k_exp: Optional[Tensor], v_exp: O
     if max_length < 0:
         raise RuntimeError("max_length must not be negative")
     lengths = _int64(lengths, rows, "lengths")
-    k = torch.empty((rows, heads, max_length, dim), dtype=BF16, device=k_cache.device)
+    k = k_cache.new_empty((rows, heads, max_length, dim), dtype=BF16)
     v = torch.empty_like(k)
     _launch(dev, "dm3_kv_read", *held, pages, size, heads, dim, *tab, lengths.data_ptr(), max_length, k.data_ptr(),
             v.data_ptr(), status.data_ptr())
@@ -756,12 +757,12 @@ def _paged_attention(q: Tensor, k_cache: Tensor, v_cache: Tensor, k_exp: Optiona
     if q.shape != (rows, q_heads, dim):
         raise RuntimeError(f"q must be [{rows}, heads, {dim}]")
     lengths = _int64(lengths, rows, "lengths")
-    out = torch.empty((rows, q_heads, dim), dtype=BF16, device=q.device)
-    lse = torch.empty((rows, q_heads), dtype=torch.float32, device=q.device)
+    out = torch.empty_like(q, memory_format=_DENSE)
+    lse = q.new_empty((rows, q_heads), dtype=torch.float32)
     # scratch from the caller's allocator: calls on other streams and in other graphs have their own
     nbytes = _lib.load().dm3_paged_attention_workspace_bytes(rows, q_heads, heads, dim, size, tab[3], k_exp is not None,
                                                               window)
-    ws = torch.empty((nbytes,), dtype=torch.uint8, device=q.device) if nbytes else None
+    ws = q.new_empty((nbytes,), dtype=torch.uint8) if nbytes else None
     _launch(dev, "dm3_paged_attention", q.data_ptr(), q.stride(0), q.stride(1), q_heads, *held, pages, size, heads, dim, *tab,
             lengths.data_ptr(), dim ** -0.5 if scale is None else scale, window, out.data_ptr(), lse.data_ptr(),
             status.data_ptr(), None if ws is None else ws.data_ptr(), nbytes)
