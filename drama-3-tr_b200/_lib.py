@@ -8,8 +8,10 @@ naming the missing file.
 from __future__ import annotations
 
 import ctypes
+import functools
 import os
 import re
+import struct
 from pathlib import Path
 
 PKG_DIR = Path(__file__).resolve().parent
@@ -71,6 +73,10 @@ SIGNATURES = {
     "dm3_paged_attention_workspace_bytes": (_sz, [_i, _i, _i, _i, _i, _i, _i, _i64]),
     "dm3_paged_attention": (_i, [_p, _i64, _i64, _i, _p, _p, _i64, _p, _p, _i64, _i, _i, _i, _i, _p, _i64, _i, _i, _p,
                                  _f32, _i64, _p, _p, _p, _p, _sz, _p]),
+    "dm3_rope_packed": (_i, [ctypes.c_char_p, _p]),
+    "dm3_kv_write_packed": (_i, [ctypes.c_char_p, _p]),
+    "dm3_kv_read_packed": (_i, [ctypes.c_char_p, _p]),
+    "dm3_paged_attention_packed": (_i, [ctypes.c_char_p, _p]),
     "dm3_last_launch_count": (_i, []),
 }
 
@@ -99,6 +105,15 @@ def load():
             fn.argtypes = args
         _lib = lib
     return _lib
+
+
+@functools.lru_cache(maxsize=None)
+def packed(name: str):
+    """(pack, entry) of an entry point that also takes its arguments packed: entry(pack(*arguments), stream) calls it.
+    Null pointers are 0."""
+    args = SIGNATURES[name][1][:-1]
+    form = "=" + "".join("d" if a in (_f32, _f64) else "q" for a in args)
+    return struct.Struct(form).pack, getattr(load(), name + "_packed")
 
 
 def check(rc: int, what: str) -> None:

@@ -4,10 +4,14 @@
 #include <cstring>
 #include <mutex>
 #include <string>
+#include <tuple>
+#include <type_traits>
+#include <utility>
 
 #include <cuda.h>
 #include <cuda_runtime.h>
 
+#include "dm3.h"
 #include "dm3_internal.h"
 
 namespace dm3 {
@@ -145,7 +149,46 @@ bool tensor_map_boxes(CUtensorMap* out, const void* base, uint64_t row_bytes, ui
   return true;
 }
 
+// Calls an entry point with its arguments from 8-byte places, the stream last.
+template <typename T>
+static bool unpack_arg(const void* args, size_t i, T& out) {
+  const char* at = static_cast<const char*>(args) + 8 * i;
+  if constexpr (std::is_floating_point_v<T>) {
+    double v;
+    std::memcpy(&v, at, 8);
+    out = static_cast<T>(v);
+    return true;
+  } else if constexpr (std::is_pointer_v<T>) {
+    static_assert(sizeof(T) == 8);
+    std::memcpy(&out, at, 8);
+    return true;
+  } else {
+    int64_t v;
+    std::memcpy(&v, at, 8);
+    out = static_cast<T>(v);
+    return static_cast<int64_t>(out) == v && (std::is_signed_v<T> || v >= 0);
+  }
+}
+template <typename... A, size_t... I>
+static int unpack_call(int (*entry)(A...), const void* args, void* stream, std::index_sequence<I...>) {
+  note_launches(0);
+  if (!args) return set_error("null arguments"), DM3_EINVAL;
+  std::tuple<A...> t;
+  if (!(unpack_arg(args, I, std::get<I>(t)) && ...)) return set_error("an argument is out of its type's range"), DM3_EINVAL;
+  std::get<sizeof...(A) - 1>(t) = stream;
+  return std::apply(entry, t);
+}
+template <typename... A>
+static int packed(int (*entry)(A...), const void* args, void* stream) {
+  return unpack_call(entry, args, stream, std::make_index_sequence<sizeof...(A) - 1>{});
+}
+
 }  // namespace dm3
+
+extern "C" int dm3_rope_packed(const void* args, void* stream) { return dm3::packed(dm3_rope, args, stream); }
+extern "C" int dm3_kv_write_packed(const void* args, void* stream) { return dm3::packed(dm3_kv_write, args, stream); }
+extern "C" int dm3_kv_read_packed(const void* args, void* stream) { return dm3::packed(dm3_kv_read, args, stream); }
+extern "C" int dm3_paged_attention_packed(const void* args, void* stream) { return dm3::packed(dm3_paged_attention, args, stream); }
 
 extern "C" const char* dm3_last_error(void) { return dm3::g_error.c_str(); }
 

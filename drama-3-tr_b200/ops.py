@@ -25,6 +25,7 @@ Ops:
 from __future__ import annotations
 
 import ctypes
+import functools
 from typing import Optional
 
 import torch
@@ -554,13 +555,13 @@ def _same_device(first: Tensor, *ts: Optional[Tensor]) -> int:
 
 def _launch(device: int, name: str, *args) -> None:
     """Calls a C entry point on the device's current stream, with that device current."""
-    fn = getattr(_lib.load(), name)
+    pack, fn = _lib.packed(name)
     stream = torch._C._cuda_getCurrentRawStream(device)
     if device == torch._C._cuda_getDevice():
-        rc = fn(*args, stream)
+        rc = fn(pack(*args), stream)
     else:
         with torch.cuda.device(device):
-            rc = fn(*args, stream)
+            rc = fn(pack(*args), stream)
     if rc:
         _lib.check(rc, name)
 
@@ -597,7 +598,7 @@ def _cache_args(k_cache: Tensor, v_cache: Tensor, k_exp: Optional[Tensor], v_exp
     pages, heads, size, dim = shape
     if strides != v_cache.stride() or strides[1:] != (size * dim, dim, 1):
         raise RuntimeError("each page of the cache must be contiguous, with the same strides for keys and values")
-    k_at = v_at = None
+    k_at = v_at = 0
     exp_stride = 0
     if k_exp is None and v_exp is None:
         if k_cache.dtype != BF16:
@@ -668,7 +669,7 @@ def _kv_write(k: Tensor, v: Tensor, positions: Tensor, table: Tensor, k_cache: T
     if k.shape != (T, heads, dim) or v.shape != k.shape:
         raise RuntimeError(f"k and v must be [T, {heads}, {dim}] as the cache")
     positions = _int64(positions, T, "positions")
-    q_at = rows_at = inv_at = None
+    q_at = rows_at = inv_at = 0
     q_heads = q_ts = q_hs = rot = 0
     if rows is not None:
         rows = _int64(rows, T, "rows")
@@ -747,6 +748,12 @@ def kv_read(k_cache: Tensor, v_cache: Tensor, k_exp: Optional[Tensor], v_exp: Op
                                                                    max_length, status)
 
 
+@functools.lru_cache(maxsize=1024)
+def _attention_workspace(device: int, *sizes) -> int:
+    with torch.cuda.device(device):
+        return _lib.load().dm3_paged_attention_workspace_bytes(*sizes)
+
+
 def _paged_attention(q: Tensor, k_cache: Tensor, v_cache: Tensor, k_exp: Optional[Tensor], v_exp: Optional[Tensor],
                      table: Tensor, lengths: Tensor, status: Tensor, scale: Optional[float] = None,
                      window: int = 0) -> tuple[Tensor, Tensor]:
@@ -760,12 +767,11 @@ def _paged_attention(q: Tensor, k_cache: Tensor, v_cache: Tensor, k_exp: Optiona
     out = torch.empty_like(q, memory_format=_DENSE)
     lse = q.new_empty((rows, q_heads), dtype=torch.float32)
     # scratch from the caller's allocator: calls on other streams and in other graphs have their own
-    nbytes = _lib.load().dm3_paged_attention_workspace_bytes(rows, q_heads, heads, dim, size, tab[3], k_exp is not None,
-                                                              window)
+    nbytes = _attention_workspace(dev, rows, q_heads, heads, dim, size, tab[3], k_exp is not None, window)
     ws = q.new_empty((nbytes,), dtype=torch.uint8) if nbytes else None
     _launch(dev, "dm3_paged_attention", q.data_ptr(), q.stride(0), q.stride(1), q_heads, *held, pages, size, heads, dim, *tab,
             lengths.data_ptr(), dim ** -0.5 if scale is None else scale, window, out.data_ptr(), lse.data_ptr(),
-            status.data_ptr(), None if ws is None else ws.data_ptr(), nbytes)
+            status.data_ptr(), 0 if ws is None else ws.data_ptr(), nbytes)
     return out, lse
 
 

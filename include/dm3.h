@@ -435,6 +435,16 @@ int dm3_paged_attention(const void* q, int64_t q_rs, int64_t q_hs, int q_heads, 
                         int per_row, const int64_t* lengths, float scale, int64_t window, void* out, float* lse,
                         uint32_t* status, void* workspace, size_t workspace_bytes, void* stream);
 
+/*
+ * The four calls above for callers that pay by the argument (ctypes takes 3.8 us for the 34 of dm3_kv_write, 0.7 this way):
+ * args holds every argument before the stream in 8 bytes, in order: pointers, integers sign-extended, float and double as
+ * double. An integer that its type does not hold is refused.
+ */
+int dm3_rope_packed(const void* args, void* stream);
+int dm3_kv_write_packed(const void* args, void* stream);
+int dm3_kv_read_packed(const void* args, void* stream);
+int dm3_paged_attention_packed(const void* args, void* stream);
+
 /* Number of kernels the last MoE / GEMV entry point launched on this host thread. */
 int dm3_last_launch_count(void);
 

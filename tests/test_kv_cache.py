@@ -198,3 +198,27 @@ def test_c_entries_with_nothing_to_do(dm3, name):
     change = dict(T=0) if "T" in CALLS[name] else dict(table_rows=0, table=None)
     assert getattr(lib, name)(*{**CALLS[name], **change}.values()) == 0
     assert lib.dm3_last_launch_count() == 0
+
+
+def _packed(dm3, name, args):
+    pack, entry = dm3._lib.packed(name)
+    return entry(pack(*(a.value if isinstance(a, ctypes.c_void_p) else a or 0 for a in list(args.values())[:-1])), None)
+
+
+@pytest.mark.parametrize("name", CALLS)
+def test_packed_entries(dm3, name):
+    """The packed form of an entry passes on every argument: the same refusals with the same words, the same answer to
+    a call with nothing to do; and a count that a C int would cut short is refused."""
+    lib = dm3._lib.load()
+    for change in BAD[name]:
+        args = {**CALLS[name], **change}
+        rc, why = getattr(lib, name)(*args.values()), lib.dm3_last_error()
+        assert (_packed(dm3, name, args), lib.dm3_last_error()) == (rc, why), (name, change)
+    change = dict(T=0) if "T" in CALLS[name] else dict(table_rows=0, table=None)
+    assert _packed(dm3, name, {**CALLS[name], **change}) == 0 and lib.dm3_last_launch_count() == 0
+    for key, kind in zip(CALLS[name], dm3._lib.SIGNATURES[name][1]):
+        if kind is ctypes.c_int:
+            for n in (2**31, 2**32, -2**31 - 1):
+                assert _packed(dm3, name, {**CALLS[name], key: n}) == dm3._lib.DM3_EINVAL
+                assert b"range" in lib.dm3_last_error()
+    assert getattr(lib, name + "_packed")(None, None) == dm3._lib.DM3_EINVAL
