@@ -68,6 +68,7 @@ struct Params {
   int64_t window;
   int splits;          // CTAs of a cluster; 0: stream
   bool longest_first;  // one CTA a unit: blockIdx.z counts the rows by their tiles
+  bool hasty;          // the wait limit is below kHasty: what has not landed when it is needed has run out
   __nv_bfloat16* out;  // [rows][q_heads][dim]
   float* lse;          // [rows][q_heads]
   // stream: the first tile of each row in the sequence and their number ([rows + 1], a tile counted once a head unit),
@@ -397,7 +398,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2)
     // block's tile i lies, and asks for it.
     constexpr int kBlock = 32 / kU;  // steps a block
     const int mine = static_cast<int>((end - begin - warp + kWarps - 1) / kWarps);  // tiles of this warp
-    int steps = mine > 0 ? (mine + kU - 1) / kU : 0;
+    const int steps = mine > 0 ? (mine + kU - 1) / kU : 0;
     int page, y, range;  // y: first row of the tile in its page
     auto find = [&](int step0) {
       const int64_t t = begin + (static_cast<int64_t>(step0) * kU + lane) * kWarps + warp;
@@ -510,19 +511,16 @@ __global__ void __launch_bounds__(kWarps * 32, 2)
     int ev0 = 0;        // the exponent of the first value row seen
     bool wide = false;  // a later one is more than 44 away
 
-    // The unit in the current slot has landed; when the wait ran out, no more are asked for.
-    auto landed = [&](int step) {
-      if (__any_sync(0xffffffffu, !mbar_wait(&full[slot], parity))) {
-        if (lane == 0) kv::set_status(p.c.status, STATUS_TIMEOUT);
-        steps = min(steps, step + (C::kRing + 1) / 2);
-        lost = true;
-      }
-    };
     auto next_slot = [&] {
       if (++slot == C::kRing) slot = 0, parity ^= 1;
     };
+    auto landed = [&] { return __all_sync(0xffffffffu, p.hasty ? mbar_test(&full[slot], parity) : mbar_wait(&full[slot], parity)); };
+    int stuck = -1;  // the unit (a step's keys or its values) whose wait ran out: the segment ends there
     for (int step = 0; step < steps; ++step) {
-      landed(step);
+      if (!landed()) {
+        stuck = 2 * step;
+        break;
+      }
       const uint8_t* unit = ring + slot * C::kUnit;
       // a product takes the sum of the one before 25 cycles later: two sums side by side where a step has but one tile
       constexpr int kChains = kU * kNT == 1 ? 2 : 1;
@@ -692,7 +690,10 @@ __global__ void __launch_bounds__(kWarps * 32, 2)
           }
         }
 
-      landed(step);
+      if (!landed()) {
+        stuck = 2 * step + 1;
+        break;
+      }
       unit = ring + slot * C::kUnit;
 #pragma unroll
       for (int u = 0; u < kU; ++u) {
@@ -751,6 +752,17 @@ __global__ void __launch_bounds__(kWarps * 32, 2)
       __syncwarp();  // the unit is read
       ask(C::kRing & 1, step + (C::kRing + 1) / 2, slot);
       next_slot();
+    }
+
+    // After a wait that ran out no more is asked for, and what was is waited for, that unit and those up to kRing behind it:
+    // the join and, once this CTA has left, another one use their places.
+    if (stuck >= 0) {
+      if (lane == 0) kv::set_status(p.c.status, STATUS_TIMEOUT);
+      lost = true;
+      for (const int asked = min(2 * steps, stuck + C::kRing); stuck < asked; ++stuck) {
+        mbar_drain(&full[slot], parity);
+        next_slot();
+      }
     }
 
     // join the warps; the ring's place is free once every warp is here (it has waited for all that it asked for)
@@ -935,6 +947,11 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constan
 }
 
 // ------------------------------------------------------------------ host side
+// A wait on an mbarrier sleeps in hardware for longer than any copy takes before its time is looked at, so limits below
+// this many nanoseconds would have no effect; they are kept for each device, and the kernel then does not wait at all.
+constexpr uint64_t kHasty = 1000;
+static std::atomic<uint64_t> g_hasty{0};  // a bit a device
+
 static int sms() {
   int dev = 0;
   cudaGetDevice(&dev);
@@ -1037,7 +1054,15 @@ static int attend(const Params& p, dim3 grid, void* stream) {
 }  // namespace attn
 }  // namespace dm3
 
-int dm3::wait_limit_attention(uint64_t ns) { return static_cast<int>(set_wait_limit_here(ns)); }
+int dm3::wait_limit_attention(uint64_t ns) {
+  const cudaError_t err = set_wait_limit_here(ns);
+  if (err != cudaSuccess) return static_cast<int>(err);
+  int dev = 0;
+  cudaGetDevice(&dev);
+  const uint64_t bit = uint64_t(1) << (dev & 63);
+  ns < attn::kHasty ? attn::g_hasty.fetch_or(bit) : attn::g_hasty.fetch_and(~bit);
+  return 0;
+}
 
 // ------------------------------------------------------------------ C ABI
 extern "C" size_t dm3_paged_attention_workspace_bytes(int rows, int q_heads, int kv_heads, int dim, int page_size,
@@ -1071,6 +1096,9 @@ extern "C" int dm3_paged_attention(const void* q, int64_t q_rs, int64_t q_hs, in
   const attn::Plan plan = attn::plan(rows, q_heads, kv_heads, dim, page_size, per_row, k_exp != nullptr, window);
   p.q = static_cast<const __nv_bfloat16*>(q), p.q_rs = q_rs, p.q_hs = q_hs, p.q_heads = q_heads, p.kv_heads = kv_heads;
   p.group = q_heads / kv_heads, p.head_tiles = plan.head_tiles, p.splits = plan.splits, p.longest_first = plan.longest_first;
+  int dev = 0;
+  cudaGetDevice(&dev);
+  p.hasty = attn::g_hasty.load(std::memory_order_relaxed) >> (dev & 63) & 1;
   p.lengths = lengths, p.scale_log2 = scale * 1.44269504088896341f, p.window = window;
   p.out = static_cast<__nv_bfloat16*>(out), p.lse = lse;
   const int heads = attn::tile_heads(p.group);

@@ -415,3 +415,42 @@ def test_two_graphs_and_two_streams(dm3):
     torch.cuda.synchronize()
     for got, w in zip([*outs, out2], want):
         assert torch.equal(got[0], w[0]) and torch.equal(got[1], w[1])
+
+
+@pytest.mark.parametrize("dim,group,quant", [(64, 4, True), (64, 16, True), (128, 4, False), (128, 16, True), (192, 4, False), (192, 12, True), (256, 8, True)])
+@pytest.mark.parametrize("rows,row_bytes", [(2, 40 << 20), (16, 5 << 18), (400, 1 << 17)])
+def test_waits_that_run_out(dm3, dim, group, quant, rows, row_bytes):
+    """With the shortest limit waits run out, in every layout (equal shares, clusters, a CTA a unit) and with rings of an even and an odd
+    number of units: the call ends all the same and its status says so; the calls after it have the right answer again.
+    Where all copies stay ahead of the products no wait runs out and the answer is right; not over long bf16 rows, which
+    wait for memory."""
+    tokens = row_bytes // (dim if quant else 2 * dim)
+    cache = dm3.KVCache(1, rows, tokens, 1, dim, page_size=16, quantised=quant)
+    g = torch.Generator("cuda").manual_seed(dim)
+    for x in (cache.k, cache.v):
+        x.view(torch.uint8).random_(0, 64, generator=g)  # e4m3 below 2, bf16 below 2^-1
+    for r in range(rows):
+        cache.reserve(r, tokens)
+    q = torch.randn(rows, group, dim, generator=g, device="cuda").to(BF)
+    lengths = torch.full((rows,), tokens, device="cuda")
+    want = cache.attend(0, q, lengths)
+    assert cache.check() == 0 and want[0].isfinite().all() and want[1].isfinite().all()
+    flush = torch.zeros(1 << 26, device="cuda")
+    try:
+        torch.cuda.synchronize()
+        dm3.ops.set_wait_limit(1)
+        ran_out = []
+        for _ in range(4):
+            flush += 1  # the cache's rows are not in L2
+            out, lse = cache.attend(0, q, lengths)
+            ran_out.append(cache.check())
+            assert ran_out[-1] == 1 or ran_out[-1] == 0 and torch.equal(out, want[0]) and torch.equal(lse, want[1])
+        print("status", ran_out)
+        assert any(ran_out) or quant or rows > 2
+    finally:
+        torch.cuda.synchronize()
+        dm3.ops.set_wait_limit(1_000_000_000)
+    for _ in range(3):
+        out, lse = cache.attend(0, q, lengths)
+        assert torch.equal(out, want[0]) and torch.equal(lse, want[1])
+    assert cache.check() == 0
