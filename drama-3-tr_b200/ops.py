@@ -30,6 +30,8 @@ from typing import Optional
 
 import torch
 from torch import Tensor
+from torch.overrides import _get_current_function_mode_stack
+from torch.utils._device import DeviceContext
 
 from . import _lib
 
@@ -527,14 +529,27 @@ def _(logits, lse, token, eos_id, semantic_begin, score):
 # ----------------------------------------------------------------------------- rotary positions and the paged cache
 # These ops take a few microseconds on the device, less than torch.library's dispatch of a Python op (20 us, 45 us with
 # mutated arguments). So `rope`, `kv_write`, `kv_read` and `paged_attention` call their kernels directly where nothing
-# has to see the call as an operator, and go through torch.ops.dm3.* under tracing, for tensor subclasses (fake
-# tensors among them) and where autograd would have to be told that there is no gradient.
+# has to see the call as an operator, and go through torch.ops.dm3.* while anything traces, records or transforms calls
+# (torch.compile and export, make_fx, torch.jit.trace, dispatch and function modes, torch.func), for tensor
+# subclasses (fake tensors among them) and where autograd would have to be told that there is no gradient.
 _INT_MAX = 2**31 - 1  # the C entries take counts as int
 _DENSE = torch.contiguous_format
 
 
+_compiling, _jit_tracing, _transform = torch.compiler.is_compiling, torch._C._is_tracing, torch._C._functorch.maybe_current_level
+_dispatch_modes, _function_modes = torch._C._len_torch_dispatch_stack, torch._C._len_torch_function_stack
+
+
+def _watched() -> bool:
+    """Whether a call has to be seen as an operator whatever its tensors are."""
+    if _compiling() or _dispatch_modes() or _jit_tracing() or _transform() is not None:
+        return True
+    # a default device is a function mode that leaves these calls as they are
+    return bool(_function_modes()) and any(type(m) is not DeviceContext for m in _get_current_function_mode_stack())
+
+
 def _plain(*ts: Optional[Tensor]) -> bool:
-    if torch.compiler.is_compiling():
+    if _watched():
         return False
     for t in ts:
         if t is not None and (type(t) is not Tensor or t.requires_grad):

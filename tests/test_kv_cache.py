@@ -222,3 +222,73 @@ def test_packed_entries(dm3, name):
                 assert _packed(dm3, name, {**CALLS[name], key: n}) == dm3._lib.DM3_EINVAL
                 assert b"range" in lib.dm3_last_error()
     assert getattr(lib, name + "_packed")(None, None) == dm3._lib.DM3_EINVAL
+
+
+@pytest.fixture
+def stub(dm3, monkeypatch):
+    """The ops on CPU tensors with the launch replaced: (ops, names of the entries that were launched directly)."""
+    names = []
+    monkeypatch.setattr(dm3.ops, "_same_device", lambda *a: 0)
+    monkeypatch.setattr(dm3.ops, "_attention_workspace", lambda *a: 0)
+    monkeypatch.setattr(dm3.ops, "_launch", lambda device, name, *a: names.append(name))
+    return dm3.ops, names
+
+
+def _op_calls(ops):
+    """{name: (call on its tensors, tensors, places of those that could have a gradient)}."""
+    x, q = torch.randn(3, 2, 64).to(BF), torch.randn(3, 4, 64).to(BF)
+    pos, inv = torch.arange(3), torch.ones(16, dtype=torch.float64)
+    k, v = torch.zeros(5, 2, 16, 64, dtype=BF), torch.zeros(5, 2, 16, 64, dtype=BF)
+    t, s = torch.zeros(3, 4, dtype=torch.int32), torch.zeros(1, dtype=torch.int32)
+    return {
+        "rope": (lambda x, pos, inv: ops.rope(x, pos, inv), (x, pos, inv), (0, 2)),
+        "kv_write": (lambda a, b, pos, t, k, v, s, q, inv: ops.kv_write(a, b, pos, t, k, v, None, None, s, None, q, inv),
+                     (x, x.clone(), pos, t, k, v, s, q, inv), (0, 1, 4, 5, 7, 8)),
+        "kv_read": (lambda k, v, t, n, s: ops.kv_read(k, v, None, None, t, n, 7, s), (k, v, t, pos, s), (0, 1)),
+        "paged_attention": (lambda q, k, v, t, n, s: ops.paged_attention(q, k, v, None, None, t, n, s), (q, k, v, t, pos, s), (0, 1, 2)),
+    }
+
+
+OPS = ["rope", "kv_write", "kv_read", "paged_attention"]
+
+
+@pytest.mark.parametrize("name", OPS)
+def test_every_tracer_sees_the_operator(stub, name):
+    """Whatever records or watches calls finds the operator, not the allocation of its result; a plain call is a direct one."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+    from torch.overrides import TorchFunctionMode
+    from torch.utils._python_dispatch import TorchDispatchMode
+
+    ops, names = stub
+    fn, args, _ = _op_calls(ops)[name]
+    op = "dm3::" + name
+    for mode in ("real", "fake"):
+        graph = make_fx(fn, tracing_mode=mode)(*args).graph
+        assert ["dm3." + name + ".default"] == [str(n.target) for n in graph.nodes if n.op == "call_function" and "getitem" not in str(n.target)]
+    kinds = [n.kind() for n in torch.jit.trace(fn, args, check_trace=False).graph.nodes()]
+    assert op in kinds and not any("empty" in k for k in kinds)
+
+    class Watch(TorchDispatchMode):
+        def __torch_dispatch__(self, func, types, a=(), kw=None):
+            seen.append(func.name())
+            return func(*a, **(kw or {}))
+
+    class See(TorchFunctionMode):
+        def __torch_function__(self, func, types, a=(), kw=None):
+            seen.append(str(func))
+            return func(*a, **(kw or {}))
+
+    seen = []
+    with Watch():
+        fn(*args)
+    assert op in seen
+    seen = []
+    with See():
+        fn(*args)
+    assert any("dm3" in x and name in x for x in seen)
+    before = len(names)
+    for plain in (torch.no_grad(), torch.inference_mode(), torch.device("cpu")):  # a default device is no tracer
+        with plain, torch.profiler.profile() as prof:
+            fn(*args)
+        assert not any(e.name.startswith("dm3::") for e in prof.events())
+    assert names[before:] == ["dm3_" + name] * 3
