@@ -30,6 +30,7 @@ from typing import Optional
 
 import torch
 from torch import Tensor
+from torch.autograd import forward_ad
 from torch.overrides import _get_current_function_mode_stack
 from torch.utils._device import DeviceContext
 
@@ -548,13 +549,17 @@ def _watched() -> bool:
     return bool(_function_modes()) and any(type(m) is not DeviceContext for m in _get_current_function_mode_stack())
 
 
-def _plain(*ts: Optional[Tensor]) -> bool:
-    if _watched():
-        return False
-    for t in ts:
-        if t is not None and (type(t) is not Tensor or t.requires_grad):
-            return False
-    return True
+def _route(direct, op, *ts: Optional[Tensor]):
+    """How a call goes: `direct`, or `op` where it has to be seen. ts: its tensors that could have a gradient. None of
+    these operators has one: backwards `op` refuses it, forwards it would be a silent zero and is refused here."""
+    plain = not _watched() and forward_ad._current_level < 0
+    if not plain and not _compiling() and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in ts):
+        raise RuntimeError("drama3_b200: rotary positions, the cache and attention have no gradient")
+    if plain:
+        for t in ts:
+            if t is not None and (type(t) is not Tensor or t.requires_grad):
+                return op
+    return direct if plain else op
 
 
 def _same_device(first: Tensor, *ts: Optional[Tensor]) -> int:
@@ -670,7 +675,7 @@ def rope(x: Tensor, positions: Tensor, inv_freq: Tensor, interleaved: bool = Fal
     """Rotary positions: x bf16 [T, heads, dim] with the first 2 * len(inv_freq) values of every head turned
     in pairs by positions[t] * inv_freq[i] (formed in 64 bits), times factor. Pair i is (2i, 2i + 1) when
     interleaved, else (i, i + len(inv_freq)). positions int64 [T], inv_freq float64 (see `Rope`)."""
-    return (_rope if _plain(x, positions, inv_freq) else _rope_op)(x, positions, inv_freq, interleaved, factor)
+    return _route(_rope, _rope_op, x, positions, inv_freq)(x, positions, inv_freq, interleaved, factor)
 
 
 def _kv_write(k: Tensor, v: Tensor, positions: Tensor, table: Tensor, k_cache: Tensor, v_cache: Tensor,
@@ -727,7 +732,7 @@ def kv_write(k: Tensor, v: Tensor, positions: Tensor, table: Tensor, k_cache: Te
     multiple of 16 values). A token with a negative row or position is padding: it is not cached and its
     query is zeros. Two tokens of one call must not share a place. See `KVCache` for the buffers; status
     collects skipped tokens (bit 4) whose place or page lies outside the table or the cache."""
-    return (_kv_write if _plain(k, v, q, k_cache, v_cache) else _kv_write_op)(
+    return _route(_kv_write, _kv_write_op, k, v, q, inv_freq, k_cache, v_cache)(
         k, v, positions, table, k_cache, v_cache, k_exp, v_exp, status, rows, q, inv_freq, interleaved, factor)
 
 
@@ -759,8 +764,7 @@ def kv_read(k_cache: Tensor, v_cache: Tensor, k_exp: Optional[Tensor], v_exp: Op
             lengths: Tensor, max_length: int, status: Tensor) -> tuple[Tensor, Tensor]:
     """The first min(lengths[r], max_length) tokens of every row of a paged cache as dense bf16 (keys, values)
     [rows, kv_heads, max_length, dim], exactly the values that the cache stands for, and zeros behind them."""
-    return (_kv_read if _plain(k_cache, v_cache) else _kv_read_op)(k_cache, v_cache, k_exp, v_exp, table, lengths,
-                                                                   max_length, status)
+    return _route(_kv_read, _kv_read_op, k_cache, v_cache)(k_cache, v_cache, k_exp, v_exp, table, lengths, max_length, status)
 
 
 @functools.lru_cache(maxsize=1024)
@@ -807,5 +811,5 @@ def paged_attention(q: Tensor, k_cache: Tensor, v_cache: Tensor, k_exp: Optional
     Returns (out bf16 [rows, q_heads, dim], lse fp32 [rows, q_heads], the natural log of the sum of exp).
     A row that sees nothing gives zeros and -inf. The launch is laid out for the table's width, so a
     narrower view of it (table[:, :n]) makes a shorter call."""
-    return (_paged_attention if _plain(q, k_cache, v_cache) else _paged_attention_op)(
+    return _route(_paged_attention, _paged_attention_op, q, k_cache, v_cache)(
         q, k_cache, v_cache, k_exp, v_exp, table, lengths, status, scale, window)

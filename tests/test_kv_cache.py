@@ -292,3 +292,22 @@ def test_every_tracer_sees_the_operator(stub, name):
             fn(*args)
         assert not any(e.name.startswith("dm3::") for e in prof.events())
     assert names[before:] == ["dm3_" + name] * 3
+
+
+@pytest.mark.parametrize("name", OPS)
+def test_every_gradient_is_refused(stub, name):
+    """A gradient asked for by any input is an error, backwards and forwards, not a silent zero."""
+    import torch.autograd.forward_ad as forward
+
+    ops, _ = stub
+    fn, args, places = _op_calls(ops)[name]
+    for at in places:
+        leaf = args[at].clone().requires_grad_()
+        # (an in-place write to a leaf is refused by the call itself)
+        with pytest.raises(RuntimeError, match="gradient|autograd|in-place"):
+            out = fn(*args[:at], leaf, *args[at + 1:])
+            (out[0] if isinstance(out, tuple) else out).double().sum().backward()
+        with forward.dual_level(), pytest.raises(RuntimeError, match="gradient"):
+            fn(*args[:at], forward.make_dual(args[at], torch.ones_like(args[at])), *args[at + 1:])
+        with pytest.raises(RuntimeError, match="gradient"):
+            torch.func.jvp(lambda x: fn(*args[:at], x, *args[at + 1:]), (args[at],), (torch.ones_like(args[at]),))
