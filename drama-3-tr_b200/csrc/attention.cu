@@ -508,7 +508,8 @@ __global__ void __launch_bounds__(kWarps * 32, 2)
       for (int h = 0; h < 2; ++h) m[nt][h] = -INFINITY, sub[nt][h] = 0.f, l[nt][h] = 0.f, qs[nt][h] = s_qs[nt * 8 + 2 * lc + h];
     }
 
-    int ev0 = 0;        // the exponent of the first value row seen
+    constexpr int kNone = 1 << 20;
+    int ev0 = kNone;    // the exponent of the first value row seen
     bool wide = false;  // a later one is more than 44 away
 
     auto next_slot = [&] {
@@ -586,17 +587,21 @@ __global__ void __launch_bounds__(kWarps * 32, 2)
           }
       // logits in log2 units (with the value rows' exponents), -inf where nothing is seen
       float back[kU][2];  // 2^-(exponent + kSpan)
-      if (kQuant && step == 0) ev0 = static_cast<int8_t>(s_exp[slot][0][16 + (s_range[slot][0] & 255)]);
+      if (kQuant && ev0 == kNone)
+#pragma unroll
+        for (int u = kU - 1; u >= 0; --u)
+          if (const int seen = s_range[slot][u]; seen != 0) ev0 = static_cast<int8_t>(s_exp[slot][u][16 + (seen & 255)]);
 #pragma unroll
       for (int u = 0; u < kU; ++u) {
         float kf[2], vf[2];
+        bool far[2] = {false, false};
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
           const int8_t* x = reinterpret_cast<const int8_t*>(&s_exp[slot][u][r * 8 + tok]);
           kf[r] = kQuant ? exp2i(x[0]) : 1.f;
           vf[r] = kQuant ? __uint_as_float(0x4b400000u + x[16]) - 12582912.f : 0.f;  // the exponent as a float, off the conversion pipe
           back[u][r] = kQuant ? exp2i(-min(max(static_cast<int>(x[16]), -119), 119) - kSpan) : 1.f;  // finite in places not seen, too
-          if (kQuant) wide |= static_cast<uint32_t>(x[16] - ev0 + 44) > 88u;
+          if (kQuant) far[r] = static_cast<uint32_t>(x[16] - ev0 + 44) > 88u;
         }
         const int seen = s_range[slot][u];
 #pragma unroll
@@ -607,14 +612,16 @@ __global__ void __launch_bounds__(kWarps * 32, 2)
             if (kQuant) z = z * kf[j >> 1] + vf[j >> 1];
             s[u][nt][j] = z;
           }
-        if (seen != kTile << 8)
+        if (seen != kTile << 8)  // places not seen hold anything, exponents among it: they count nowhere
 #pragma unroll
-          for (int nt = 0; nt < kNT; ++nt)
+          for (int r = 0; r < 2; ++r) {
+            const int t = tok + r * 8;
+            if (t >= (seen & 255) && t < seen >> 8) continue;
+            far[r] = false;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              const int r = tok + (j >> 1) * 8;
-              if (r < (seen & 255) || r >= seen >> 8) s[u][nt][j] = -INFINITY;
-            }
+            for (int nt = 0; nt < kNT; ++nt) s[u][nt][2 * r] = s[u][nt][2 * r + 1] = -INFINITY;
+          }
+        wide |= far[0] || far[1];
       }
       __syncwarp();  // the unit is read
       ask(!(C::kRing & 1), step + C::kRing / 2, slot);

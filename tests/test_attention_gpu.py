@@ -454,3 +454,37 @@ def test_waits_that_run_out(dm3, dim, group, quant, rows, row_bytes):
         out, lse = cache.attend(0, q, lengths)
         assert torch.equal(out, want[0]) and torch.equal(lse, want[1])
     assert cache.check() == 0
+
+
+@pytest.mark.parametrize("dim", [64, 128, 192, 256])
+@pytest.mark.parametrize("group", [4, 16])
+@pytest.mark.parametrize("lengths,capacity,window", [([1, 17, 40, 100, 130], None, 0), ([90] * 150, 700, 0), ([90] * 150, 700, 21), ([3000, 77], 100000, 0),
+                                                     ([100, 60], None, 0)])
+def test_what_is_not_seen_decides_nothing(dm3, dim, group, lengths, capacity, window):
+    """Equal bits whatever the places behind a row's length, before its window, and of pages that it does not have hold, and whatever
+    earlier calls left in shared memory."""
+    d = paged(lengths, 1, dim, 16, True, dim + group, capacity=capacity)
+    if len(lengths) == 2 and lengths[0] == 100:
+        d["table"][:, 0] = -1  # the first tile has no page
+    hole = (d["k"].view(torch.uint8) == 0x7F).all(-1)
+    dev, q = to_cuda(d), _q(len(lengths), group, dim, 3).cuda()
+    if window:  # what the window leaves out
+        for r, n in enumerate(lengths):
+            for t in range(n - window):
+                hole[int(d["table"][r, t // 16]), 0, t % 16] = True
+    hole = hole.cuda()
+    other = dm3.KVCache(1, 200, 500, 1, dim, page_size=16, quantised=True)
+    other.table.random_(0, other.k.shape[1])
+    for x in (other.k_exp, other.v_exp):
+        x.random_(-110, 120)
+    lens = torch.full((200,), 500, device="cuda")
+    first = None
+    for e in (0, 3, 127, -128, -60, 0):
+        for name in ("k", "v"):
+            dev[name].view(torch.uint8)[hole] = 0x7F if e else 0x11
+            dev[name + "_exp"][hole] = e
+        if e:
+            other.attend(0, q[:1].expand(200, -1, -1), lens)
+        got = dm3.ops.paged_attention(q, *held(dev), dev["table"], dev["lengths"], dev["status"], None, window)
+        first = first or got
+        assert torch.equal(got[0], first[0]) and torch.equal(got[1], first[1]), e
