@@ -33,6 +33,12 @@
 // [2^14, 2^15), where fp16 holds a bf16 row to 2^-40 of its largest value; a weight is rounded once to 11 bits (2^-11 of
 // it at most, 1/8 of what rounding the output to bf16 costs). With a bf16 cache a weight goes to the tensor cores
 // as a bf16 pair, high and low part: 16 bits.
+//
+// l in terms of M can be anything from 2^-113 (one token at exponent 119) to 2^155 (2^31 tokens at -110, all just under the
+// slack), more than 32 bits hold. So a warp sums w_t * 2^(e - e_t), e the exponent of the first row that it sees, while no other is
+// more than 44 from it: then no term is over 2^58, and that of the largest logit not under 2^-38. From the first row that is,
+// it sums 2^(s_t + e_t - M) * 2^-e_t, formed from the logit, in 64 bits in shared memory, at a price that only such rows pay.
+// Warps, CTAs and parts are joined with a reference R of their sums beside M: sum exp = l 2^R, out = O 2^M / (l 2^R).
 #include <atomic>
 #include <cmath>
 #include <cstdint>
@@ -55,8 +61,11 @@ constexpr int kTile = 16;  // tokens of one tile; pages hold whole tiles
 // The maximum is raised only when a logit exceeds it by more than kSlack (log2): weights reach 2^kSlack. fp16
 // weights carry 2^kLift besides, so that they stay normal down to 2^-(14 + kLift).
 constexpr float kSlack = 8.f, kLift = 6.f;
-// With e4m3 rows l is held times 2^-kSpan: 2^-e_t reaches 2^110 there, and a sum of many has to stay finite.
-constexpr int kSpan = 7;
+// The exponents that a warp's 32-bit sum takes: within kNear of the first one's.
+constexpr int kNear = 44;
+struct Part {  // what a CTA leaves of a shared unit's head: maximum, sum and its reference
+  float m, l, r, none;
+};
 
 struct Params {
   const __nv_bfloat16* q;  // [rows][q_heads][dim]
@@ -74,8 +83,8 @@ struct Params {
   // stream: the first tile of each row in the sequence and their number ([rows + 1], a tile counted once a head unit),
   // and what a CTA leaves of the row that it starts in ([2 * cta]) and of the one that it ends in ([2 * cta + 1])
   int64_t* row_at;
-  float* part_o;    // [2 * ctas][heads of a unit][dim]
-  float2* part_ml;  // [2 * ctas][heads of a unit]
+  float* part_o;  // [2 * ctas][heads of a unit][dim]
+  Part* part_ml;  // [2 * ctas][heads of a unit]
 };
 
 // The tokens and tiles that a row sees.
@@ -173,7 +182,7 @@ struct Shape {
   static constexpr int kUnit = kU * kTileBytes;
   static constexpr int kQBytes = kNT * kDim * 16;  // 8 * kNT heads of kDim 16-bit values
   static constexpr int kSide = (kQuant ? kU * 32 : 0) + kU * 4 + 8 + 4;  // a unit's exponents, ranges and barrier
-  static constexpr int kStats = (2 * kWarps + 1 + kMaxCluster) * kHeads * 4;
+  static constexpr int kStats = (3 * kWarps + 1 + kMaxCluster) * kHeads * 4;
   // Two CTAs an SM: few warps with much to do at once did better than more of them with smaller steps and fewer
   // registers (96 ragged rows, 16 heads a cache head, e4m3: 74.6 us; three CTAs and half the step 80.6, four 88.6)
   static constexpr int kRoom = 112 * 1024 - kQBytes - kStats - 1024;  // 1024: aligning the ring
@@ -192,16 +201,27 @@ __device__ __forceinline__ int token_of(int lr) {
   return kBox == 128 ? ((lr ^ lr >> 2) & 1) << 2 | (lr & 2) | lr >> 2 : lr;
 }
 
-// l with its maximum raised from `from` to `to`: l * 2^(from - to), where the power alone may vanish, since maxima that l
-// refers to can lie 2^229 apart (see the exponents above). Before any logit l is 0, or NaN where all of them were.
+// l with its reference raised from `from` to `to`: l * 2^(from - to), where the power alone may vanish: those of e4m3 rows
+// can lie 229 further apart than the logits. Before any logit l is 0, or NaN where all of them were.
 __device__ __forceinline__ float raise_sum(float l, float from, float to) {
   const float h = from == -INFINITY ? 1.f : ex2(0.5f * (from - to));
   return l * h * h;
 }
-__device__ __forceinline__ float lse_of(float m, float l, bool quant) {  // natural log of the sum, from log2 units
-  return l == 0.f ? -INFINITY : (m + (quant ? kSpan - kLift : 0.f) + log2f(l)) * 0.69314718055994531f;
+__device__ __forceinline__ double raise_sum(double l, float from, float to) {
+  const float h = from == -INFINITY ? 1.f : ex2(0.25f * (from - to));
+  const double hh = static_cast<double>(h) * h;
+  return l * hh * hh;
 }
-__device__ __forceinline__ float inverse(float l, bool quant) { return l == 0.f ? 0.f : (quant ? 1.f / (1 << kSpan) : 1.f) / l; }
+__device__ __forceinline__ double exp2d(int e) { return __hiloint2double((1023 + e) << 20, 0); }
+__device__ __forceinline__ float lse_of(float r, float l) {  // natural log of the sum, from log2 units
+  return l == 0.f ? -INFINITY : (r + log2f(l)) * 0.69314718055994531f;
+}
+// What turns O into out, in two factors that stay in range where their product may not (2^-155 for 2^31 tokens at -110).
+__device__ __forceinline__ float2 scale_of(float m, float r, float l, bool quant) {
+  if (l == 0.f) return make_float2(0.f, 0.f);
+  const float h = quant ? ex2(0.5f * (m - kLift - r)) : 1.f;
+  return make_float2(1.f / l * h, h);
+}
 
 __device__ __forceinline__ bool elect_one() {  // true in one lane of the warp
   uint32_t r;
@@ -212,7 +232,7 @@ __device__ __forceinline__ bool elect_one() {  // true in one lane of the warp
 __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
-__device__ __forceinline__ uint32_t in_cta(const float* p, int rank) {  // the place of p in another CTA of the cluster
+__device__ __forceinline__ uint32_t in_cta(const void* p, int rank) {  // the place of p in another CTA of the cluster
   uint32_t r;
   asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_u32(p)), "r"(rank));
   return r;
@@ -222,10 +242,50 @@ __device__ __forceinline__ float ld_cluster(const float* p, int rank) {
   asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(in_cta(p, rank)) : "memory");
   return v;
 }
-__device__ __forceinline__ float2 ld_cluster2(const float* p, int rank) {
+__device__ __forceinline__ float2 ld_cluster2(const void* p, int rank) {
   float2 v;
   asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(in_cta(p, rank)) : "memory");
   return v;
+}
+
+template <typename T>
+__device__ __forceinline__ T lane_sum(T x) {  // over the lanes of a head
+#pragma unroll
+  for (int w = 4; w < 32; w *= 2) x += __shfl_xor_sync(0xffffffffu, x, w);
+  return x;
+}
+// The sums of a warp whose value rows' exponents lie far apart (kNear), a head's in its place of `sums`, referring to the
+// maximum in its place of `refers`: begun with what the lanes hold, and a step's logits (with exponents, s) added. Out of the
+// kernel's body, where the few calls that come here would cost every other one instructions to fetch (48 ragged e4m3 rows, 12
+// heads of 192 a cache head: 46.9 us inlined, 45.9 so).
+struct WideSums {
+  double* sums;
+  float* refers;
+};
+template <int kNT>
+__device__ __noinline__ void begin_wide(WideSums to, const float (*l)[2], const float (*m)[2], int e) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int i = 0; i < 2 * kNT; ++i) {
+    const float t = lane_sum(l[i / 2][i % 2]);
+    const int head = i / 2 * 8 + 2 * (lane & 3) + i % 2;
+    if (lane < 4) to.sums[head] = t * exp2d(-e), to.refers[head] = m[i / 2][i % 2];
+  }
+}
+template <int kU, int kNT>
+__device__ __noinline__ void add_wide(WideSums to, const float (*s)[kNT][4], const int (*ev)[2], const float (*m)[2], const float (*sub)[2]) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int i = 0; i < 2 * kNT; ++i) {
+    const int nt = i / 2, h = i % 2, head = nt * 8 + 2 * (lane & 3) + h;
+    float t = 0.f;  // times 2^-4: up to 128 terms of 2^124; the largest logit's, 2^-113 at least, keeps 32 bits under it
+#pragma unroll
+    for (int u = 0; u < kU; ++u)
+#pragma unroll
+      for (int r = 0; r < 2; ++r) t += ex2_all(s[u][nt][2 * r + h] - sub[nt][h] - static_cast<float>(ev[u][r] + 4));
+    t = lane_sum(t);
+    if (lane < 4) to.sums[head] = raise_sum(to.sums[head], to.refers[head], m[nt][h]) + 16. * t, to.refers[head] = m[nt][h];
+  }
 }
 
 // The row with the nth most tiles, of 128 rows at most (the nth one where all are short). All threads call it; scratch: 129
@@ -351,8 +411,10 @@ __global__ void __launch_bounds__(kWarps * 32, 2)
   int(*const s_range)[kU] = reinterpret_cast<int(*)[kU]>(side) + warp * C::kRing;  // rows of a tile that are seen: from | to << 8
   side += kWarps * C::kRing * kU * 4;
   float(*const s_m)[C::kHeads] = reinterpret_cast<float(*)[C::kHeads]>(side);
-  float(*const s_l)[C::kHeads] = s_m + kWarps;
-  float* const s_qs = s_m[2 * kWarps];
+  float2(*const s_l)[C::kHeads] = reinterpret_cast<float2(*)[C::kHeads]>(s_m + kWarps);    // sum and reference
+  double(*const s_wide)[C::kHeads] = reinterpret_cast<double(*)[C::kHeads]>(s_m + kWarps);  // in their place until the join
+  float(*const s_f)[C::kHeads] = reinterpret_cast<float(*)[C::kHeads]>(s_l + kWarps);       // [kMaxCluster]
+  float* const s_qs = s_f[kMaxCluster];
   if (lane == 0) {
 #pragma unroll
     for (int i = 0; i < C::kRing; ++i) mbar_init(&full[i], 1);
@@ -510,7 +572,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2)
 
     constexpr int kNone = 1 << 20;
     int ev0 = kNone;    // the exponent of the first value row seen
-    bool wide = false;  // a later one is more than 44 away
+    bool wide = false;  // a later one is more than kNear away: from then on l is in s_wide
 
     auto next_slot = [&] {
       if (++slot == C::kRing) slot = 0, parity ^= 1;
@@ -586,7 +648,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2)
             for (int i = 1; i < kChains; ++i) s[u][nt][j] += part[i][u][nt][j];
           }
       // logits in log2 units (with the value rows' exponents), -inf where nothing is seen
-      float back[kU][2];  // 2^-(exponent + kSpan)
+      int ev[kU][2];  // exponents of the value rows, ev0 in places not seen
       if (kQuant && ev0 == kNone)
 #pragma unroll
         for (int u = kU - 1; u >= 0; --u)
@@ -594,14 +656,12 @@ __global__ void __launch_bounds__(kWarps * 32, 2)
 #pragma unroll
       for (int u = 0; u < kU; ++u) {
         float kf[2], vf[2];
-        bool far[2] = {false, false};
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
           const int8_t* x = reinterpret_cast<const int8_t*>(&s_exp[slot][u][r * 8 + tok]);
           kf[r] = kQuant ? exp2i(x[0]) : 1.f;
           vf[r] = kQuant ? __uint_as_float(0x4b400000u + x[16]) - 12582912.f : 0.f;  // the exponent as a float, off the conversion pipe
-          back[u][r] = kQuant ? exp2i(-min(max(static_cast<int>(x[16]), -119), 119) - kSpan) : 1.f;  // finite in places not seen, too
-          if (kQuant) far[r] = static_cast<uint32_t>(x[16] - ev0 + 44) > 88u;
+          ev[u][r] = kQuant ? x[16] : 0;
         }
         const int seen = s_range[slot][u];
 #pragma unroll
@@ -617,19 +677,30 @@ __global__ void __launch_bounds__(kWarps * 32, 2)
           for (int r = 0; r < 2; ++r) {
             const int t = tok + r * 8;
             if (t >= (seen & 255) && t < seen >> 8) continue;
-            far[r] = false;
+            ev[u][r] = ev0;
 #pragma unroll
             for (int nt = 0; nt < kNT; ++nt) s[u][nt][2 * r] = s[u][nt][2 * r + 1] = -INFINITY;
           }
-        wide |= far[0] || far[1];
       }
       __syncwarp();  // the unit is read
       ask(!(C::kRing & 1), step + C::kRing / 2, slot);
       next_slot();
 
-      // Weights of rows whose exponents lie far apart can vanish where their share of l does not: from then on l takes its
-      // terms from the logits themselves.
-      if (kQuant) wide = __any_sync(0xffffffffu, wide);
+      if constexpr (kQuant) {
+        bool far = false;
+#pragma unroll
+        for (int u = 0; u < kU; ++u)
+#pragma unroll
+          for (int r = 0; r < 2; ++r) far |= static_cast<uint32_t>(ev[u][r] - ev0 + kNear) > 2u * kNear;
+        if (__builtin_expect(__any_sync(0xffffffffu, far && !wide), 0)) {
+          wide = true;
+          // before the maximum is raised, maybe by more than 32 bits hold
+          float l_now[kNT][2], m_now[kNT][2];
+#pragma unroll
+          for (int i = 0; i < 2 * kNT; ++i) l_now[i / 2][i % 2] = l[i / 2][i % 2], m_now[i / 2][i % 2] = m[i / 2][i % 2];
+          begin_wide<kNT>({s_wide[warp], s_m[warp]}, l_now, m_now, ev0);
+        }
+      }
       bool above = false;
 #pragma unroll
       for (int nt = 0; nt < kNT; ++nt)
@@ -658,30 +729,34 @@ __global__ void __launch_bounds__(kWarps * 32, 2)
             for (int i = 0; i < kDim / 16; ++i) o[nt][i][h] *= f, o[nt][i][2 + h] *= f;
           }
       }
-      if (kQuant && wide) {
+      if constexpr (kQuant)
+        if (__builtin_expect(wide, 0)) {
+          float s_now[kU][kNT][4], m_now[kNT][2], sub_now[kNT][2];
+          int ev_now[kU][2];
 #pragma unroll
-        for (int u = 0; u < kU; ++u)
+          for (int u = 0; u < kU; ++u) {
 #pragma unroll
-          for (int r = 0; r < 2; ++r) {
-            const float shift = static_cast<float>(static_cast<int>(__float_as_uint(back[u][r]) >> 23) - 127);
-            back[u][r] = 0.f;
-#pragma unroll
-            for (int nt = 0; nt < kNT; ++nt)
-#pragma unroll
-              for (int h = 0; h < 2; ++h) l[nt][h] += ex2_all(s[u][nt][2 * r + h] - sub[nt][h] + shift);
+            for (int i = 0; i < 4 * kNT; ++i) s_now[u][i / 4][i % 4] = s[u][i / 4][i % 4];
+            ev_now[u][0] = ev[u][0], ev_now[u][1] = ev[u][1];
           }
-      }
+#pragma unroll
+          for (int i = 0; i < 2 * kNT; ++i) m_now[i / 2][i % 2] = m[i / 2][i % 2], sub_now[i / 2][i % 2] = sub[i / 2][i % 2];
+          add_wide<kU, kNT>({s_wide[warp], s_m[warp]}, s_now, ev_now, m_now, sub_now);
+        }
       // weights, as the second product's B operands
       uint32_t ph[kU][kNT][2], pl[kU][kNT][2];
 #pragma unroll
-      for (int u = 0; u < kU; ++u)
+      for (int u = 0; u < kU; ++u) {
+        float back[2];
+#pragma unroll
+        for (int r = 0; r < 2; ++r) back[r] = kQuant && !wide ? exp2i(ev0 - ev[u][r]) : 0.f;
 #pragma unroll
         for (int nt = 0; nt < kNT; ++nt) {
           float w[4];
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             w[j] = ex2(s[u][nt][j] - sub[nt][j & 1]);
-            l[nt][j & 1] += kQuant ? w[j] * back[u][j >> 1] : w[j];
+            l[nt][j & 1] += kQuant ? w[j] * back[j >> 1] : w[j];
           }
 #pragma unroll
           for (int r = 0; r < 2; ++r) {
@@ -696,6 +771,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2)
             }
           }
         }
+      }
 
       if (!landed()) {
         stuck = 2 * step + 1;
@@ -780,28 +856,38 @@ __global__ void __launch_bounds__(kWarps * 32, 2)
       for (int h = 0; h < 2; ++h) {
 #pragma unroll
         for (int w = 4; w < 32; w *= 2) l[nt][h] += __shfl_xor_sync(0xffffffffu, l[nt][h], w);
-        if (lr == 0) s_m[warp][nt * 8 + 2 * lc + h] = m[nt][h], s_l[warp][nt * 8 + 2 * lc + h] = l[nt][h];
+        if (lr == 0) {
+          const int head = nt * 8 + 2 * lc + h;
+          s_m[warp][head] = m[nt][h];
+          float2 sum = make_float2(l[nt][h], kQuant && ev0 != kNone ? m[nt][h] - kLift - ev0 : m[nt][h]);
+          if (kQuant && wide) {  // the reference takes the 64 bits' exponent
+            const double t = s_wide[warp][head];
+            const int e = max((__double2hiint(t) >> 20) - 1023, -1000);
+            sum = make_float2(static_cast<float>(t * exp2d(-e)), m[nt][h] - kLift + e);
+          }
+          s_l[warp][head] = sum;
+        }
       }
     __syncthreads();
     const bool whole = p.splits ? p.splits == 1 : begin == 0 && end == sp.tiles;
     const int64_t to = 2 * static_cast<int64_t>(blockIdx.x) + (part ? 1 : 0);  // stream: where a shared row's part goes
-    if (threadIdx.x < C::kHeads) {  // each warp's factor into s_m, the joined sum and maximum into s_l[0], s_l[1]
+    if (threadIdx.x < C::kHeads) {  // each warp's factor into s_m, the joined sum into s_l[0], maximum into [1], out's scale into [2]
       const int h = threadIdx.x;
-      float mm = -INFINITY, ll = 0.f;
+      float mm = -INFINITY, rr = -INFINITY, ll = 0.f;
 #pragma unroll
-      for (int w = 0; w < kWarps; ++w) mm = fmaxf(mm, s_m[w][h]);
+      for (int w = 0; w < kWarps; ++w) mm = fmaxf(mm, s_m[w][h]), rr = fmaxf(rr, s_l[w][h].y);
 #pragma unroll
       for (int w = 0; w < kWarps; ++w) {
         const float f = s_m[w][h] == -INFINITY ? 0.f : ex2(s_m[w][h] - mm);
-        ll += raise_sum(s_l[w][h], s_m[w][h], mm);
+        ll += raise_sum(s_l[w][h].x, s_l[w][h].y, rr);
         s_m[w][h] = f;
       }
-      s_l[0][h] = ll, s_l[1][h] = mm;
-      s_qs[h] = whole ? inverse(ll, kQuant) : 1.f;
+      s_l[0][h] = make_float2(ll, rr), s_l[1][h].x = mm;
       if (whole) {
-        if (h0 + h < p.group) p.lse[qrow + h] = lse_of(mm, ll, kQuant);
+        s_l[2][h] = scale_of(mm, rr, ll, kQuant);
+        if (h0 + h < p.group) p.lse[qrow + h] = lse_of(rr, ll);
       } else if (!p.splits) {
-        p.part_ml[to * C::kHeads + h] = make_float2(mm, ll);
+        p.part_ml[to * C::kHeads + h] = {mm, ll, rr, 0.f};
       }
     }
     // (value d of both heads of a pair) at d with its low bits turned by lr, so that neither these writes (lanes kE
@@ -818,6 +904,9 @@ __global__ void __launch_bounds__(kWarps * 32, 2)
     __syncthreads();
     auto place = [&](int d) { return (d ^ (d / C::kE & 3)) * 2; };
     auto put = [&](int h, int d, float x, float y) {
+      const float4 by = *reinterpret_cast<const float4*>(&s_l[2][h]);
+      x *= by.x, y *= by.z;
+      if (kQuant) x *= by.y, y *= by.w;
       if (h0 + h < p.group) p.out[(qrow + h) * kDim + d] = __float2bfloat16_rn(x);
       if (h0 + h + 1 < p.group) p.out[(qrow + h + 1) * kDim + d] = __float2bfloat16_rn(y);
     };
@@ -830,7 +919,6 @@ __global__ void __launch_bounds__(kWarps * 32, 2)
         const float2 f = *reinterpret_cast<const float2*>(&s_m[w][h]);
         x += v.x * f.x, y += v.y * f.y;
       }
-      x *= s_qs[h], y *= s_qs[h + 1];
       if (whole) {
         put(h, d, x, y);
       } else if (p.splits) {
@@ -844,22 +932,27 @@ __global__ void __launch_bounds__(kWarps * 32, 2)
       if (p.splits == 1) return;
       // every CTA of the cluster joins its part of the values
       const int rank = blockIdx.x;
-      float(*const s_f)[C::kHeads] = s_m + 2 * kWarps + 1;  // [splits]
       cluster_sync();
+      // (maximum, sum, reference) of every CTA's heads, fetched at once, one a thread, into a place of the ring that is free now
+      float4(*const s_all)[C::kHeads] = reinterpret_cast<float4(*)[C::kHeads]>(s_o[1]);
+      static_assert(kMaxCluster * C::kHeads <= kWarps * 32 && kMaxCluster * C::kHeads * 16 <= sizeof(s_o[1]));
+      if (const int i = threadIdx.x; i < p.splits * C::kHeads) {
+        const int r = i / C::kHeads, h = i % C::kHeads;
+        const float2 sum = ld_cluster2(&s_l[0][h], r);
+        s_all[r][h] = make_float4(ld_cluster(&s_l[1][h].x, r), sum.x, sum.y, 0.f);
+      }
+      __syncthreads();
       if (threadIdx.x < C::kHeads) {
         const int h = threadIdx.x;
-        float mm = -INFINITY, ll = 0.f;
+        float mm = -INFINITY, rr = -INFINITY, ll = 0.f;
+        for (int r = 0; r < p.splits; ++r) mm = fmaxf(mm, s_all[r][h].x), rr = fmaxf(rr, s_all[r][h].z);
         for (int r = 0; r < p.splits; ++r) {
-          s_f[r][h] = ld_cluster(&s_l[1][h], r);
-          mm = fmaxf(mm, s_f[r][h]);
+          const float4 part = s_all[r][h];
+          ll += raise_sum(part.y, part.z, rr);
+          s_f[r][h] = part.x == -INFINITY ? 0.f : ex2(part.x - mm);
         }
-        for (int r = 0; r < p.splits; ++r) {
-          const float f = s_f[r][h] == -INFINITY ? 0.f : ex2(s_f[r][h] - mm);
-          ll += raise_sum(ld_cluster(&s_l[0][h], r), s_f[r][h], mm);
-          s_f[r][h] = f;
-        }
-        s_qs[h] = inverse(ll, kQuant);
-        if (rank == 0 && h0 + h < p.group) p.lse[qrow + h] = lse_of(mm, ll, kQuant);
+        s_l[2][h] = scale_of(mm, rr, ll, kQuant);
+        if (rank == 0 && h0 + h < p.group) p.lse[qrow + h] = lse_of(rr, ll);
       }
       __syncthreads();
       for (int i = rank * blockDim.x + threadIdx.x; i < C::kHeads / 2 * kDim; i += p.splits * blockDim.x) {
@@ -870,7 +963,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2)
           const float2 v = ld_cluster2(&s_o[0][hp][place(d)], r);
           x += v.x * s_f[r][h], y += v.y * s_f[r][h + 1];
         }
-        put(h, d, x * s_qs[h], y * s_qs[h + 1]);
+        put(h, d, x, y);
       }
       cluster_sync();  // no CTA leaves while another reads its shared memory
       return;
@@ -888,8 +981,8 @@ __global__ void __launch_bounds__(kWarps * 32, 2)
 // Joins the parts of a shared row's unit: blockIdx = (row and unit, slice of its heads' values). A thread holds 4 values;
 // `groups` threads take their parts in turn, each with a running maximum of its own, and meet in shared memory.
 constexpr int kJoinThreads = 256, kJoinBatch = 4;
-__global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constant__ Params p, int dim, int ctas, int heads, int groups, bool quant) {
-  __shared__ float s_m[kJoinThreads], s_l[kJoinThreads];
+__global__ void __launch_bounds__(kJoinThreads, 4) join_kernel(const __grid_constant__ Params p, int dim, int ctas, int heads, int groups, bool quant) {
+  __shared__ float s_m[kJoinThreads], s_l[kJoinThreads], s_r[kJoinThreads];
   __shared__ float4 s_x[kJoinThreads];
   griddep_launch();
   griddep_wait();
@@ -901,56 +994,57 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constan
   const int per = kJoinThreads / groups, g = threadIdx.x / per, i4 = blockIdx.y * per + threadIdx.x % per;
   const int h = i4 * 4 / dim, in_group = unit % p.head_tiles * heads + h;
   const bool on = h < heads && in_group < p.group;
-  const float2* const ml = p.part_ml + 2 * first * heads + h;
+  const float4* const ml = reinterpret_cast<const float4*>(p.part_ml + 2 * first * heads + h);
   const float4* const po = reinterpret_cast<const float4*>(p.part_o + 2 * first * heads * dim) + i4;
-  float m = -INFINITY, l = 0.f;
+  float m = -INFINITY, l = 0.f, r = -INFINITY;
   float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
   for (int i0 = g; i0 < n && on; i0 += groups * kJoinBatch) {
-    float2 a[kJoinBatch];
+    float4 a[kJoinBatch];  // parts
     float4 y[kJoinBatch];
 #pragma unroll
     for (int b = 0; b < kJoinBatch; ++b) {
       const int i = i0 + b * groups, slot = 2 * i + (i == 0 ? skip : 0);
-      a[b] = i < n ? ml[slot * heads] : make_float2(-INFINITY, 0.f);
+      a[b] = i < n ? ml[slot * heads] : make_float4(-INFINITY, 0.f, -INFINITY, 0.f);
       y[b] = i < n ? po[slot * (heads * dim / 4)] : make_float4(0.f, 0.f, 0.f, 0.f);
     }
-    float mm = m;
+    float mm = m, rr = r;
 #pragma unroll
-    for (int b = 0; b < kJoinBatch; ++b) mm = fmaxf(mm, a[b].x);
+    for (int b = 0; b < kJoinBatch; ++b) mm = fmaxf(mm, a[b].x), rr = fmaxf(rr, a[b].z);
     const float back = m == -INFINITY ? 0.f : ex2(m - mm);
-    l = raise_sum(l, m, mm);
+    l = raise_sum(l, r, rr);
     x.x *= back, x.y *= back, x.z *= back, x.w *= back;
 #pragma unroll
     for (int b = 0; b < kJoinBatch; ++b) {
       const float f = a[b].x == -INFINITY ? 0.f : ex2(a[b].x - mm);
-      l += raise_sum(a[b].y, a[b].x, mm);
+      l += raise_sum(a[b].y, a[b].z, rr);
       x.x += y[b].x * f, x.y += y[b].y * f, x.z += y[b].z * f, x.w += y[b].w * f;
     }
-    m = mm;
+    m = mm, r = rr;
   }
   if (groups > 1) {
-    s_m[threadIdx.x] = m, s_l[threadIdx.x] = l, s_x[threadIdx.x] = x;
+    s_m[threadIdx.x] = m, s_l[threadIdx.x] = l, s_r[threadIdx.x] = r, s_x[threadIdx.x] = x;
     __syncthreads();
     if (g) return;
-    float mm = m;
-    for (int i = 1; i < groups; ++i) mm = fmaxf(mm, s_m[i * per + threadIdx.x]);
+    float mm = m, rr = r;
+    for (int i = 1; i < groups; ++i) mm = fmaxf(mm, s_m[i * per + threadIdx.x]), rr = fmaxf(rr, s_r[i * per + threadIdx.x]);
     const float f0 = m == -INFINITY ? 0.f : ex2(m - mm);
-    l = raise_sum(l, m, mm);
+    l = raise_sum(l, r, rr);
     x.x *= f0, x.y *= f0, x.z *= f0, x.w *= f0;
     for (int i = 1; i < groups; ++i) {
       const float mi = s_m[i * per + threadIdx.x], f = mi == -INFINITY ? 0.f : ex2(mi - mm);
       const float4 y = s_x[i * per + threadIdx.x];
-      l += raise_sum(s_l[i * per + threadIdx.x], mi, mm);
+      l += raise_sum(s_l[i * per + threadIdx.x], s_r[i * per + threadIdx.x], rr);
       x.x += y.x * f, x.y += y.y * f, x.z += y.z * f, x.w += y.w * f;
     }
-    m = mm;
+    m = mm, r = rr;
   }
   if (!on) return;
   const int64_t head = static_cast<int64_t>(row) * p.q_heads + unit / p.head_tiles * p.group + in_group;
-  const float inv = inverse(l, quant);
+  const float2 scale = scale_of(m, r, l, quant);
+  auto value = [scale](float v) { return v * scale.x * scale.y; };
   const int d = i4 * 4 - h * dim;
-  *reinterpret_cast<uint2*>(p.out + head * dim + d) = make_uint2(pack_bf16(x.x * inv, x.y * inv), pack_bf16(x.z * inv, x.w * inv));
-  if (d == 0) p.lse[head] = lse_of(m, l, quant);
+  *reinterpret_cast<uint2*>(p.out + head * dim + d) = make_uint2(pack_bf16(value(x.x), value(x.y)), pack_bf16(value(x.z), value(x.w)));
+  if (d == 0) p.lse[head] = lse_of(r, l);
 }
 
 // ------------------------------------------------------------------ host side
@@ -1003,7 +1097,7 @@ static Plan plan(int rows, int q_heads, int kv_heads, int dim, int page_size, in
 static size_t part_bytes(const Plan& r, int rows, int q_heads, int kv_heads, int dim) {
   if (r.splits) return 0;
   const size_t heads = tile_heads(q_heads / kv_heads);
-  return 2 * static_cast<size_t>(r.ctas) * heads * (dim * sizeof(float) + sizeof(float2)) + (static_cast<size_t>(rows) + 1) * sizeof(int64_t);
+  return 2 * static_cast<size_t>(r.ctas) * heads * (dim * sizeof(float) + sizeof(Part)) + (static_cast<size_t>(rows) + 1) * sizeof(int64_t);
 }
 
 template <typename... A>
@@ -1113,7 +1207,7 @@ extern "C" int dm3_paged_attention(const void* q, int64_t q_rs, int64_t q_hs, in
     if (workspace_bytes < attn::part_bytes(plan, rows, q_heads, kv_heads, dim)) return set_error("workspace too small"), DM3_ENOSPACE;
     if (!workspace || reinterpret_cast<uintptr_t>(workspace) % 256) return set_error("workspace must be 256-byte aligned"), DM3_EINVAL;
     p.part_o = static_cast<float*>(workspace);
-    p.part_ml = reinterpret_cast<float2*>(p.part_o + 2 * static_cast<int64_t>(plan.ctas) * heads * dim);
+    p.part_ml = reinterpret_cast<attn::Part*>(p.part_o + 2 * static_cast<int64_t>(plan.ctas) * heads * dim);
     p.row_at = reinterpret_cast<int64_t*>(p.part_ml + 2 * static_cast<int64_t>(plan.ctas) * heads);
   }
   const dim3 grid = plan.splits ? dim3(plan.splits, kv_heads * plan.head_tiles, rows) : dim3(plan.ctas);

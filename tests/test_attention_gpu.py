@@ -488,3 +488,35 @@ def test_what_is_not_seen_decides_nothing(dm3, dim, group, lengths, capacity, wi
         got = dm3.ops.paged_attention(q, *held(dev), dev["table"], dev["lengths"], dev["status"], None, window)
         first = first or got
         assert torch.equal(got[0], first[0]) and torch.equal(got[1], first[1]), e
+
+
+@pytest.mark.parametrize("tokens,rows,capacity", [(2500, 1, 0), (8000, 300, 0), (5000, 3, 200000), (600000, 1, 0)])
+@pytest.mark.parametrize("low,high", [(-110, -110), (-110, 119), (119, 119), (-110, -60)])
+@pytest.mark.parametrize("group", [2, 16])
+def test_sums_at_the_ends_of_the_exponents(dm3, tokens, rows, capacity, low, high, group):
+    """Many tokens whose logits lie just under what raises the maximum (2^8 in units of log2) above the first one's, over value rows with
+    exponents at either end: a term of the sum is 2^(14 - exponent), 2^124 at -110, and thousands of them are added."""
+    dim, size = 64, 16
+    g = torch.Generator().manual_seed(tokens + high)
+    pages = 40
+    k, ke = torch.zeros(pages, 1, size, dim), torch.zeros(pages, 1, size, dtype=torch.int8)
+    k[1:, :, :, 0], ke[1:] = 352.0, -6  # 352 * 2^-6 = 5.5 = 7.93 ln 2; page 0's logits are 0
+    d = {"k": k.to(torch.float8_e4m3fn), "k_exp": ke, "status": torch.zeros(1, dtype=torch.int32)}
+    d["v"] = (torch.randn(pages, 1, size, dim, generator=g) * 100).clamp(-448, 448).to(torch.float8_e4m3fn)
+    pick = torch.rand(pages, 1, size, generator=g) < 0.9
+    pick[0] = True
+    e = torch.where(pick, low, high)
+    per_row = -(-max(tokens, capacity) // size)
+    table = torch.randint(1, pages, (rows, per_row), generator=g, dtype=torch.int32)
+    table[:, :40] = 0  # the first steps of the warps
+    d["table"], d["lengths"] = table, torch.full((rows,), tokens, dtype=torch.int64)
+    q = torch.zeros(rows, group, dim)
+    q[:, :, 0] = 1.0
+    q = q.to(BF)
+    d["v_exp"] = e.to(torch.int8)
+    out, lse = _run(dm3, d, q, 1.0)
+    assert out.isfinite().all() and lse.isfinite().all()
+    # rows are alike: a few of them against the oracle, the values brought near 1
+    d["v_exp"] = (e - max(low, high)).clamp(min=-128).to(torch.int8)
+    few = {**d, "table": table[:2], "lengths": d["lengths"][:2]}
+    check_attention(out[:2].double() * 2.0 ** -max(low, high), lse[:2], few, q[:2], 1.0)
