@@ -147,6 +147,8 @@ class KVCache:
                max_tokens: Optional[int] = None) -> Tuple[Tensor, Tensor]:
         """One new token's attention a row: (out, lse), see `ops.paged_attention`. max_tokens: no row is longer
         (one of a few bucket sizes, as the engine's graphs have, engine.py:412-415)."""
+        if max_tokens is not None and max_tokens < 0:
+            raise ValueError("max_tokens must not be negative")
         table = self.table if max_tokens is None else self.table[:, :-(-max_tokens // self.page_size)]
         return ops.paged_attention(q, *self.layer(layer), table, lengths, self.status, scale, window)
 

@@ -311,3 +311,16 @@ def test_every_gradient_is_refused(stub, name):
             fn(*args[:at], forward.make_dual(args[at], torch.ones_like(args[at])), *args[at + 1:])
         with pytest.raises(RuntimeError, match="gradient"):
             torch.func.jvp(lambda x: fn(*args[:at], x, *args[at + 1:]), (args[at],), (torch.ones_like(args[at]),))
+
+
+def test_a_negative_bound_is_refused(dm3, stub):
+    """attend's max_tokens narrows the table; a negative one would count its columns from the end."""
+    c = dm3.KVCache(1, 2, 200, 1, 64, page_size=16, device="cpu")
+    q, n = torch.zeros(2, 4, 64, dtype=BF), torch.zeros(2, dtype=torch.int64)
+    for bad in (-1, -15, -16, -100):
+        with pytest.raises(ValueError, match="max_tokens"):
+            c.attend(0, q, n, max_tokens=bad)
+    assert stub[1] == []
+    for fine in (None, 0, 1, 200, 5000):
+        c.attend(0, q, n, max_tokens=fine)
+    assert len(stub[1]) == 5
