@@ -609,14 +609,31 @@ def _angles(inv_freq: Tensor) -> Tensor:
     return inv_freq.contiguous()
 
 
+def _page_stride(a: Tensor, b: Tensor, page: tuple) -> Optional[int]:
+    """The elements from one page to the next of two buffers alike, whose other strides have to be `page`; None where
+    they are not. Strides of a side of one mean nothing."""
+    strides = a.stride()
+    if strides[1:] == page and strides == b.stride() and a.shape[0] != 1:
+        return strides[0]
+    heads = a.shape[1]
+    for t in (a, b):
+        got = t.stride()
+        if got[2:] != page[1:] or (heads != 1 and got[1] != page[0]):
+            return None
+    if a.shape[0] == 1:
+        return heads * page[0]
+    return a.stride(0) if a.stride(0) == b.stride(0) else None
+
+
 def _cache_args(k_cache: Tensor, v_cache: Tensor, k_exp: Optional[Tensor], v_exp: Optional[Tensor], table: Tensor,
                 status: Tensor):
     """((k, v, page stride, k_exp, v_exp, exp stride), (pages, page_size), (kv_heads, dim), table arguments)."""
-    shape, strides = k_cache.shape, k_cache.stride()
+    shape = k_cache.shape
     if len(shape) != 4 or shape != v_cache.shape or k_cache.dtype != v_cache.dtype:
         raise RuntimeError("the cache must be two [pages, kv_heads, page_size, dim] buffers of one type")
     pages, heads, size, dim = shape
-    if strides != v_cache.stride() or strides[1:] != (size * dim, dim, 1):
+    stride = _page_stride(k_cache, v_cache, (size * dim, dim, 1))
+    if stride is None:
         raise RuntimeError("each page of the cache must be contiguous, with the same strides for keys and values")
     k_at = v_at = 0
     exp_stride = 0
@@ -627,11 +644,11 @@ def _cache_args(k_cache: Tensor, v_cache: Tensor, k_exp: Optional[Tensor], v_exp
         if k_exp is None or v_exp is None or k_cache.dtype not in (E4M3, torch.uint8):
             raise RuntimeError("a quantised cache is float8_e4m3fn (or uint8) with exponents for keys and values")
         for e in (k_exp, v_exp):
-            if e.dtype != torch.int8 or e.shape != shape[:3] or e.stride()[1:] != (size, 1):
-                raise RuntimeError("exponents must be int8 [pages, kv_heads, page_size], each page contiguous")
-        exp_stride = k_exp.stride(0)
-        if exp_stride != v_exp.stride(0):
-            raise RuntimeError("key and value exponents must have the same strides")
+            if e.dtype != torch.int8 or e.shape != shape[:3]:
+                raise RuntimeError("exponents must be int8 [pages, kv_heads, page_size]")
+        exp_stride = _page_stride(k_exp, v_exp, (size, 1))
+        if exp_stride is None:
+            raise RuntimeError("each page of the exponents must be contiguous, with the same strides for keys and values")
         k_at, v_at = k_exp.data_ptr(), v_exp.data_ptr()
     if table.dtype != torch.int32 or table.dim() != 2:
         raise RuntimeError("the page table must be int32 [rows, pages a row] with unit column stride")
@@ -643,7 +660,7 @@ def _cache_args(k_cache: Tensor, v_cache: Tensor, k_exp: Optional[Tensor], v_exp
         raise RuntimeError("the page table must be int32 [rows, pages a row] with unit column stride")
     if status.dtype != torch.int32 or status.numel() != 1:
         raise RuntimeError("status must be one int32")
-    return ((k_cache.data_ptr(), v_cache.data_ptr(), strides[0], k_at, v_at, exp_stride), (pages, size), (heads, dim),
+    return ((k_cache.data_ptr(), v_cache.data_ptr(), stride, k_at, v_at, exp_stride), (pages, size), (heads, dim),
             (table.data_ptr(), step if rows > 1 else per_row, rows, per_row))
 
 

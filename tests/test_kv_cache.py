@@ -324,3 +324,37 @@ def test_a_negative_bound_is_refused(dm3, stub):
     for fine in (None, 0, 1, 200, 5000):
         c.attend(0, q, n, max_tokens=fine)
     assert len(stub[1]) == 5
+
+
+@pytest.mark.parametrize("quant", [False, True])
+def test_strides_of_sides_of_one(dm3, stub, monkeypatch, quant):
+    """A contiguous page is taken whatever the strides of its sides of one are, and so are the strides of a single page."""
+    ops, _ = stub
+    got = []
+    monkeypatch.setattr(ops, "_launch", lambda device, name, *a: got.append((name, a)))
+    dtype = torch.float8_e4m3fn if quant else BF
+    t, s, n = torch.zeros(2, 3, dtype=torch.int32), torch.zeros(1, dtype=torch.int32), torch.zeros(2, dtype=torch.int64)
+    q = torch.zeros(2, 4, 64, dtype=BF)
+    for pages in (1, 5):
+        # one head: [pages, tokens, heads, dim] seen as [pages, heads, tokens, dim]
+        flat = [torch.zeros(pages, 16, 1, 64).to(dtype).transpose(1, 2) for _ in range(2)]
+        exps = [torch.zeros(pages, 16, 1, dtype=torch.int8).transpose(1, 2) if quant else None for _ in range(2)]
+        odd = [torch.as_strided(x, x.shape, (x.stride(0), 7, *x.stride()[2:])) for x in flat]
+        alone = [torch.as_strided(x, x.shape, (3 if pages == 1 else x.stride(0), *x.stride()[1:])) for x in flat]
+        mixed = [flat[0], odd[1]]
+        for c in (flat, odd, alone, mixed):
+            ops.kv_write(q[:, :1], q[:, :1], n, t, *c, *exps, s)
+            ops.kv_read(*c, *exps, t, n, 4, s)
+            ops.paged_attention(q, *c, *exps, t, n, s)
+    assert len(got) == 24
+    # what the entries are told: pages of 16 tokens of one head
+    for name, a in got:
+        assert 16 * 64 in a and (not quant or 16 in a), (name, a)
+    two = [torch.zeros(5, 2, 16, 64).to(dtype) for _ in range(2)]
+    ex = [torch.zeros(5, 2, 16, dtype=torch.int8) if quant else None for _ in range(2)]
+    wrong = [x.transpose(1, 2).contiguous().transpose(1, 2) for x in two]
+    for c, e in ((wrong, ex), (two, [None if x is None else x.transpose(1, 2).contiguous().transpose(1, 2) for x in ex])):
+        if c is two and not quant:
+            continue
+        with pytest.raises(RuntimeError, match="contiguous"):
+            ops.kv_read(*c, *e, t, n, 4, s)
