@@ -3,7 +3,8 @@
 //   s_t = scale * q . k_t,  p = softmax(s) over the tokens seen,  out = sum_t p_t v_t,
 //   lse = log sum_t exp(s_t),  seen: max(0, n - window) <= t < n (window 0: all), n the row's length
 //
-// One pass with a running maximum M and sum l; a row that sees nothing gives zeros and lse = -inf.
+// One pass with a running maximum M and sum l; a row that sees nothing gives zeros and lse = -inf. A logit of -inf is a token
+// that is not seen (its weight is 0); one of +inf or NaN makes l, and with it out and lse, NaN.
 //
 // Bound: the bytes of the cache's rows, each used by the group of query heads that shares them (2 * group flops a byte
 // and less), so the kernel is laid out to keep copies in flight and to spend few instructions a row, not for the
@@ -25,14 +26,14 @@
 //   * Clusters: the `splits` CTAs of a cluster (1 to 8) share a unit's tiles and join over distributed shared memory: one
 //     launch, for short rows.
 //   * Stream: the tiles of all rows and heads are one sequence, cut into equal shares for two CTAs an SM whatever the
-//     rows' lengths; a CTA leaves (M, l, O) in fp32 of a unit that it shares, and a second kernel joins them.
+//     rows' lengths; a CTA leaves (M, l, R, O) in fp32 of a unit that it shares, and a second kernel joins them.
 //
 // An e4m3 row is code * 2^e. For keys 2^e joins the logit's scale. For values it joins the weight's exponent:
 // w_t = 2^(s_t + e_t - M) with M the running maximum of s_t + e_t, so weights are in fp16's range whatever the rows'
 // sizes, and l sums w_t * 2^-e_t. Codes are exact in fp16; queries are scaled by a power of two to
-// [2^14, 2^15), where fp16 holds a bf16 row to 2^-40 of its largest value; a weight is rounded once to 11 bits (2^-11 of
-// it at most, 1/8 of what rounding the output to bf16 costs). With a bf16 cache a weight goes to the tensor cores
-// as a bf16 pair, high and low part: 16 bits.
+// [2^14, 2^15), where fp16 holds a bf16 row to 2^-39 of its largest value; a weight is rounded once to 11 bits, 2^-11 of
+// it (1/8 of what rounding the output to bf16 costs), or, under 2^-20 of the row's largest weight, to 2^-31 of that one. With
+// a bf16 cache a weight goes to the tensor cores as a bf16 pair, high and low part: 16 bits.
 //
 // l in terms of M can be anything from 2^-113 (one token at exponent 119) to 2^155 (2^31 tokens at -110, all just under the
 // slack), more than 32 bits hold. So a warp sums w_t * 2^(e - e_t), e the exponent of the first row that it sees, while no other is

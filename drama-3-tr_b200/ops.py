@@ -826,7 +826,8 @@ def paged_attention(q: Tensor, k_cache: Tensor, v_cache: Tensor, k_exp: Optional
     max(0, n - window) <= t < n of its row, n = lengths[r] with the new token already written (window 0: all
     of them); query head h reads cache head h // (q_heads // kv_heads); scale defaults to dim ** -0.5.
     Returns (out bf16 [rows, q_heads, dim], lse fp32 [rows, q_heads], the natural log of the sum of exp).
-    A row that sees nothing gives zeros and -inf. The launch is laid out for the table's width, so a
+    A row that sees nothing gives zeros and -inf; a logit of -inf is a token that is not seen, one of +inf or NaN
+    makes its head's out and lse NaN. The launch is laid out for the table's width, so a
     narrower view of it (table[:, :n]) makes a shorter call."""
     return _route(_paged_attention, _paged_attention_op, q, k_cache, v_cache)(
         q, k_cache, v_cache, k_exp, v_exp, table, lengths, status, scale, window)

@@ -426,7 +426,11 @@ size_t dm3_paged_attention_workspace_bytes(int rows, int q_heads, int kv_heads, 
 /*
  * One new token's attention for every row: out[r, h] = sum_t p_t v_t with p = softmax(scale * q[r, h] . k_t)
  * over max(0, n - window) <= t < n = lengths[r] (window 0: all), query head h reading cache head
- * h / (q_heads / kv_heads); lse[r, h] = log sum exp. A row that sees nothing gives zeros and -inf.
+ * h / (q_heads / kv_heads); lse[r, h] = log sum exp. A row that sees nothing gives zeros and -inf; a logit of
+ * -inf is a token that is not seen, one of +inf or NaN makes its head's out and lse NaN.
+ * Sums are held in 32 bits or more. A bf16 cache's weights p_t are rounded to 16 bits. A quantised one's, p_t * 2^exp_t, are
+ * rounded to 11 bits, and those under 2^-20 of the row's largest to 2^-31 of it. Equal inputs give equal bits, whatever lies in
+ * places that are not seen.
  *   q    bf16 [rows, q_heads, dim], row stride q_rs and head stride q_hs (16-byte aligned rows)
  *   out  bf16 [rows, q_heads, dim]; lse fp32 [rows, q_heads]
  *   workspace  dm3_paged_attention_workspace_bytes (may be 0), 256-byte aligned, not shared by calls that may overlap

@@ -520,3 +520,65 @@ def test_sums_at_the_ends_of_the_exponents(dm3, tokens, rows, capacity, low, hig
     d["v_exp"] = (e - max(low, high)).clamp(min=-128).to(torch.int8)
     few = {**d, "table": table[:2], "lengths": d["lengths"][:2]}
     check_attention(out[:2].double() * 2.0 ** -max(low, high), lse[:2], few, q[:2], 1.0)
+
+
+@pytest.mark.parametrize("lengths", [[70, 90, 30], [3000, 40, 2000], [90] * 300])
+def test_infinite_logits(dm3, lengths):
+    """A logit of -inf is a token that is not seen, a row of them a row that sees nothing; one of +inf makes its head's out and lse NaN."""
+    d = paged(lengths, 1, 64, 16, False, 5)
+    q = _q(len(lengths), 4, 64, 6, 0.1)
+    q[:, :, 3] = torch.tensor([1.0, -1.0, 0.5, -2.0]).to(BF)
+    at = lambda r, t: (int(d["table"][r, t // 16]), 0, t % 16)  # noqa: E731
+    for t in range(lengths[0]):
+        d["k"][at(0, t)][3] = -math.inf  # heads 0 and 2 of row 0 see nothing, 1 and 3 are infinite
+    d["k"][at(1, 25)][3] = -math.inf  # of row 1, heads 0 and 2 see one token less
+    dev = to_cuda(d)
+    out, lse = dm3.ops.paged_attention(q.cuda(), *held(dev), dev["table"], dev["lengths"], dev["status"])
+    assert out[:2, 1::2].isnan().all() and lse[:2, 1::2].isnan().all()
+    assert (out[0, ::2] == 0).all() and (lse[0, ::2] == -math.inf).all()
+    # the rest against the oracle, the token left out by its page: a copy of row 1 without it
+    n = lengths[1]
+    k, _ = kv_oracle.tokens(d["k"], None, d["table"], 1, n)
+    v, _ = kv_oracle.tokens(d["v"], None, d["table"], 1, n)
+    keep = torch.arange(n) != 25
+    for h in (0, 2):
+        s = q[1, h].double() @ k[0, keep].T * 64 ** -0.5
+        want = s.softmax(-1) @ v[0, keep]
+        spread = s.softmax(-1) @ v[0, keep].abs()
+        assert ((out[1, h].double().cpu() - want).abs() <= want.abs() * 2.0**-8 + spread * 2.0**-10).all()
+        assert abs(float(lse[1, h]) - float(s.logsumexp(-1))) < 1e-4
+    rest = {**d, "table": d["table"][2:], "lengths": d["lengths"][2:]}
+    check_attention(out[2:], lse[2:], rest, q[2:])
+
+
+@pytest.mark.parametrize("above", [0, 12, 24, 33, 60])
+@pytest.mark.parametrize("lengths", [[200, 50], [20000, 300], [400] * 300])
+def test_value_rows_beside_a_larger_one(dm3, above, lengths):
+    """One value row 2^above times the others' size with a single value that is not 0: the other values of out come from the
+    other rows alone. A weight is held to 2^-11 of it, or to 2^-31 of the row's largest (the last places of fp16 below a
+    weight that is 2^6 at least): that bounds each of out's values."""
+    dim = 64
+    d = paged(lengths, 1, dim, 16, True, 9)
+    q = _q(len(lengths), 4, dim, 2, 0.3)
+    few = min(len(lengths), 3)
+    for r in range(len(lengths)):
+        at = (int(d["table"][r, 1]), 0, 4)
+        d["v"].view(torch.uint8)[at] = 0
+        d["v"][at][5] = 256.0
+        d["v_exp"][at] = above
+    out, lse = _run(dm3, d, q)
+    out, lse = out[:few], lse[:few]
+    small = {**d, "table": d["table"][:few], "lengths": d["lengths"][:few]}
+    ref, rlse, spread, reach = kv_oracle.attention(q[:few], *held(small), small["table"], small["lengths"])
+    floor = torch.zeros_like(ref)
+    for r in range(few):
+        n = lengths[r]
+        k, _ = kv_oracle.tokens(d["k"], d["k_exp"], d["table"], r, n)
+        page, at = d["table"][r].long()[torch.arange(n) // 16], torch.arange(n) % 16
+        code, e = d["v"].double()[page, 0, at], d["v_exp"].double()[page, 0, at]
+        p = (q[r].double() @ k[0].T * dim ** -0.5).softmax(-1)
+        floor[r] = (p * torch.exp2(e)).amax(-1, keepdim=True) * 2.0**-31 * code.abs().sum(0)
+    n, logit = max(lengths), reach * (dim / 16 + 4) * 2.0**-22
+    tol = ref.abs() * 2.0**-8 + spread * (2.0**-11 + 2 * logit + (n / 16 + 8) * 2.0**-22)[..., None] + floor
+    assert ((out.double().cpu() - ref).abs() <= tol).all()
+    assert ((lse.double().cpu() - rlse).abs() <= logit + rlse.abs() * 2.0**-22 + (n / 16 + 8) * 2.0**-22).all()
