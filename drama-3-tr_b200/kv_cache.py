@@ -30,7 +30,10 @@ def rope_frequencies(rotary_dim: int, base: float = 10000.0, scaling: Optional[s
     scaling None: base ** (-2i / rotary_dim). "linear": positions compressed by stretch. "ntk": base
     enlarged so that the slowest pair is slowed by stretch and the fastest stays. "yarn": pairs that turn more
     than 32 times over trained_length stay, those that turn less than once are slowed by stretch, a linear
-    ramp between, and the rotated values grow by 0.1 ln(stretch) + 1."""
+    ramp in the number of turns between, and the rotated values grow by 0.1 ln(stretch) + 1. Checkpoints are also
+    trained and served with a ramp that is linear in the pair's index between those two, with other bounds, or
+    with another factor; frequencies in between then differ by tens of percent. Such a model's own frequencies
+    and factor go into a `Rope` as they are."""
     if rotary_dim < 2 or rotary_dim % 2:
         raise ValueError("rotary_dim must be even and at least 2")
     if base <= 0 or stretch < 1:
@@ -53,7 +56,10 @@ def rope_frequencies(rotary_dim: int, base: float = 10000.0, scaling: Optional[s
 
 
 class Rope:
-    """Rotary positions of one kind of head: `rope(x, positions)` turns bf16 [T, heads, dim]."""
+    """Rotary positions of one kind of head: `rope(x, positions)` turns bf16 [T, heads, dim].
+
+    inv_freq (float64 [rotary_dim / 2] on the device) and factor are plain attributes: a model whose frequencies
+    none of the scalings gives sets them after construction."""
 
     def __init__(self, rotary_dim: int, base: float = 10000.0, interleaved: bool = False, scaling: Optional[str] = None,
                  stretch: float = 1.0, trained_length: int = 0, device="cuda"):

@@ -358,3 +358,19 @@ def test_strides_of_sides_of_one(dm3, stub, monkeypatch, quant):
             continue
         with pytest.raises(RuntimeError, match="contiguous"):
             ops.kv_read(*c, *e, t, n, 4, s)
+
+
+def test_frequencies_of_the_callers(dm3, stub, monkeypatch):
+    """A Rope's frequencies and factor can be set: calls and the cache's writes take them."""
+    got = []
+    monkeypatch.setattr(dm3.ops, "_launch", lambda device, name, *a: got.append(a))
+    rope = dm3.Rope(64, scaling="yarn", stretch=4.0, trained_length=100, device="cpu")
+    mine = torch.linspace(1.0, 0.1, 16, dtype=torch.float64)
+    rope.inv_freq, rope.factor = mine, 1.25
+    c = dm3.KVCache(1, 1, 16, 1, 64, device="cpu")
+    x, n = torch.zeros(1, 1, 64, dtype=BF), torch.zeros(1, dtype=torch.int64)
+    rope(x, n)
+    c.write(0, x, x, n, None, x, rope)
+    for a in got:
+        at = a.index(mine.data_ptr())
+        assert a[at + 1] == 32 and a[at + 3] == 1.25
