@@ -185,7 +185,9 @@ struct Shape {
   static constexpr int kSide = (kQuant ? kU * 32 : 0) + kU * 4 + 8 + 4;  // a unit's exponents, ranges and barrier
   static constexpr int kStats = (3 * kWarps + 1 + kMaxCluster) * kHeads * 4;
   // Two CTAs an SM: few warps with much to do at once did better than more of them with smaller steps and fewer
-  // registers (96 ragged rows, 16 heads a cache head, e4m3: 74.6 us; three CTAs and half the step 80.6, four 88.6)
+  // registers (96 ragged rows, 16 heads a cache head, e4m3: 74.6 us; three CTAs and half the step 80.6, four 88.6, all
+  // three before sums held for every exponent; 77.8 now). The two CTAs' 255 registers are not enough for 16 heads of 256
+  // (12 bytes spilled with a bf16 cache, 104 with an e4m3 one).
   static constexpr int kRoom = 112 * 1024 - kQBytes - kStats - 1024;  // 1024: aligning the ring
   static constexpr int kFit = kRoom / kWarps / (kUnit + kSide), kRing = kFit < 6 ? kFit : 6;
   static constexpr int kPitch = 2 * kDim + 8;  // floats of a head pair in the join (8: no bank conflicts)
@@ -1068,10 +1070,12 @@ static int tile_heads(int group) { return group > 8 ? 16 : 8; }
 //   last sums takes 4.5 (one CTA a unit) or 7.5 (a cluster a unit). One CTA a unit leaves the machine idle at the end, 5%,
 //   unless the units are more than run at once and the longest start first, which takes 1.5 (row_by_length). The
 //   stream takes 12 (the count of the rows, and the join's launch).
-// Measured at 1 / 4 / 32 / 128 units (one row, 2 x 2, 8 x 4, 16 x 8) of up to 1,000 tokens: one CTA a unit 19.8 / 19.8 /
-// 12.3 / 15.5 us, clusters 10.0 / 10.1 / 8.5 / -, stream 10.4 / 13.5 / 13.8 / 22.4; of up to 8,000: 129 / 129 / 74 / 83,
-// 22.6 / 22.7 / 26 / -, 13.0 / 16.8 / 23.7 / 67 (256-value heads for the first two, else 128; bf16). 512 units (64 x 8) of up
-// to 8,192: one CTA a unit 193, longest first 169, stream 185; of up to 2,000 50.3 and 44.7; of up to 600 21.5 and 22.1.
+// Measured at 1 / 2 / 32 / 128 units (one row, 2 x 1, 8 x 4, 16 x 8) of up to 1,000 tokens: one CTA a unit 20.5 / 20.6 /
+// 12.8 / 15.9 us, clusters 8.2 / 8.4 / 8.6 / -, stream 10.3 / 14.0 / 14.3 / 23.1; of up to 8,000: 133 / 133 / 76 / 84,
+// 22.7 / 22.9 / 26.5 / -, 13.5 / 18.0 / 24.7 / 68 (256-value heads for the first two, else 128; bf16). 512 units (64 x 8) of up
+// to 8,192: one CTA a unit 195, longest first 171, stream 192; of up to 2,000 50.7 and 44.5; of up to 600 21.5 and 22.1.
+// What the rule does not know is lengths: of those 512 units, one row of 8,192 tokens among rows of 200 to 400 takes 82 us by
+// it, where the stream would take 36.
 struct Plan {
   int head_tiles, splits, ctas;  // splits: CTAs of a cluster, 0: stream over `ctas`
   bool longest_first;            // more CTAs than run at once: the long rows' start first

@@ -306,8 +306,9 @@ __device__ __forceinline__ int row_exponent(float amax) {
 
 // As rope_kernel, over the rows of q, then those of k, then those of v; each of the three starts with a warp, so a warp
 // is at one of them at a time. A row belongs to kSeg neighbouring lanes, so the amax of a quantised row is a few
-// shuffles. A quantised key is turned to 2^-46: it is the code of the exactly turned key, whichever call wrote it (in
-// 32 bits about one value in 10^6 would fall on the other side of a code's border).
+// shuffles. A quantised key is turned to 2^-46 by its angle, which is formed in 64 bits (2^-52 of its size): it is the code of
+// the key turned by that, whichever call wrote it (in 32 bits about one value in 10^6 would fall on the other side of a
+// code's border).
 //
 // Loads in flight: the next row's while a thread is at one, in four CTAs an SM; or (kMany) two rows' at a time in five.
 // With a bf16 cache the second is faster for many tokens and slower for few (written and read back: 100,000 tokens with

@@ -232,8 +232,9 @@ int dm3_moe_noalloc_status(uint32_t* status, void* stream);
  * current device, in nanoseconds; 1 s by default. A wait that runs out sets STATUS_TIMEOUT in the
  * status word and the kernel stops its work uniformly. Call while no kernel of this library runs
  * on the device. The reference has no device-side waits; this exists for failure detection.
- * Below 1,000 ns dm3_paged_attention does not wait at all: what has not landed has run out. Whatever
- * the limit, it ends only once its copies have landed (or 1 s for each has passed).
+ * Below 1,000 ns dm3_paged_attention does not wait at all: what has not landed has run out (a call that
+ * a graph captured keeps to what the limit was then). Whatever the limit, it ends only once its copies
+ * have landed (or 1 s for each has passed).
  */
 int dm3_set_wait_limit_ns(uint64_t ns);
 
