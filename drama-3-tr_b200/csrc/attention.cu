@@ -34,6 +34,7 @@
 // [2^14, 2^15), where fp16 holds a bf16 row to 2^-39 of its largest value; a weight is rounded once to 11 bits, 2^-11 of
 // it (1/8 of what rounding the output to bf16 costs), or, under 2^-20 of the row's largest weight, to 2^-31 of that one. With
 // a bf16 cache a weight goes to the tensor cores as a bf16 pair, high and low part: 16 bits.
+// s_t + e_t is held in 32 bits: where exponents lie over 64 lse is off by up to 2^-17 for it.
 //
 // l in terms of M can be anything from 2^-113 (one token at exponent 119) to 2^155 (2^31 tokens at -110, all just under the
 // slack), more than 32 bits hold. So a warp sums w_t * 2^(e - e_t), e the exponent of the first row that it sees, while no other is
@@ -78,7 +79,7 @@ struct Params {
   int64_t window;
   int splits;          // CTAs of a cluster; 0: stream
   bool longest_first;  // one CTA a unit: blockIdx.z counts the rows by their tiles
-  bool hasty;          // the wait limit is below kHasty: what has not landed when it is needed has run out
+  int hasty;           // the wait limit is below kHasty: what has not landed when it is needed has run out
   __nv_bfloat16* out;  // [rows][q_heads][dim]
   float* lse;          // [rows][q_heads]
   // stream: the first tile of each row in the sequence and their number ([rows + 1], a tile counted once a head unit),
@@ -186,7 +187,7 @@ struct Shape {
   static constexpr int kStats = (3 * kWarps + 1 + kMaxCluster) * kHeads * 4;
   // Two CTAs an SM: few warps with much to do at once did better than more of them with smaller steps and fewer
   // registers (96 ragged rows, 16 heads a cache head, e4m3: 74.6 us; three CTAs and half the step 80.6, four 88.6, all
-  // three before sums held for every exponent; 77.8 now). The two CTAs' 255 registers are not enough for 16 heads of 256
+  // three before sums held for every exponent; 77.0 now). The two CTAs' 255 registers are not enough for 16 heads of 256
   // (12 bytes spilled with a bf16 cache, 104 with an e4m3 one).
   static constexpr int kRoom = 112 * 1024 - kQBytes - kStats - 1024;  // 1024: aligning the ring
   static constexpr int kFit = kRoom / kWarps / (kUnit + kSide), kRing = kFit < 6 ? kFit : 6;
@@ -580,7 +581,8 @@ __global__ void __launch_bounds__(kWarps * 32, 2)
     auto next_slot = [&] {
       if (++slot == C::kRing) slot = 0, parity ^= 1;
     };
-    auto landed = [&] { return __all_sync(0xffffffffu, p.hasty ? mbar_test(&full[slot], parity) : mbar_wait(&full[slot], parity)); };
+    // (a test before the wait: 96 ragged e4m3 rows, 16 heads a cache head, 77.0 against 78.3 us)
+    auto landed = [&] { return __all_sync(0xffffffffu, mbar_test(&full[slot], parity) || (!p.hasty && mbar_wait(&full[slot], parity))); };
     int stuck = -1;  // the unit (a step's keys or its values) whose wait ran out: the segment ends there
     for (int step = 0; step < steps; ++step) {
       if (!landed()) {
